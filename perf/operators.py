@@ -394,7 +394,7 @@ def _verify_own(s):
 
     if "call" not in s:
         case, draft, size = s["case"], s["draft"], C.c_size_t()
-        args = capi.VerifyArgs(precision={"f16": capi.LOGITS_F16, "bf16": capi.LOGITS_BF16, "f32": capi.LOGITS_F32}[case["type"]], n_seqs=case["seqs"], rows=s["total"], max_rows=case["rows"],
+        args = capi.VerifyArgs(precision={"f16": capi.LOGITS_F16, "bf16": capi.LOGITS_BF16, "f32": capi.LOGITS_F32}[case["type"]], n_seqs=case["seqs"], rows=s["total"],
                                vocab=case["vocab"], target_stride=s["target"].stride(0), row_start=s["row_start"].data_ptr(), target=s["target"].data_ptr(), tokens=s["tokens"].data_ptr(),
                                temperature=s["temperature"].data_ptr(), random=s["random"].data_ptr(), out_tokens=s["out"].data_ptr(), accepted=s["accepted"].data_ptr())
         if draft is not None:
