@@ -820,6 +820,90 @@ SMELT_CUDA_API smelt_status smelt_cuda_prefill(smelt_cuda_ctx* ctx, const smelt_
                                                const int32_t* tokens, int n_tokens, int32_t start_pos, int chunk,
                                                int32_t* out_token);
 
+/* ── a batch over a paged cache, and drafted tokens (no reference counterpart) ──
+ * What a server needs to step sequences of different lengths together, some of them with drafted tokens to check.
+ * A cache is two pools of pages: page p holds page_size tokens of every key head; the head_dim values of a token and head are
+ * adjacent, and page_stride, head_stride and token_stride (in values, multiples of 8) say where the next one lies, so pages may
+ * have their heads or their tokens outermost.
+ * A batch is packed: the rows of sequence s are row_start[s] .. row_start[s + 1] - 1 (row_start[0] = 0; rows past
+ * row_start[n_seqs] are not touched); length[s] counts the tokens on its own pages, this call's rows included, so that row i of n is
+ * its token length[s] - n + i, and token t lies in place t % page_size of page table[s table_stride + t / page_size].  All sequences
+ * may share a prefix of prefix_length tokens on the pages prefix_table lists: it comes first, and token t of a sequence is at
+ * position prefix_length + t.  A sequence may have no rows or no tokens.  Lengths, starts and tables are read on the device, so that a
+ * captured call follows them; they are cut to what the arrays can hold.  A page id outside the pool is not followed: nothing is written, its tokens
+ * read as zeros, and bit 16 of the device error word is set (smelt_cuda_device_error then returns SMELT_ERR_OUT_OF_RANGE). */
+enum { SMELT_PAGED_F16 = 0, SMELT_PAGED_BF16 = 1 };
+typedef struct {
+    int32_t precision;           /* of the pools, the queries and the outputs: SMELT_PAGED_* */
+    int32_t n_q, n_kv, head_dim; /* query heads a multiple of key heads; head_dim 64, 128 or 256 */
+    int32_t page_size, n_pages;
+    int64_t page_stride, head_stride, token_stride;
+    void *k, *v;                 /* device, 16-byte aligned */
+} smelt_paged_cache;
+typedef struct {
+    int32_t n_seqs, rows;        /* rows: what the row arrays hold */
+    int32_t max_rows;            /* the most rows of one sequence, as far as the host knows: decides how the work is cut, not what is computed */
+    int32_t table_stride;        /* pages a row of the table holds */
+    int32_t prefix_length;
+    const void *row_start, *length, *table, *prefix_table; /* device, int32: [n_seqs + 1], [n_seqs], [n_seqs, table_stride], [prefix pages] */
+} smelt_paged_batch;
+enum { SMELT_ROPE_ADJACENT = 0, SMELT_ROPE_HALVES = 1 }; /* which values turn together: 2 i and 2 i + 1, or i and i + rope_dim / 2 */
+typedef struct {
+    int32_t rope_dim;            /* the first rope_dim values of a head are rotated (even, 0: none) */
+    int32_t layout;
+    float factor;                /* of sine and cosine (1 where positions are not scaled) */
+    const void* freq;            /* device, double [rope_dim / 2]: radians per position */
+    const void* position;        /* device, int32 [rows]: positions of the rows; null: those of the batch */
+} smelt_rope_desc;
+/* Frequencies of the pairs, for positions past those a model was made for; host only.  PLAIN: theta^(-2 i / rope_dim).  LINEAR:
+ * over factor.  BASE: theta factor^(rope_dim / (rope_dim - 2)) in the place of theta.  RAMP: pairs that turn over fast_turns times in
+ * known_positions stay, those that turn less than slow_turns times are divided by factor, between them a ramp over the pairs' indices
+ * (out_factor 0.1 ln(factor) + 1).  BANDS: the same with a ramp over the turns (out_factor 1).  out_factor may be null. */
+enum { SMELT_ROPE_PLAIN = 0, SMELT_ROPE_LINEAR = 1, SMELT_ROPE_BASE = 2, SMELT_ROPE_RAMP = 3, SMELT_ROPE_BANDS = 4 };
+typedef struct {
+    int32_t rope_dim, kind;
+    double theta, factor, known_positions, slow_turns, fast_turns;
+} smelt_rope_scaling;
+SMELT_CUDA_API smelt_status smelt_cuda_rope_frequencies(const smelt_rope_scaling* scaling, double* out_freq, float* out_factor);
+/* The batch's new rows: queries (null: none) rotated into q_out (may be q), keys rotated and values as they are onto the pages.
+ * Rows of n_q (n_kv) heads lie q_stride (...) values apart: multiples of 8, 16-byte aligned, so that they may be parts of one
+ * row of projections.  rope null: no rotation. */
+SMELT_CUDA_API smelt_status smelt_cuda_paged_append(smelt_cuda_ctx* ctx, const smelt_paged_cache* cache, const smelt_paged_batch* batch,
+                                                    const smelt_rope_desc* rope, const void* q_dev, int64_t q_stride, const void* k_dev,
+                                                    int64_t k_stride, const void* v_dev, int64_t v_stride, void* q_out_dev, int64_t q_out_stride);
+/* Attention of the batch's rows over the prefix and the sequences' own pages: row i of n of a sequence sees the positions up to
+ * its own, with a window (0: none) the last `window` of them.  A row that sees nothing
+ * (a sequence with more rows than tokens) gets zeros.  out may be q.  The prefix is read once for all
+ * sequences.  At most 1024 sequences.  The workspace (smelt_cuda_paged_attention_workspace bytes, 16-byte aligned) holds partial sums
+ * during the call; its contents need no preparation; calls that may run at the same time need one each. */
+SMELT_CUDA_API smelt_status smelt_cuda_paged_attention_workspace(smelt_cuda_ctx* ctx, const smelt_paged_cache* cache,
+                                                                 const smelt_paged_batch* batch, size_t* out_bytes);
+SMELT_CUDA_API smelt_status smelt_cuda_paged_attention(smelt_cuda_ctx* ctx, const smelt_paged_cache* cache, const smelt_paged_batch* batch,
+                                                       const void* q_dev, int64_t q_stride, void* out_dev, int64_t out_stride, float scale,
+                                                       uint32_t window, void* workspace_dev, size_t workspace_bytes);
+/* Drafted tokens against the target.  Packed rows as above: the target read tokens[row_start[s] ..] (the last token that is
+ * certain, then the drafts) and left logits for every row.  With p = softmax(target / T) and q = softmax(draft / T): draft j (token
+ * x = tokens[row_start[s] + 1 + j], judged by target row j and the draft model's row (s, j)) stands while
+ * random[row_start[s] + j] q(x) < p(x).  The token behind the drafts that stand is drawn from max(p - q, 0) of the
+ * first that falls (from p where that leaves nothing), or from p of the last row: the first index whose running sum passes
+ * random[row_start[s + 1] - 1] times the whole.  Without draft logits (null) a draft counts as certain: q(x) = 1.
+ * T = temperature[s] (null: 1); 0 or less takes the lowest index of the largest logit and accepts drafts that are it.
+ * Logits of -inf or NaN have no chance; a drafted id outside the vocabulary falls.
+ * Leaves out_tokens[row_start[s] + i] = the accepted drafts, the drawn token (-1 where no token has a chance), then -1, and accepted[s]. */
+enum { SMELT_LOGITS_F16 = 0, SMELT_LOGITS_BF16 = 1, SMELT_LOGITS_F32 = 2 };
+typedef struct {
+    int32_t precision;           /* of both logits: SMELT_LOGITS_* */
+    int32_t n_seqs, rows, vocab;
+    int64_t target_stride, draft_step_stride, draft_seq_stride; /* values: from row to row; from step to step, from sequence to sequence */
+    const void *row_start, *target, *draft, *tokens;            /* device; int32 [n_seqs + 1], [rows, vocab], null or [steps, n_seqs, vocab], int32 [rows] */
+    const void *temperature, *random;                           /* device; fp32 [n_seqs] or null, fp32 [rows] in [0, 1) */
+    void *out_tokens, *accepted;                                /* device; int32 [rows] (not `tokens`), int32 [n_seqs] */
+    void* workspace;                                            /* device, 16-byte aligned, for this call alone */
+    size_t workspace_bytes;
+} smelt_verify_args;
+SMELT_CUDA_API smelt_status smelt_cuda_verify_drafts_workspace(smelt_cuda_ctx* ctx, const smelt_verify_args* args, size_t* out_bytes);
+SMELT_CUDA_API smelt_status smelt_cuda_verify_drafts(smelt_cuda_ctx* ctx, const smelt_verify_args* args);
+
 /* ── signed activation bit-planes (the Bonsai low-bit path) ──────────────────
  * Producers (Resources/Shaders/signed_quant.metal:751-932): per group of 128 activations one fp16
  * scale and a symmetric integer of n_planes bits as magnitude planes + a sign plane:

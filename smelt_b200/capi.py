@@ -160,6 +160,49 @@ class MoeArgs(C.Structure):
                 + [(n, C.c_void_p) for n in ("logits", "h", "up", "down", "chosen", "place", "table", "permuted", "inner", "rows", "y")])
 
 
+class PagedCache(C.Structure):
+    """``smelt_paged_cache``: two pools of pages."""
+    _fields_ = ([(n, C.c_int32) for n in ("precision", "n_q", "n_kv", "head_dim", "page_size", "n_pages")] + [(n, C.c_int64) for n in ("page_stride", "head_stride", "token_stride")]
+                + [("k", C.c_void_p), ("v", C.c_void_p)])
+
+
+class PagedBatch(C.Structure):
+    """``smelt_paged_batch``: a packed batch of sequences."""
+    _fields_ = [(n, C.c_int32) for n in ("n_seqs", "rows", "max_rows", "table_stride", "prefix_length")] + [(n, C.c_void_p) for n in ("row_start", "length", "table", "prefix_table")]
+
+
+class RopeDesc(C.Structure):
+    """``smelt_rope_desc``."""
+    _fields_ = [("rope_dim", C.c_int32), ("layout", C.c_int32), ("factor", C.c_float), ("freq", C.c_void_p), ("position", C.c_void_p)]
+
+
+class RopeScaling(C.Structure):
+    """``smelt_rope_scaling``."""
+    _fields_ = [("rope_dim", C.c_int32), ("kind", C.c_int32)] + [(n, C.c_double) for n in ("theta", "factor", "known_positions", "slow_turns", "fast_turns")]
+
+
+class VerifyArgs(C.Structure):
+    """``smelt_verify_args``."""
+    _fields_ = ([(n, C.c_int32) for n in ("precision", "n_seqs", "rows", "vocab")] + [(n, C.c_int64) for n in ("target_stride", "draft_step_stride", "draft_seq_stride")]
+                + [(n, C.c_void_p) for n in ("row_start", "target", "draft", "tokens", "temperature", "random", "out_tokens", "accepted", "workspace")] + [("workspace_bytes", C.c_size_t)])
+
+
+PAGED_F16, PAGED_BF16 = 0, 1
+ROPE_ADJACENT, ROPE_HALVES = 0, 1
+ROPE_PLAIN, ROPE_LINEAR, ROPE_BASE, ROPE_RAMP, ROPE_BANDS = range(5)
+LOGITS_F16, LOGITS_BF16, LOGITS_F32 = range(3)
+
+
+def rope_frequencies(rope_dim: int, theta: float, kind: int = ROPE_PLAIN, factor: float = 1.0, known_positions: float = 0.0, slow_turns: float = 1.0, fast_turns: float = 32.0):
+    """Radians per position of each pair (float64) and the factor of sine and cosine (``smelt_cuda_rope_frequencies``)."""
+    freq, scale = np.empty(max(rope_dim // 2, 1), np.float64), C.c_float()
+    args = RopeScaling(rope_dim, kind, theta, factor, known_positions, slow_turns, fast_turns)
+    status = load().smelt_cuda_rope_frequencies(C.byref(args), freq.ctypes.data_as(C.c_void_p), C.byref(scale))
+    if status:
+        raise SmeltError(status, "rope_frequencies: bad scaling")
+    return freq, scale.value
+
+
 class PackageOptions(C.Structure):
     _fields_ = [("context_capacity", C.c_uint32), ("context_limit", C.c_uint32)]
 
@@ -202,7 +245,7 @@ def _ctype_of(param: str):
         return C.c_char_p if param.startswith("const char") else C.c_void_p  # char* out buffers stay void*
     t = param.rsplit(" ", 1)[0].replace("const ", "").strip()
     return {"int": C.c_int, "int32_t": C.c_int32, "uint32_t": C.c_uint32, "size_t": C.c_size_t, "float": C.c_float,
-            "uint64_t": C.c_uint64}[t]
+            "uint64_t": C.c_uint64, "int64_t": C.c_int64}[t]
 
 
 _lib = None
@@ -326,7 +369,7 @@ class Context:
         """The device error word, read and cleared, without raising when it is non-zero."""
         flags = C.c_uint32(0)
         st = self.lib.smelt_cuda_device_error(self.h, C.byref(flags))
-        if st not in (OK, DEVICE_TIMEOUT):
+        if st not in (OK, OUT_OF_RANGE, DEVICE_TIMEOUT):
             self._check(st)
         return flags.value
 
