@@ -65,7 +65,7 @@ cudaError_t launch_paged_append(const Launch& l, PagedType type, int head_dim, c
 // shares with others, one at each end.  Lengths are read on the device, so that a captured call follows them.
 struct PagedLine {
     int columns, keys, ctas;
-    int with_prefix, with_own;
+    int with_prefix, with_own, wide;
     int64_t* cum;     // [n_seqs + 3] written by CTA 0: steps before each source, and the first prefix key that any row sees
     float* slot_o;    // [2 ctas][columns][D] weighted sums of items shared by several CTAs
     float2* slot_ml;  // [2 ctas][columns] their running maxima and sums
@@ -82,9 +82,14 @@ struct PagedAttentionArgs {
     float scale2;  // scale log2(e)
     uint32_t window;
 };
-int paged_narrow_columns(int head_dim, int columns);  // columns of a block of the streaming kernel, 0 where it has none as wide
+int paged_narrow_columns(int head_dim, int64_t columns);  // columns of a block of the streaming kernel for so many of a source
 int paged_narrow_keys(int head_dim);
 cudaError_t launch_paged_narrow(const Launch& l, PagedType type, int head_dim, const PagedAttentionArgs& a, int line);
+// The tensor-core kernel (paged_wide.cu) and whether its shared memory holds a batch of n_seqs.
+int paged_wide_columns(int head_dim);
+int paged_wide_keys(int head_dim);
+bool paged_wide_takes(int head_dim, int n_seqs);
+cudaError_t launch_paged_wide(const Launch& l, PagedType type, int head_dim, const PagedAttentionArgs& a, int line);
 cudaError_t launch_paged_merge(const Launch& l, PagedType type, int head_dim, const PagedAttentionArgs& a);
 
 // Drafted tokens against the target (verify.cu).

@@ -62,18 +62,34 @@ size_t attention_plan(const smelt_cuda_ctx* ctx, const smelt_paged_cache* k, con
         at += (bytes + 15) & ~(size_t)15;
         return p;
     };
+    // Columns of a source: up to 32 on the streaming kernel (16 with heads of 256), more on the tensor core.  A launch takes sequences and
+    // prefix together where they go to the same kernel.
     const int64_t own = (int64_t)(b->max_rows > 0 ? b->max_rows : 1) * a->c.ratio, prefix = b->prefix_length > 0 ? (int64_t)b->rows * a->c.ratio : 0;
-    const int64_t most = own > prefix ? own : prefix;
-    a->lines = 1;
-    PagedLine& line = a->line[0];
-    line.columns = paged_narrow_columns(D, (int)(most < 1000 ? most : 1000));
-    line.keys = paged_narrow_keys(D);
-    line.ctas = ctx->sm_count;
-    line.with_own = 1;
-    line.with_prefix = b->prefix_length > 0;
-    line.cum = (int64_t*)room((size_t)(b->n_seqs + 3) * sizeof(int64_t));
-    line.slot_o = (float*)room((size_t)2 * line.ctas * line.columns * D * sizeof(float));
-    line.slot_ml = (float2*)room((size_t)2 * line.ctas * line.columns * sizeof(float2));
+    const bool can = paged_wide_takes(D, b->n_seqs);
+    const int64_t most = D == 256 ? 16 : 32;
+    const bool own_wide = can && own > most, prefix_wide = can && prefix > most;
+    a->lines = 0;
+    auto add = [&](bool wide, bool with_own, bool with_prefix) {
+        PagedLine& line = a->line[a->lines++];
+        line.wide = wide;
+        line.with_own = with_own;
+        line.with_prefix = with_prefix;
+        const int64_t columns = with_own && with_prefix ? (own > prefix ? own : prefix) : with_own ? own : prefix;
+        line.columns = wide ? paged_wide_columns(D) : paged_narrow_columns(D, columns);
+        line.keys = wide ? paged_wide_keys(D) : paged_narrow_keys(D);
+        line.ctas = ctx->sm_count;
+        line.cum = (int64_t*)room((size_t)(b->n_seqs + 3) * sizeof(int64_t));
+        line.slot_o = (float*)room((size_t)2 * line.ctas * line.columns * D * sizeof(float));
+        line.slot_ml = (float2*)room((size_t)2 * line.ctas * line.columns * sizeof(float2));
+    };
+    if (prefix == 0) {
+        add(own_wide, true, false);
+    } else if (own_wide == prefix_wide) {
+        add(own_wide, true, true);
+    } else {
+        add(prefix_wide, false, true);
+        add(own_wide, true, false);
+    }
     if (b->prefix_length > 0) {
         a->whole_o = (float*)room((size_t)2 * b->rows * k->n_q * D * sizeof(float));
         a->whole_ml = (float2*)room((size_t)2 * b->rows * k->n_q * sizeof(float2));
@@ -174,7 +190,8 @@ smelt_status smelt_cuda_paged_attention(smelt_cuda_ctx* ctx, const smelt_paged_c
     a.q = q; a.out = out; a.q_stride = q_stride; a.out_stride = out_stride;
     a.scale2 = scale * 1.4426950408889634f;
     a.window = window;
-    cudaError_t e = launch_paged_narrow(l, (PagedType)cache->precision, cache->head_dim, a, 0);
+    cudaError_t e = cudaSuccess;
+    for (int i = 0; i < a.lines && e == cudaSuccess; ++i) e = (a.line[i].wide ? launch_paged_wide : launch_paged_narrow)(l, (PagedType)cache->precision, cache->head_dim, a, i);
     if (e == cudaSuccess) e = launch_paged_merge(l, (PagedType)cache->precision, cache->head_dim, a);
     return check_cuda(ctx, e, "paged attention");
 }

@@ -48,13 +48,19 @@ template <class E> __device__ __forceinline__ bool pair_not_finite(uint32_t v) {
 
 // O^T += V^T P^T where some value is not finite and not every column sees every key: column by column, with the rows that it does not
 // see taken as zero.
+template <int D, int NH>
+struct MaskedTile {
+    float o[NH][D / 16][4];
+    uint32_t p[NH][4];
+    Range keys[NH][2];
+};
 template <int D, int NH, class E>
-__device__ __noinline__ void weighted_sum_masked(const unsigned char* vu, float (&o)[NH][D / 16][4], const uint32_t (&pb)[NH][4], const Range (&keys)[NH][2], int k0, int t) {
+__device__ __noinline__ void weighted_sum_masked(const unsigned char* vu, MaskedTile<D, NH>& m, int k0, int t) {
     constexpr int VC = D / 64;
     for (int nh = 0; nh < NH; ++nh)
         for (int col = 0; col < 8; ++col) {
             const int from = (threadIdx.x & 28) | (col >> 1);
-            const int lo = __shfl_sync(0xffffffffu, col & 1 ? keys[nh][1].lo : keys[nh][0].lo, from), hi = __shfl_sync(0xffffffffu, col & 1 ? keys[nh][1].hi : keys[nh][0].hi, from);
+            const int lo = __shfl_sync(0xffffffffu, m.keys[nh][col & 1].lo, from), hi = __shfl_sync(0xffffffffu, m.keys[nh][col & 1].hi, from);
             uint32_t keep[4];
             const int mine[4] = {k0 + 2 * t, k0 + 2 * t + 1, k0 + 2 * t + 8, k0 + 2 * t + 9};
             for (int i = 0; i < 4; ++i) keep[i] = mine[i] >= lo && mine[i] < hi ? 0xffffffffu : 0u;
@@ -68,9 +74,9 @@ __device__ __noinline__ void weighted_sum_masked(const unsigned char* vu, float 
                     float add[4] = {0.f, 0.f, 0.f, 0.f};
                     const uint32_t a0 = __byte_perm(r[0][e], r[1][e], 0x5410), a1 = __byte_perm(r[0][e], r[1][e], 0x7632);
                     const uint32_t a2 = __byte_perm(r[2][e], r[3][e], 0x5410), a3 = __byte_perm(r[2][e], r[3][e], 0x7632);
-                    TileElem<E>::mma(add, a0, a1, a2, a3, pb[nh][0], pb[nh][1]);
-                    TileElem<E>::mma(add, a0, a1, a2, a3, pb[nh][2], pb[nh][3]);
-                    if ((col >> 1) == t) { o[nh][4 * c + e][col & 1] += add[col & 1]; o[nh][4 * c + e][2 + (col & 1)] += add[2 + (col & 1)]; }
+                    TileElem<E>::mma(add, a0, a1, a2, a3, m.p[nh][0], m.p[nh][1]);
+                    TileElem<E>::mma(add, a0, a1, a2, a3, m.p[nh][2], m.p[nh][3]);
+                    if ((col >> 1) == t) { m.o[nh][4 * c + e][col & 1] += add[col & 1]; m.o[nh][4 * c + e][2 + (col & 1)] += add[2 + (col & 1)]; }
                 }
             }
         }
@@ -274,7 +280,25 @@ __global__ void __launch_bounds__(kWarps<D> * 32, 1) paged_narrow_kernel(const P
                     odd = __any_sync(0xffffffffu, odd);
                 }
                 if (odd) {
-                    weighted_sum_masked<D, NH, E>(vu, o, pb, keys, k0, t);
+                    MaskedTile<D, NH> rare;  // a copy: what is passed by address does not stay in registers
+#pragma unroll
+                    for (int nh = 0; nh < NH; ++nh) {
+                        rare.keys[nh][0] = keys[nh][0];
+                        rare.keys[nh][1] = keys[nh][1];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) rare.p[nh][i] = pb[nh][i];
+#pragma unroll
+                        for (int i = 0; i < MT; ++i)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) rare.o[nh][i][e] = o[nh][i][e];
+                    }
+                    weighted_sum_masked<D, NH, E>(vu, rare, k0, t);
+#pragma unroll
+                    for (int nh = 0; nh < NH; ++nh)
+#pragma unroll
+                        for (int i = 0; i < MT; ++i)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) o[nh][i][e] = rare.o[nh][i][e];
                 } else {
                     uint32_t b0[NH], b1[NH], l0[NH], l1[NH];
 #pragma unroll
@@ -356,6 +380,7 @@ struct Joined {
         for (int i = 0; i < D / 32; ++i) o[i] = 0.f;
     }
     __device__ __forceinline__ void add(const float2 ml, const float* part, int lane) {
+        if (ml.y == 0.f) return;  // sees nothing of the part, whatever its sums are
         float v[D / 32];
 #pragma unroll
         for (int i = 0; i < D / 32; ++i) v[i] = __ldcg(part + lane + 32 * i);
@@ -455,7 +480,7 @@ cudaError_t narrow(const Launch& l, PagedType type, const PagedAttentionArgs& a,
 
 }  // namespace
 
-int paged_narrow_columns(int head_dim, int columns) {
+int paged_narrow_columns(int head_dim, int64_t columns) {
     const int most = head_dim == 256 ? 16 : 32;
     return columns <= 8 ? 8 : columns <= 16 ? 16 : most;
 }

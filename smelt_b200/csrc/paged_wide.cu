@@ -1,0 +1,607 @@
+// Attention over pages for blocks of many columns (prompt chunks, drafts of wide groups, a prefix that a whole batch shares): the
+// products on the fifth-generation tensor core.
+//
+// A block is 256 columns ((row, query head of the group) pairs of one key head; 128 with heads of 256) as two tiles of 128 lanes of tensor memory, a step
+// 128 keys (64).  Roles: four warps copy pages to shared memory (16-byte cp.async a row, so pages may have any size and strides;
+// 128-byte swizzle), one warp issues the products S = Q K^T and O += P V, and two sets of four warps take a tile each: a thread has
+// a column, so the softmax needs no exchange.  P overwrites S in tensor memory and is the product's operand from there.  While one
+// set is at its exponentials (128 x 128 of them take the SM's 16 a clock 1024 clocks) the tensor core works for the other (1024 clocks a
+// tile and step).  A block of 128 columns or fewer gives both sets the same tile and every other step, and their sums are joined at the
+// end.  The maximum that P is relative to moves only when the running one is past it by 2^8 (P stays exact to a rounding: fp16 and bf16
+// hold 2^8 as well as 1), so that O is rescaled a few times an item instead of at every step.
+// P is rounded once to the 16-bit type, the type of the values it is multiplied with; sums are fp32.
+//
+// Value rows that are not finite and that not every column of the step sees are taken out of the product (as zeros) and added
+// for the columns that see them alone, so that nothing reaches a row that it does not see.
+#include <cuda_bf16.h>
+
+#include <type_traits>
+
+#include "paged_line.cuh"
+#include "tcgen05.cuh"
+
+namespace smelt {
+namespace {
+
+using namespace paged;
+
+template <int D>
+struct Cfg {
+    static constexpr int kSets = D == 256 ? 1 : 2;   // of four softmax warps, each with an accumulator of its own
+    static constexpr int kKeys = D == 256 ? 64 : 128;
+    static constexpr int kStages = D == 64 ? 3 : 2;
+    static constexpr int kColumns = kSets * 128;
+    static constexpr int kQTile = 128 * D * 2, kTile = kKeys * D * 2;
+    static constexpr int kLoadWarp = kSets * 4, kMmaWarp = kLoadWarp + 4, kThreads = (kMmaWarp + 1) * 32;
+    static constexpr int kSum = 2 * kKeys;  // first column of the accumulators: behind two of scores
+};
+
+struct Shared {  // behind the tiles
+    uint64_t k_full[3], k_empty[3], v_full[3], v_empty[3], s_full[2], p_ready[2], pv_done[2], q_full, q_empty;
+    uint32_t tmem, dead;
+    uint32_t keep[2];    // the first product of an item adds to what its set has put into the accumulator
+    uint32_t odd[3][4];  // keys of a stage's step whose values are not finite, and were taken out
+    float2 ml[2][128];
+    long long row[128];  // of a step's keys in the pools, in elements (head 0); -1: none
+};
+template <int D>
+constexpr size_t wide_shared(int n_seqs) {
+    return (size_t)Cfg<D>::kSets * Cfg<D>::kQTile + 2 * Cfg<D>::kStages * Cfg<D>::kTile + (Cfg<D>::kSets == 2 ? 128 * 32 * 4 : 0) + ((sizeof(Shared) + 15) & ~(size_t)15) + batch_bytes(n_seqs);
+}
+
+template <class E> struct Pack;
+template <> struct Pack<__half> {
+    static constexpr uint32_t kType = 0u, kInf = 0x7C00u;
+    static __device__ __forceinline__ uint32_t two(float x, float y) { return h2_as_u32(__floats2half2_rn(x, y)); }
+    static __device__ __forceinline__ float one(uint16_t v) { return __half2float(__ushort_as_half(v)); }
+};
+template <> struct Pack<__nv_bfloat16> {
+    static constexpr uint32_t kType = (1u << 7) | (1u << 10), kInf = 0x7F80u;
+    static __device__ __forceinline__ uint32_t two(float x, float y) {
+        const __nv_bfloat162 v = __floats2bfloat162_rn(x, y);
+        return *reinterpret_cast<const uint32_t*>(&v);
+    }
+    static __device__ __forceinline__ float one(uint16_t v) { return __uint_as_float((uint32_t)v << 16); }
+};
+
+__device__ __forceinline__ float exp2_approx(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// K-major operand: smem_desc_sw128 (tcgen05.cuh).  The values of a step are [key][64 values of a head] blocks of 128-byte rows: as the
+// product's second operand that is the other major order, eight keys to an atom of 1024 bytes, the next 64 values one block further.
+__device__ __forceinline__ uint64_t value_desc(uint32_t smem_addr, uint32_t block_bytes) {
+    return (uint64_t)((smem_addr >> 4) & 0x3FFFu) | ((uint64_t)(block_bytes >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+// D[128 x N] (+)= A[128 x 64] . B[64 x N], A from tensor memory, B values: four steps of 16 keys (2048 bytes).
+__device__ __forceinline__ void umma_values_block(uint32_t d, uint32_t a, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p, q, t;\n\t.reg .b32 a1, a2, a3;\n\t.reg .b64 b1, b2, b3;\n\t"
+        "elect.sync _|q, 0xffffffff;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\tsetp.eq.b32 t, 0, 0;\n\t"
+        "add.u32 a1, %1, 8;\n\tadd.u32 a2, %1, 16;\n\tadd.u32 a3, %1, 24;\n\t"
+        "add.u64 b1, %2, 128;\n\tadd.u64 b2, %2, 256;\n\tadd.u64 b3, %2, 384;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [a1], b1, %3, t;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [a2], b2, %3, t;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [a3], b3, %3, t;\n\t}"
+        ::"r"(d), "r"(a), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_ld32(uint32_t t, uint32_t (&v)[32]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]),
+                   "=r"(v[15]), "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]),
+                   "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+                 : "r"(t)
+                 : "memory");
+}
+// The loads behind v have arrived (v is named so that nothing is read of it earlier).
+__device__ __forceinline__ void tmem_wait_ld32(uint32_t (&v)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]), "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]),
+                   "+r"(v[15]), "+r"(v[16]), "+r"(v[17]), "+r"(v[18]), "+r"(v[19]), "+r"(v[20]), "+r"(v[21]), "+r"(v[22]), "+r"(v[23]), "+r"(v[24]), "+r"(v[25]), "+r"(v[26]), "+r"(v[27]), "+r"(v[28]),
+                   "+r"(v[29]), "+r"(v[30]), "+r"(v[31])::"memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t t, const uint32_t (&v)[16]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(t), "r"(v[0]), "r"(v[1]), "r"(v[2]),
+                 "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void barrier(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool take) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(take ? 16 : 0) : "memory");
+}
+template <class E> __device__ __forceinline__ bool word_not_finite(const uint4& w) {
+    constexpr uint32_t m = Pack<E>::kInf;
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+    bool odd = false;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) odd = odd || (u[i] & m) == m || ((u[i] >> 16) & m) == m;
+    return odd;
+}
+
+// What every role knows of an item.
+struct Item {
+    Seq seq;        // of the prefix: all rows
+    int f0, width;  // first column of the block among the source's, and how many it has
+    Range clear;    // keys that every column sees
+};
+__device__ __forceinline__ Item item_of(const PagedArgs& c, const PagedLine& line, uint32_t window, const Batch& b, const Cursor& cur) {
+    Item it;
+    it.seq = cur.source == 0 ? Seq{0, b.row[c.n_seqs], 0} : b.seq(cur.source - 1);
+    it.f0 = cur.block * line.columns;
+    it.width = min(line.columns, it.seq.n * c.ratio - it.f0);
+    // of the prefix: without a window all columns, but for rows without a token, whose sums are dropped
+    it.clear = cur.source ? Range{own_keys(it.seq, (it.f0 + it.width - 1) / c.ratio, window).lo, own_keys(it.seq, it.f0 / c.ratio, window).hi} : window ? Range{0, 0} : Range{0, c.prefix_length};
+    return it;
+}
+
+template <int D, class E>
+__global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_wide_kernel(const PagedAttentionArgs a, const int which) {
+    using C = Cfg<D>;
+    constexpr int KEYS = C::kKeys, S = C::kStages, CHUNKS = D / 8;  // 16-byte chunks of a row
+    extern __shared__ __align__(1024) unsigned char raw[];
+    unsigned char *q_tiles = raw, *k_tiles = q_tiles + C::kSets * C::kQTile, *v_tiles = k_tiles + S * C::kTile;
+    float* joint = reinterpret_cast<float*>(v_tiles + S * C::kTile);  // [128][32] of the set that is added to the other
+    Shared& sh = *reinterpret_cast<Shared*>(reinterpret_cast<unsigned char*>(joint) + (C::kSets == 2 ? 128 * 32 * 4 : 0));
+    const PagedArgs& c = a.c;
+    const PagedLine& line = a.line[which];
+    const int tid = threadIdx.x, warp = uniform(tid >> 5), lane = tid & 31;
+    volatile uint32_t* dead = &sh.dead;
+    if (tid == 0) {
+        for (int i = 0; i < S; ++i) {
+            mbar_init(&sh.k_full[i], 4); mbar_init(&sh.v_full[i], 4);
+            mbar_init(&sh.k_empty[i], 1); mbar_init(&sh.v_empty[i], 1);
+        }
+        for (int i = 0; i < 2; ++i) { mbar_init(&sh.s_full[i], 1); mbar_init(&sh.p_ready[i], 4); mbar_init(&sh.pv_done[i], 1); }
+        mbar_init(&sh.q_full, 4);
+        mbar_init(&sh.q_empty, 1);
+        sh.dead = 0;
+        mbar_fence_init();
+        fence_async_smem();
+    }
+    if (warp == C::kMmaWarp) tmem_alloc(&sh.tmem, 512);
+    tc_fence_before();
+    pdl_trigger();
+    pdl_wait();
+    Batch batch;
+    scan_line<C::kThreads>(c, line, a.window, batch, reinterpret_cast<unsigned char*>(&sh) + ((sizeof(Shared) + 15) & ~(size_t)15));
+    tc_fence_after();
+    const uint32_t tmem = (uint32_t)uniform((int)sh.tmem);
+    const long long total = batch.cum[c.n_seqs + 1];
+    const int ctas = line_ctas(total, line.ctas);
+    const long long begin = (int)blockIdx.x < ctas ? line_begin(total, blockIdx.x, ctas) : 0, end = (int)blockIdx.x < ctas ? line_begin(total, blockIdx.x + 1, ctas) : 0;
+    // A role that gives up a wait goes through the rest of its schedule without work, so that no barrier is short of a thread.
+    bool alive = true;
+    // An item's steps in this CTA: tasks, one a step, or with two tiles one a tile and step; task T of the CTA has score buffer T & 1.
+    auto each_item = [&](auto&& body) {
+        if (begin >= end) return;
+        Cursor cur;
+        cur.seek(c, line, a.window, batch, begin);
+        uint32_t task = 0, step = 0;
+        for (long long pos = begin; pos < end;) {
+            const int n = (int)min((long long)(cur.steps - cur.step), end - pos);
+            const Item it = item_of(c, line, a.window, batch, cur);
+            const bool pair = it.width > 128;
+            const int tasks = pair ? 2 * n : n;
+            body(cur, it, pair, n, tasks, task, step, pos);
+            task += tasks;
+            step += n;
+            pos += n;
+            if (pos < end) {
+                cur.step = cur.steps - 1;
+                cur.advance(c, line, a.window, batch);
+            }
+        }
+    };
+
+    if (warp >= C::kLoadWarp && warp < C::kMmaWarp) {
+        // ── pages to shared memory ──
+        const int lt = tid - C::kLoadWarp * 32;
+        constexpr int LANES = CHUNKS < 32 ? CHUNKS : 32, ROWS = 128 / LANES;  // lanes of a row, rows of a turn of the four warps
+        const int ch = lt % LANES, r_first = lt / LANES;
+        auto place = [](int rows, int row, int chunk) { return (uint32_t)((chunk >> 3) * rows * 128 + row * 128 + (((chunk & 7) ^ (row & 7)) << 4)); };
+        auto warp_wait = [&](uint64_t* bar, uint32_t parity) { alive = __all_sync(0xffffffffu, alive && wait_alive(bar, parity, dead)) != 0; };
+        auto arrive = [&](uint64_t* bar) {
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar);
+        };
+        const uint32_t flip = a.scale2 < 0.f ? 0x80008000u : 0u;  // the softmax wants a positive scale
+        uint32_t items = 0;
+        int v_behind = -1;        // stage of the values that were asked for last and not handed over yet
+        bool v_check = false;     // ... that not every column sees all of
+        auto hand_over_values = [&] {
+            if (v_behind < 0) return;
+            if (v_check) {
+                unsigned char* tile = v_tiles + v_behind * C::kTile;
+                barrier(1, 128);  // the stage's words of odd keys are zero
+                for (int r = r_first; r < KEYS; r += ROWS)
+                    for (int k = ch; k < CHUNKS; k += LANES)
+                        if (word_not_finite<E>(*reinterpret_cast<const uint4*>(tile + place(KEYS, r, k)))) atomicOr(&sh.odd[v_behind][r >> 5], 1u << (r & 31));
+                barrier(1, 128);
+                for (int r = r_first; r < KEYS; r += ROWS)
+                    if (sh.odd[v_behind][r >> 5] >> (r & 31) & 1u)
+                        for (int k = ch; k < CHUNKS; k += LANES) *reinterpret_cast<uint4*>(tile + place(KEYS, r, k)) = make_uint4(0, 0, 0, 0);
+            }
+            arrive(&sh.v_full[v_behind]);
+            v_behind = -1;
+        };
+        each_item([&](const Cursor& cur, const Item& it, bool pair, int n, int, uint32_t, uint32_t step0, long long) {
+            // queries, behind everything that was asked for before them
+            cp_async_wait<0>();
+            hand_over_values();
+            if (items > 0) warp_wait(&sh.q_empty, (items - 1) & 1);
+            ++items;
+            if (alive) {
+                for (int f = r_first; f < (pair ? 256 : 128); f += ROWS)
+                    for (int k = ch; k < CHUNKS; k += LANES) {
+                        uint4 v = make_uint4(0, 0, 0, 0);
+                        if (f < it.width) {
+                            const int ff = it.f0 + f;
+                            v = *reinterpret_cast<const uint4*>(static_cast<const E*>(a.q) + (size_t)(it.seq.row + ff / c.ratio) * a.q_stride + (size_t)(cur.head * c.ratio + ff % c.ratio) * D + 8 * k);
+                            v.x ^= flip; v.y ^= flip; v.z ^= flip; v.w ^= flip;
+                        }
+                        *reinterpret_cast<uint4*>(q_tiles + (f >> 7) * C::kQTile + place(128, f & 127, k)) = v;
+                    }
+            }
+            arrive(&sh.q_full);
+            const int32_t* table = cur.source == 0 ? c.prefix_table : c.table + (size_t)(cur.source - 1) * c.table_stride;
+            const long long head_at = (long long)cur.head * c.head_stride;
+            for (int i = 0; i < n; ++i) {
+                const uint32_t step = step0 + i, s = step % S, use = step / S;
+                const int k0 = (cur.first + cur.step + i) * KEYS;
+                barrier(1, 128);  // the rows of the step before have been read
+                if (lt < KEYS) {
+                    const int key = k0 + lt;
+                    long long at = -1;
+                    if (key >= cur.keys.lo && key < cur.keys.hi) {
+                        const int p = divide(key, c.page_div), page = table[p];
+                        if ((uint32_t)page < (uint32_t)c.n_pages) at = (long long)page * c.page_stride + (long long)(key - p * c.page_size) * c.token_stride + head_at;
+                        else if (c.err) atomicOr(c.err, KERR_BAD_PAGE);
+                    }
+                    sh.row[lt] = at;
+                }
+                barrier(1, 128);
+                auto copy = [&](const void* pool, unsigned char* tiles) {
+                    const uint32_t dst = smem_u32(tiles + s * C::kTile);
+                    if (alive) {
+#pragma unroll 4
+                        for (int r = r_first; r < KEYS; r += ROWS) {
+                            const long long at = sh.row[r];
+                            for (int k = ch; k < CHUNKS; k += LANES) copy16(dst + place(KEYS, r, k), static_cast<const E*>(pool) + max(at, 0ll) + 8 * k, at >= 0);
+                        }
+                    }
+                    cp_async_commit();
+                };
+                if (use > 0) warp_wait(&sh.k_empty[s], (use - 1) & 1);
+                copy(c.k, k_tiles);
+                cp_async_wait<1>();  // the values of the step before have arrived
+                hand_over_values();
+                if (use > 0) warp_wait(&sh.v_empty[s], (use - 1) & 1);
+                if (lt < 4) sh.odd[s][lt] = 0;
+                copy(c.v, v_tiles);
+                cp_async_wait<1>();
+                arrive(&sh.k_full[s]);
+                v_behind = (int)s;
+                v_check = k0 < it.clear.lo || min(k0 + KEYS, cur.keys.hi) > it.clear.hi;
+            }
+        });
+        cp_async_wait<0>();
+        hand_over_values();
+    } else if (warp == C::kMmaWarp) {
+        // ── products ──
+        constexpr uint32_t kScores = (1u << 4) | Pack<E>::kType | ((uint32_t)(KEYS >> 3) << 17) | ((128u >> 4) << 24);
+        constexpr uint32_t kValues = (1u << 4) | Pack<E>::kType | (1u << 16) | ((uint32_t)(D >> 3) << 17) | ((128u >> 4) << 24);
+        const uint64_t q_desc = smem_desc_sw128(smem_u32(q_tiles)), k_desc = smem_desc_sw128(smem_u32(k_tiles)), v_desc = value_desc(smem_u32(v_tiles), KEYS * 128);
+        auto wait = [&](uint64_t* bar, uint32_t parity) {
+            alive = __all_sync(0xffffffffu, alive && wait_alive(bar, parity, dead)) != 0;
+            tc_fence_after();
+        };
+        uint32_t items = 0, done = 0;
+        each_item([&](const Cursor&, const Item&, bool pair, int, int tasks, uint32_t task0, uint32_t step0, long long) {
+            wait(&sh.q_full, items & 1);
+            ++items;
+            auto scores = [&](int t) {
+                const uint32_t b = (task0 + t) & 1, step = step0 + (pair ? t >> 1 : t), s = step % S;
+                const bool first = !pair || !(t & 1), last = !pair || (t & 1);
+                if (first) wait(&sh.k_full[s], (step / S) & 1);
+                if (!alive) return;
+                const uint64_t q = q_desc + (uint64_t)((pair ? t & 1 : 0) * (C::kQTile / 16)), k = k_desc + (uint64_t)(s * (C::kTile / 16));
+#pragma unroll
+                for (int x = 0; x < D / 64; ++x) umma_f16_block(tmem + b * KEYS, q + x * (128 * 128 / 16), k + x * (KEYS * 128 / 16), kScores, x > 0);
+                commit_elected(smem_u32(&sh.s_full[b]));
+                if (last) commit_elected(smem_u32(&sh.k_empty[s]));
+                if (t + 1 == tasks) commit_elected(smem_u32(&sh.q_empty));
+            };
+            scores(0);
+            if (tasks > 1) scores(1);
+#pragma unroll 1
+            for (int t = 0; t < tasks; ++t) {
+                const uint32_t T = task0 + t, b = T & 1, step = step0 + (pair ? t >> 1 : t), s = step % S;
+                const bool first = !pair || !(t & 1), last = !pair || (t & 1);
+                if (first) wait(&sh.v_full[s], (step / S) & 1);
+                wait(&sh.p_ready[b], (T >> 1) & 1);
+                if (alive) {
+                    const uint32_t o = tmem + C::kSum + (C::kSets == 2 ? b * D : 0);
+                    const bool add = t >= C::kSets || *(volatile uint32_t*)&sh.keep[b];
+                    const uint64_t v = v_desc + (uint64_t)(s * (C::kTile / 16));
+#pragma unroll
+                    for (int x = 0; x < KEYS / 64; ++x) umma_values_block(o, tmem + b * KEYS + 32 * x, v + x * (64 * 128 / 16), kValues, x > 0 || add);
+                    commit_elected(smem_u32(&sh.pv_done[b]));
+                    if (last) commit_elected(smem_u32(&sh.v_empty[s]));
+                    done = T + 1;
+                }
+                if (t + 2 < tasks) scores(t + 2);
+            }
+        });
+        // the products in flight read shared memory and write tensor memory
+        if (done > 0) mbar_poll_bounded(&sh.pv_done[(done - 1) & 1], ((done - 1) >> 1) & 1);
+        if (done > 1) mbar_poll_bounded(&sh.pv_done[done & 1], ((done - 2) >> 1) & 1);
+    } else {
+        // ── softmax: a thread a column ──
+        const int set = warp >> 2, me = (warp & 3) * 32 + lane;
+        const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16), o_at = lanes + C::kSum + set * D;
+        const float scale2 = fabsf(a.scale2);
+        auto wait = [&](uint64_t* bar, uint32_t parity) {
+            alive = __all_sync(0xffffffffu, alive && wait_alive(bar, parity, dead)) != 0;
+            tc_fence_after();
+        };
+        each_item([&](const Cursor& cur, const Item& it, bool pair, int n, int tasks, uint32_t task0, uint32_t step0, long long pos) {
+            const int t_first = C::kSets == 1 ? 0 : (int)((task0 & 1) ^ set), f = (pair ? t_first * 128 : 0) + me, ff = it.f0 + f;
+            Range keys = {0, 0};
+            if (f < it.width) {
+                const int i = ff / c.ratio;
+                if (cur.source) {
+                    keys = own_keys(it.seq, i, a.window);
+                } else {
+                    const Seq s = batch.seq(seq_of_row(batch, c.n_seqs, i));
+                    keys = prefix_keys(s, i - s.row, c.prefix_length, a.window);
+                }
+            }
+            const bool blind = __any_sync(0xffffffffu, f < it.width && keys.hi == 0);  // a row of the prefix's block that sees nothing
+            float m = kLowest, l = 0.f;
+            uint32_t last = 0;
+            bool any = false;
+            for (int t = t_first; t < tasks; t += C::kSets) {
+                const uint32_t T = task0 + t, b = T & 1, use = T >> 1, step = step0 + (pair ? t >> 1 : t);
+                const int k0 = (cur.first + cur.step + (pair ? t >> 1 : t)) * KEYS;
+                const bool clear = k0 >= max(it.clear.lo, cur.keys.lo) && k0 + KEYS <= min(it.clear.hi, cur.keys.hi) && !blind;
+                const bool checked = k0 < it.clear.lo || min(k0 + KEYS, cur.keys.hi) > it.clear.hi;
+                const uint32_t s_at = lanes + b * KEYS;
+                wait(&sh.s_full[b], use & 1);
+                if (alive) {
+                    float top = kLowest;
+#pragma unroll
+                    for (int x = 0; x < KEYS; x += 32) {
+                        uint32_t v[32];
+                        tmem_ld32(s_at + x, v);
+                        tmem_wait_ld32(v);
+                        float t0 = kLowest, t1 = kLowest;
+                        if (clear) {
+#pragma unroll
+                            for (int e = 0; e < 32; e += 2) { t0 = fmaxf(t0, __uint_as_float(v[e])); t1 = fmaxf(t1, __uint_as_float(v[e + 1])); }
+                        } else {
+#pragma unroll
+                            for (int e = 0; e < 32; ++e)
+                                if (k0 + x + e >= keys.lo && k0 + x + e < keys.hi) t0 = fmaxf(t0, __uint_as_float(v[e]));
+                        }
+                        top = fmaxf(top, fmaxf(t0, t1));
+                    }
+                    top = top == kLowest ? kLowest : top * scale2;
+                    const bool begun = any;
+                    const bool move = top > m + 8.f || !begun;
+                    if (!begun) {
+                        m = top;
+                    } else if (__any_sync(0xffffffffu, move)) {
+                        const float keep = move ? exp2_approx(m - top) : 1.f;
+                        if (move) m = top;
+                        l *= keep;
+                        wait(&sh.pv_done[last & 1], (last >> 1) & 1);
+                        if (alive) {
+#pragma unroll 1
+                            for (int x = 0; x < D; x += 16) {
+                                uint32_t v[16];
+                                tmem_ld16(o_at + x, v);
+                                tmem_wait_ld16(v);
+#pragma unroll
+                                for (int e = 0; e < 16; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * keep);
+                                tmem_st16(o_at + x, v);
+                            }
+                        }
+                    }
+                    const float minus = -m;
+                    float l0 = 0.f, l1 = 0.f;
+#pragma unroll
+                    for (int x = 0; x < KEYS; x += 32) {
+                        uint32_t v[32], p[16];
+                        tmem_ld32(s_at + x, v);
+                        tmem_wait_ld32(v);
+#pragma unroll
+                        for (int e = 0; e < 32; e += 2) {
+                            float p0 = exp2_approx(fmaf(__uint_as_float(v[e]), scale2, minus)), p1 = exp2_approx(fmaf(__uint_as_float(v[e + 1]), scale2, minus));
+                            if (!clear) {
+                                const int k = k0 + x + e;
+                                if (k < keys.lo || k >= keys.hi) p0 = 0.f;
+                                if (k + 1 < keys.lo || k + 1 >= keys.hi) p1 = 0.f;
+                            }
+                            l0 += p0;
+                            l1 += p1;
+                            p[e / 2] = Pack<E>::two(p0, p1);
+                        }
+                        tmem_st16(s_at + x / 2, p);
+                    }
+                    l += l0 + l1;
+                    tmem_wait_st();
+                    uint32_t keep_sum = 0;
+                    if (checked) {  // values that were taken out of this step's product
+                        const uint32_t s = step % S;
+                        wait(&sh.v_full[s], (step / S) & 1);
+                        uint32_t odd[4];
+                        for (int i = 0; i < 4; ++i) odd[i] = i * 32 < KEYS ? *(volatile uint32_t*)&sh.odd[s][i] : 0u;
+                        if (alive && (odd[0] | odd[1] | odd[2] | odd[3])) {
+                            if (begun) {
+                                wait(&sh.pv_done[last & 1], (last >> 1) & 1);
+                            } else {
+                                keep_sum = 1;
+                                uint32_t zero[16] = {};
+                                for (int x = 0; x < D; x += 16) tmem_st16(o_at + x, zero);
+                                tmem_wait_st();
+                            }
+                            const int32_t* table = cur.source == 0 ? c.prefix_table : c.table + (size_t)(cur.source - 1) * c.table_stride;
+                            for (int k = 0; k < KEYS; ++k) {
+                                if (!(odd[k >> 5] >> (k & 31) & 1u)) continue;
+                                const int key = k0 + k, page_at = divide(key, c.page_div), page = table[page_at];  // in the pool: its row was copied
+                                const E* row = static_cast<const E*>(c.v) + (long long)page * c.page_stride + (long long)(key - page_at * c.page_size) * c.token_stride + (long long)cur.head * c.head_stride;
+                                uint32_t pk[8];
+                                tmem_ld8(s_at + ((k >> 1) & ~7), pk);
+                                tmem_wait_ld();
+                                float p = 0.f;
+                                for (int e = 0; e < 8; ++e)
+                                    if (e == ((k >> 1) & 7)) p = Pack<E>::one((uint16_t)(k & 1 ? pk[e] >> 16 : pk[e] & 0xffffu));
+                                const bool sees = key >= keys.lo && key < keys.hi;
+                                for (int x = 0; x < D; x += 16) {
+                                    uint32_t v[16];
+                                    tmem_ld16(o_at + x, v);
+                                    tmem_wait_ld16(v);
+                                    for (int e = 0; e < 16; ++e)
+                                        if (sees) v[e] = __float_as_uint(__uint_as_float(v[e]) + p * (float)row[x + e]);
+                                    tmem_st16(o_at + x, v);
+                                    tmem_wait_st();
+                                }
+                            }
+                        }
+                    }
+                    if (t < C::kSets) *(volatile uint32_t*)&sh.keep[b] = keep_sum;
+                    tmem_wait_st();
+                    tc_fence_before();
+                    any = true;
+                    last = T;
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sh.p_ready[b]);
+            }
+            // ── the item's sums ──
+            if (any) wait(&sh.pv_done[last & 1], (last >> 1) & 1);
+            const long long item_at = pos - cur.step;
+            const bool here = item_at >= begin && item_at + cur.steps <= end;
+            const bool both = C::kSets == 2 && !pair;
+            float mine = 1.f;
+            if (both) {
+                sh.ml[set][me] = make_float2(m, l);
+                barrier(2, 256);
+                const float2 other = sh.ml[set ^ 1][me];
+                const float top = fmaxf(m, other.x);
+                mine = exp2_approx(m - top);
+                l = l * mine + other.y * exp2_approx(other.x - top);
+                m = top;
+            }
+            const bool writer = !both || t_first == 0;
+            const size_t row = (size_t)it.seq.row + ff / c.ratio, head = (size_t)cur.head * c.ratio + ff % c.ratio;
+            float* part = nullptr;
+            float2* part_ml = nullptr;
+            if (!here) {
+                const size_t at = (size_t)(2 * blockIdx.x + (item_at < begin ? 0 : 1)) * line.columns + f;
+                part = line.slot_o + at * D;
+                part_ml = line.slot_ml + at;
+            } else if (a.whole_o) {
+                const size_t at = ((cur.source == 0 ? (size_t)c.rows : 0) + row) * c.n_q + head;
+                part = a.whole_o + at * D;
+                part_ml = a.whole_ml + at;
+            }
+            const bool write = writer && f < it.width && alive;
+            if (write && part) *part_ml = make_float2(m, l);
+            const float rate = part ? 1.f : l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;
+#pragma unroll 1
+            for (int x = 0; x < D; x += 32) {
+                uint32_t v[32];
+                if (any && alive) {
+                    tmem_ld32(o_at + x, v);
+                    tmem_wait_ld32(v);
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * mine);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) v[e] = 0u;
+                }
+                if (both) {  // [column][32 values], 16-byte groups turned by the column
+                    float* to = joint + me * 32;
+                    if (!writer)
+#pragma unroll
+                        for (int e = 0; e < 32; e += 4) *reinterpret_cast<uint4*>(to + (((e >> 2) ^ (me & 7)) << 2)) = make_uint4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+                    barrier(2, 256);
+                    if (writer)
+#pragma unroll
+                        for (int e = 0; e < 32; e += 4) {
+                            const float4 w = *reinterpret_cast<const float4*>(to + (((e >> 2) ^ (me & 7)) << 2));
+                            v[e] = __float_as_uint(__uint_as_float(v[e]) + w.x); v[e + 1] = __float_as_uint(__uint_as_float(v[e + 1]) + w.y);
+                            v[e + 2] = __float_as_uint(__uint_as_float(v[e + 2]) + w.z); v[e + 3] = __float_as_uint(__uint_as_float(v[e + 3]) + w.w);
+                        }
+                    barrier(2, 256);
+                }
+                if (write) {
+                    if (part) {
+#pragma unroll
+                        for (int e = 0; e < 32; e += 4) *reinterpret_cast<uint4*>(part + x + e) = make_uint4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+                    } else {
+                        E* out = static_cast<E*>(a.out) + row * a.out_stride + head * D + x;
+                        uint32_t w[16];
+#pragma unroll
+                        for (int e = 0; e < 32; e += 2)
+                            w[e / 2] = l == 0.f ? 0u : Pack<E>::two(__uint_as_float(v[e]) * rate, __uint_as_float(v[e + 1]) * rate);
+#pragma unroll
+                        for (int e = 0; e < 16; e += 4) *reinterpret_cast<uint4*>(out + 2 * e) = make_uint4(w[e], w[e + 1], w[e + 2], w[e + 3]);
+                    }
+                }
+            }
+            tc_fence_before();
+        });
+    }
+    __syncthreads();
+    if (tid == 0 && c.err && *dead) atomicOr(c.err, 0x1000u);
+    tc_fence_before();
+    __syncthreads();
+    if (warp == C::kMmaWarp) {
+        tc_fence_after();
+        tmem_dealloc(tmem, 512);
+    }
+}
+
+template <int D, class E>
+cudaError_t go(const Launch& l, const PagedAttentionArgs& a, int line) {
+    auto kernel = paged_wide_kernel<D, E>;
+    const size_t shared = wide_shared<D>(a.c.n_seqs);
+    cudaError_t e = allow_shared(kernel, shared);
+    if (e == cudaSuccess) e = prefer_max_shared(kernel);
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(a.line[line].ctas);
+    cfg.blockDim = dim3(Cfg<D>::kThreads);
+    cfg.dynamicSmemBytes = shared;
+    cfg.stream = l.stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = l.pdl ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, kernel, a, line);
+}
+
+}  // namespace
+
+int paged_wide_columns(int head_dim) { return head_dim == 256 ? Cfg<256>::kColumns : Cfg<128>::kColumns; }
+int paged_wide_keys(int head_dim) { return head_dim == 256 ? Cfg<256>::kKeys : Cfg<128>::kKeys; }
+bool paged_wide_takes(int head_dim, int n_seqs) {
+    const size_t most = 227 * 1024 - 1024;  // less what the scan of the batch holds, up to the tiles' alignment
+    return (head_dim == 64 ? wide_shared<64>(n_seqs) : head_dim == 128 ? wide_shared<128>(n_seqs) : wide_shared<256>(n_seqs)) <= most;
+}
+cudaError_t launch_paged_wide(const Launch& l, PagedType type, int head_dim, const PagedAttentionArgs& a, int line) {
+    if (type == kPagedF16) return head_dim == 64 ? go<64, __half>(l, a, line) : head_dim == 128 ? go<128, __half>(l, a, line) : go<256, __half>(l, a, line);
+    return head_dim == 64 ? go<64, __nv_bfloat16>(l, a, line) : head_dim == 128 ? go<128, __nv_bfloat16>(l, a, line) : go<256, __nv_bfloat16>(l, a, line);
+}
+
+}  // namespace smelt
