@@ -43,7 +43,7 @@ smelt_status cache_args(smelt_cuda_ctx* ctx, const smelt_paged_cache* k, const s
     c->k = k->k; c->v = k->v;
     c->page_stride = k->page_stride; c->head_stride = k->head_stride; c->token_stride = k->token_stride;
     c->page_size = k->page_size; c->n_pages = k->n_pages; c->page_div = Divisor::of((uint32_t)k->page_size);
-    c->n_q = k->n_q; c->n_kv = k->n_kv; c->ratio = k->n_q / k->n_kv;
+    c->n_q = k->n_q; c->n_kv = k->n_kv; c->ratio = k->n_q / k->n_kv; c->ratio_div = Divisor::of((uint32_t)c->ratio);
     c->n_seqs = b->n_seqs; c->rows = b->rows; c->table_stride = b->table_stride; c->prefix_length = b->prefix_length;
     const int64_t tokens = (int64_t)b->table_stride * k->page_size;
     c->table_tokens = (int)(tokens < 0x3fffffff ? tokens : 0x3fffffff);
@@ -78,9 +78,9 @@ size_t attention_plan(const smelt_cuda_ctx* ctx, const smelt_paged_cache* k, con
         line.columns = wide ? paged_wide_columns(D) : paged_narrow_columns(D, columns);
         line.keys = wide ? paged_wide_keys(D) : paged_narrow_keys(D);
         line.ctas = ctx->sm_count;
-        line.cum = (int64_t*)room((size_t)(b->n_seqs + 3) * sizeof(int64_t));
-        line.slot_o = (float*)room((size_t)2 * line.ctas * line.columns * D * sizeof(float));
-        line.slot_ml = (float2*)room((size_t)2 * line.ctas * line.columns * sizeof(float2));
+        line.cum = (int32_t*)room((size_t)(b->n_seqs + 3) * sizeof(int32_t));
+        line.slot_o = (float*)room(((size_t)2 * line.ctas << line.columns) * D * sizeof(float));
+        line.slot_ml = (float2*)room(((size_t)2 * line.ctas << line.columns) * sizeof(float2));
     };
     if (prefix == 0) {
         add(own_wide, true, false);
@@ -184,12 +184,23 @@ smelt_status smelt_cuda_paged_attention(smelt_cuda_ctx* ctx, const smelt_paged_c
     if (!rows_ok(q, q_stride, cache->n_q * D, rows) || !rows_ok(out, out_stride, cache->n_q * D, rows)) return fail(ctx, SMELT_ERR_BAD_ARGUMENT, "paged attention: rows are 16-byte aligned, strides multiples of 8");
     if (q == out && q_stride != out_stride) return fail(ctx, SMELT_ERR_BAD_ARGUMENT, "paged attention: an output in the place of the queries keeps their stride");
     if (!(scale == scale) || std::isinf(scale)) return fail(ctx, SMELT_ERR_BAD_ARGUMENT, "paged attention: scale is not finite");
+    {  // the line of work is counted in 32 bits
+        attention_plan(ctx, cache, batch, &a, nullptr);
+        double steps = 0;
+        for (int i = 0; i < a.lines; ++i) {
+            const PagedLine& line = a.line[i];
+            const double blocks = (double)(rows * a.c.ratio >> line.columns) + 1;
+            if (line.with_own) steps += (blocks + batch->n_seqs) * cache->n_kv * ((a.c.table_tokens >> line.keys) + 2.0);
+            if (line.with_prefix) steps += blocks * cache->n_kv * ((batch->prefix_length >> line.keys) + 2.0);
+        }
+        if (steps > 1e9) return fail(ctx, SMELT_ERR_OUT_OF_RANGE, "paged attention: more rows times pages than a call takes");
+    }
     if (!workspace || !aligned16(workspace) || workspace_bytes < attention_plan(ctx, cache, batch, &a, nullptr))
         return fail(ctx, SMELT_ERR_BAD_ARGUMENT, "paged attention: workspace missing, misaligned or smaller than smelt_cuda_paged_attention_workspace says");
     attention_plan(ctx, cache, batch, &a, workspace);
     a.q = q; a.out = out; a.q_stride = q_stride; a.out_stride = out_stride;
     a.scale2 = scale * 1.4426950408889634f;
-    a.window = window;
+    a.window = window < 0x7fffffffu ? window : 0;  // positions are below that
     cudaError_t e = cudaSuccess;
     for (int i = 0; i < a.lines && e == cudaSuccess; ++i) e = (a.line[i].wide ? launch_paged_wide : launch_paged_narrow)(l, (PagedType)cache->precision, cache->head_dim, a, i);
     if (e == cudaSuccess) e = launch_paged_merge(l, (PagedType)cache->precision, cache->head_dim, a);

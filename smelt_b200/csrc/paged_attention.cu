@@ -6,14 +6,16 @@
 // of few columns (a column is a row and a query head of the group that shares a key head) and the kernel that joins shared items.
 //
 // paged_narrow_kernel: one CTA a SM, each with as many steps of the line of work (paged.h).  A warp takes 16 keys of a step at a time as
-// S^T = K Q^T and O^T += V^T P^T on mma.sync (the tile arithmetic of attention.cuh): the columns of the block are the narrow side of the
-// product, so eight columns cost what one costs.  A tile's K and V halves are copied row by row with cp.async into a ring of the
-// warp's own and read back by the lanes that copied them; the ring runs on across items, so that the pages of the next sequence are on
-// their way while this one's warps join their sums.
+// S^T = K Q^T and O^T += V^T P^T on mma.sync: the columns of the block are the narrow side of the product, so eight columns cost what one
+// costs.  A lane brings a key's row with one bulk copy for K and one for V, wherever its page is, into a ring of the warp's own; rows lie 16
+// bytes more than their length apart, so that ldmatrix reads them without conflicts, and the warp waits on its own barriers
+// only.  The ring runs on across items, so that the pages of the next sequence are on their way while this one's warps join their sums.
 // P goes into the product as two 16-bit parts: the kernel waits for memory, and rounding P once would cost up to half a step of the
-// 16-bit type.  Keys outside an item are not read (zero fill), and a value row that is not finite reaches only the columns that see it.
+// 16-bit type.  Keys outside an item are not read (zeros), and a value row that is not finite reaches only the columns that see it.
+// paged_merge_kernel joins the items that several CTAs share, and the prefix with the sequences.
 #include "attention.cuh"
 #include "paged_line.cuh"
+#include "tcgen05.cuh"
 
 namespace smelt {
 namespace {
@@ -21,20 +23,27 @@ namespace {
 using namespace paged;
 using attn::movmatrix_trans;
 using attn::TileElem;
-using attn::tile_scores;
-using attn::tile_weighted_sum;
 
 template <int D> constexpr int kWarps = D == 256 ? 4 : 8;
-template <int D> constexpr int kUnits = D == 64 ? 10 : 5;  // of a warp's ring: a K or V half of a 16-key tile each, 20 KB (40 KB) a warp
-template <int D> constexpr int kUnitBytes = 16 * D * 2;
+template <int D> constexpr int kUnits = D == 64 ? 10 : 5;  // of a warp's ring: the K or V rows of 16 keys each
+template <int D> constexpr int kPitch = D * 2 + 16;
+template <int D> constexpr int kUnitBytes = 16 * kPitch<D>;
 
 template <int D>
-constexpr size_t narrow_shared(int n_seqs) {  // rings, one column group's sums of all warps, their maxima and sums, the batch
-    return (size_t)kWarps<D> * kUnits<D> * kUnitBytes<D> + (size_t)kWarps<D> * 8 * D * 4 + (size_t)kWarps<D> * 8 * 8 + batch_bytes(n_seqs);
+constexpr size_t narrow_shared(int n_seqs) {  // rings, one column group's sums of all warps, their maxima and sums, barriers, the batch
+    return (size_t)kWarps<D> * kUnits<D> * kUnitBytes<D> + (size_t)kWarps<D> * 8 * (D + 1) * 4 + (size_t)kWarps<D> * 8 * 8 + (size_t)kWarps<D> * kUnits<D> * 8 + batch_bytes(n_seqs);
 }
 
-__device__ __forceinline__ void cp_async16_or_zero(void* dst, const void* src, bool take) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(take ? 16 : 0) : "memory");
+__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t at) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+__device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], uint32_t at) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+__device__ __forceinline__ float exp2_approx(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
 }
 
 template <class E> __device__ __forceinline__ E round_to(float v);
@@ -42,7 +51,7 @@ template <> __device__ __forceinline__ __half round_to<__half>(float v) { return
 template <> __device__ __forceinline__ __nv_bfloat16 round_to<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
 template <class E> __device__ __forceinline__ bool pair_not_finite(uint32_t v) {  // a pair of values with an exponent of all ones
-    constexpr uint32_t m = sizeof(E) == 2 && std::is_same<E, __half>::value ? 0x7C00u : 0x7F80u;
+    constexpr uint32_t m = std::is_same<E, __half>::value ? 0x7C00u : 0x7F80u;
     return (v & m) == m || ((v >> 16) & m) == m;
 }
 
@@ -55,105 +64,103 @@ struct MaskedTile {
     Range keys[NH][2];
 };
 template <int D, int NH, class E>
-__device__ __noinline__ void weighted_sum_masked(const unsigned char* vu, MaskedTile<D, NH>& m, int k0, int t) {
-    constexpr int VC = D / 64;
+__device__ __noinline__ void weighted_sum_masked(uint32_t values, MaskedTile<D, NH>& m, int k0, int t) {
     for (int nh = 0; nh < NH; ++nh)
         for (int col = 0; col < 8; ++col) {
             const int from = (threadIdx.x & 28) | (col >> 1);
             const int lo = __shfl_sync(0xffffffffu, m.keys[nh][col & 1].lo, from), hi = __shfl_sync(0xffffffffu, m.keys[nh][col & 1].hi, from);
-            uint32_t keep[4];
-            const int mine[4] = {k0 + 2 * t, k0 + 2 * t + 1, k0 + 2 * t + 8, k0 + 2 * t + 9};
-            for (int i = 0; i < 4; ++i) keep[i] = mine[i] >= lo && mine[i] < hi ? 0xffffffffu : 0u;
-            for (int c = 0; c < VC; ++c) {
-                uint32_t r[4][4];
-                for (int i = 0; i < 4; ++i) {
-                    const uint4 v = *reinterpret_cast<const uint4*>(vu + (4 * c + i) * 512);
-                    r[i][0] = v.x & keep[i]; r[i][1] = v.y & keep[i]; r[i][2] = v.z & keep[i]; r[i][3] = v.w & keep[i];
-                }
-                for (int e = 0; e < 4; ++e) {
-                    float add[4] = {0.f, 0.f, 0.f, 0.f};
-                    const uint32_t a0 = __byte_perm(r[0][e], r[1][e], 0x5410), a1 = __byte_perm(r[0][e], r[1][e], 0x7632);
-                    const uint32_t a2 = __byte_perm(r[2][e], r[3][e], 0x5410), a3 = __byte_perm(r[2][e], r[3][e], 0x7632);
-                    TileElem<E>::mma(add, a0, a1, a2, a3, m.p[nh][0], m.p[nh][1]);
-                    TileElem<E>::mma(add, a0, a1, a2, a3, m.p[nh][2], m.p[nh][3]);
-                    if ((col >> 1) == t) { m.o[nh][4 * c + e][col & 1] += add[col & 1]; m.o[nh][4 * c + e][2 + (col & 1)] += add[2 + (col & 1)]; }
-                }
+            auto sees = [&](int k) { return k >= lo && k < hi; };
+            const int k = k0 + 2 * t;
+            const uint32_t near = (sees(k) ? 0xffffu : 0u) | (sees(k + 1) ? 0xffff0000u : 0u), far = (sees(k + 8) ? 0xffffu : 0u) | (sees(k + 9) ? 0xffff0000u : 0u);
+            for (int i = 0; i < D / 16; ++i) {
+                uint32_t v[4];
+                ldmatrix4_trans(v, values + 32 * i);
+                float add[4] = {0.f, 0.f, 0.f, 0.f};
+                TileElem<E>::mma(add, v[0] & near, v[1] & near, v[2] & far, v[3] & far, m.p[nh][0], m.p[nh][1]);
+                TileElem<E>::mma(add, v[0] & near, v[1] & near, v[2] & far, v[3] & far, m.p[nh][2], m.p[nh][3]);
+                if ((col >> 1) == t) { m.o[nh][i][col & 1] += add[col & 1]; m.o[nh][i][2 + (col & 1)] += add[2 + (col & 1)]; }
             }
         }
 }
 
 template <int D, int NH, class E>
-__global__ void __launch_bounds__(kWarps<D> * 32, 1) paged_narrow_kernel(const PagedAttentionArgs a, const int which) {
-    constexpr int W = kWarps<D>, THREADS = W * 32, NU = kUnits<D>, UNIT = kUnitBytes<D>, KEYS = W * 16, MT = D / 16, KJ = D / 32, VC = D / 64;
+__global__ void __launch_bounds__(kWarps<D> * 32, 1) paged_narrow_kernel(const __grid_constant__ PagedAttentionArgs a, const int which) {
+    constexpr int W = kWarps<D>, THREADS = W * 32, NU = kUnits<D>, UNIT = kUnitBytes<D>, PITCH = kPitch<D>, KEYS = W * 16, MT = D / 16;
     extern __shared__ __align__(16) unsigned char smem[];
-    float* sums = reinterpret_cast<float*>(smem + (size_t)W * NU * UNIT);   // [W][8][D]
-    float2* state = reinterpret_cast<float2*>(sums + W * 8 * D);            // [W][8]
+    float* sums = reinterpret_cast<float*>(smem + (size_t)W * NU * UNIT);     // [W][8][D + 1]
+    float2* state = reinterpret_cast<float2*>(sums + W * 8 * (D + 1));        // [W][8]
+    uint64_t* bars = reinterpret_cast<uint64_t*>(state + W * 8);              // [W][NU]
     const PagedArgs& c = a.c;
     const PagedLine& line = a.line[which];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    uint64_t* bar = bars + warp * NU;
+    if (lane < NU) mbar_init(bar + lane, 1);
+    mbar_fence_init();
+    fence_async_smem();
     pdl_trigger();
     pdl_wait();
     Batch batch;
-    scan_line<THREADS>(c, line, a.window, batch, reinterpret_cast<unsigned char*>(state + W * 8));
-    const long long total = batch.cum[c.n_seqs + 1];
-    const int ctas = line_ctas(total, line.ctas);
-    if ((int)blockIdx.x >= ctas) return;
-    const long long begin = line_begin(total, blockIdx.x, ctas), end = line_begin(total, blockIdx.x + 1, ctas);
-    const E* K = static_cast<const E*>(c.k);
-    const E* V = static_cast<const E*>(c.v);
+    scan_line<THREADS>(c, line, a.window, batch, reinterpret_cast<unsigned char*>(bars + W * NU));
+    const Share share(batch.cum[c.n_seqs + 1], line.ctas);
+    if ((int)blockIdx.x >= share.ctas) return;
+    const int begin = share.begin(blockIdx.x), end = share.begin(blockIdx.x + 1);
 
     // ── the ring: unit u holds K (even) or V (odd) of this warp's tile of step begin + u / 2 ──
-    unsigned char* ring = smem + (size_t)warp * NU * UNIT + lane * 16;
-    Cursor ahead;  // the step whose page is looked up next
-    long long at = begin;
-    ahead.seek(c, line, a.window, batch, begin);
-    int page = -1, key = 0, head = 0;  // lane i (and i + 16): page of key i of the tile that is issued next, -1 where it is outside the item
+    unsigned char* ring = smem + (size_t)warp * NU * UNIT;
+    Cursor cur;
+    cur.seek(c, line, a.window, batch, begin);
+    Cursor ahead = cur;  // the step whose page is looked up next
+    int at = begin;
+    int page = 0, slot = 0, head = 0;  // lane i (and i + 16): page and place of key i of the tile that is issued next
+    bool inside = false;               // ... which is one of the item's
     auto look_up = [&]() {
-        page = -1;
+        inside = false;
         if (at >= end) return;
-        key = (ahead.first + ahead.step) * KEYS + warp * 16 + (lane & 15);
+        const int key = (ahead.first + ahead.step) * KEYS + warp * 16 + (lane & 15);
         head = ahead.head;
-        if (key >= ahead.keys.lo && key < ahead.keys.hi) {
+        inside = key >= ahead.keys.lo && key < ahead.keys.hi;
+        if (inside) {
             const int32_t* table = ahead.source == 0 ? c.prefix_table : c.table + (size_t)(ahead.source - 1) * c.table_stride;
-            page = table[divide(key, c.page_div)];
-            if ((uint32_t)page >= (uint32_t)c.n_pages) { page = -1; if (c.err && lane < 16) atomicOr(c.err, KERR_BAD_PAGE); }
+            const int p = divide(key, c.page_div);
+            slot = key - p * c.page_size;
+            page = table[p];
         }
         if (++at < end) ahead.advance(c, line, a.window, batch);
     };
-    long long row = 0;  // of lane's key, in elements; -1: none
-    auto issue_unit = [&](int u) {
-        unsigned char* dst = ring + (size_t)(u % NU) * UNIT;
+    long long row = -1;  // of lane's key in the pools, in elements; -1: none
+    int rows = 0;        // of the tile that there are
+    auto issue_unit = [&](int u, int place) {
+        unsigned char* dst = ring + place * UNIT + (lane & 15) * PITCH;
         if ((u & 1) == 0) {
-            row = page < 0 ? -1ll : (long long)page * c.page_stride + (long long)(key - divide(key, c.page_div) * c.page_size) * c.token_stride + (long long)head * c.head_stride;
+            row = -1;
+            if (inside) {
+                if ((uint32_t)page < (uint32_t)c.n_pages) row = (long long)page * c.page_stride + (long long)slot * c.token_stride + (long long)head * c.head_stride;
+                else if (c.err && lane < 16) atomicOr(c.err, KERR_BAD_PAGE);
+            }
+            rows = __popc(__ballot_sync(0xffffffffu, row >= 0) & 0xffffu);
             look_up();
-            const long long ra = __shfl_sync(0xffffffffu, row, g), rb = __shfl_sync(0xffffffffu, row, g + 8);
-            const E *pa = K + max(ra, 0ll) + 8 * t, *pb = K + max(rb, 0ll) + 8 * t;
-#pragma unroll
-            for (int j = 0; j < KJ; ++j) {
-                cp_async16_or_zero(dst + (2 * j) * 512, pa + 32 * j, ra >= 0);
-                cp_async16_or_zero(dst + (2 * j + 1) * 512, pb + 32 * j, rb >= 0);
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const long long r = __shfl_sync(0xffffffffu, row, 2 * t + (i & 1) + 8 * (i >> 1));
-                const E* p = V + max(r, 0ll) + 8 * g;
-#pragma unroll
-                for (int cc = 0; cc < VC; ++cc) cp_async16_or_zero(dst + (4 * cc + i) * 512, p + 64 * cc, r >= 0);
-            }
         }
-        cp_async_commit();
+        __syncwarp();  // the unit's last readers are through
+        if (rows < 16) {
+            if (row < 0 && lane < 16)
+                for (int i = 0; i < D * 2; i += 16) *reinterpret_cast<uint4*>(dst + i) = make_uint4(0, 0, 0, 0);
+            fence_async_smem();  // a copy writes there later
+        }
+        if (lane == 0) mbar_arrive_expect_tx(bar + place, rows * D * 2);
+        __syncwarp();
+        if (row >= 0 && lane < 16) bulk_g2s(dst, static_cast<const E*>((u & 1) == 0 ? c.k : c.v) + row, D * 2, bar + place);
     };
     look_up();
-    const int n_units = 2 * (int)(end - begin);
-    int issued = 0;
-    for (; issued < NU - 1; ++issued) {
-        if (issued < n_units) issue_unit(issued);
-        else cp_async_commit();
-    }
+    const int n_units = 2 * (end - begin);
+    int issued = 0, issue_place = 0;  // the next unit to issue, and its place in the ring
+    auto issue_next = [&]() {
+        if (issued < n_units) issue_unit(issued, issue_place);
+        ++issued;
+        if (++issue_place == NU) issue_place = 0;
+    };
+#pragma unroll 1
+    for (int i = 0; i < NU - 1; ++i) issue_next();
 
-    Cursor cur;
-    cur.seek(c, line, a.window, batch, begin);
     const E* q = static_cast<const E*>(a.q);
     uint32_t qf[NH][D / 8];
     float m_run[NH][2], l_run[NH][2], o[NH][MT][4];
@@ -161,17 +168,28 @@ __global__ void __launch_bounds__(kWarps<D> * 32, 1) paged_narrow_kernel(const P
     int clear_lo = 0, clear_hi = 0;  // every column of the block sees the keys [clear_lo, clear_hi)
     Seq seq{0, 0, 0};
     int width = 0;  // columns of the block
-    unsigned used = 0;
+    int use_place = 0;
+    uint32_t use_phase = 0;
+    bool alive = true;
+    // ldmatrix: this lane's row of a tile of keys (as they are) and of values (turned)
+    const uint32_t k_lane = smem_u32(ring) + ((lane & 7) + ((lane >> 3) & 1) * 8) * PITCH + (lane >> 4) * 16;
+    const uint32_t v_lane = smem_u32(ring) + ((lane & 7) + (lane >> 4) * 8) * PITCH + ((lane >> 3) & 1) * 16;
+    auto arrived = [&]() {  // the unit at use_place, which it leaves in `place`
+        alive = alive && mbar_poll_bounded(bar + use_place, use_phase);
+        const int place = use_place;
+        if (++use_place == NU) { use_place = 0; use_phase ^= 1u; }
+        return place;
+    };
 
-    for (long long pos = begin; pos < end;) {
+    for (int pos = begin; pos < end;) {
         // ── an item: its columns' queries and key ranges ──
-        const int f0 = cur.block * line.columns;
+        const int f0 = cur.block << line.columns;
         if (cur.source == 0) seq = {0, batch.row[c.n_seqs], 0};
         else seq = batch.seq(cur.source - 1);
-        width = min(line.columns, seq.n * c.ratio - f0);
+        width = min(1 << line.columns, seq.n * c.ratio - f0);
         auto range_of = [&](int f) -> Range {
             if (f >= width) return {0, 0};
-            const int i = (f0 + f) / c.ratio;
+            const int i = divide(f0 + f, c.ratio_div);
             if (cur.source) return own_keys(seq, i, a.window);
             const Seq s = batch.seq(seq_of_row(batch, c.n_seqs, i));
             return prefix_keys(s, i - s.row, c.prefix_length, a.window);
@@ -180,24 +198,22 @@ __global__ void __launch_bounds__(kWarps<D> * 32, 1) paged_narrow_kernel(const P
         clear_hi = 0x7fffffff;
 #pragma unroll
         for (int nh = 0; nh < NH; ++nh) {
+            const int f = nh * 8 + g;
+            if (f < width) {
+                const int i = divide(f0 + f, c.ratio_div);
+                const E* row_q = q + (size_t)(seq.row + i) * a.q_stride + (size_t)(cur.head * c.ratio + f0 + f - i * c.ratio) * D + 2 * t;
+#pragma unroll
+                for (int j = 0; j < D / 8; ++j) qf[nh][j] = *reinterpret_cast<const uint32_t*>(row_q + 8 * j);
+            } else {
+#pragma unroll
+                for (int j = 0; j < D / 8; ++j) qf[nh][j] = 0u;
+            }
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
                 keys[nh][x] = range_of(nh * 8 + 2 * t + x);
                 if (nh * 8 + 2 * t + x < width) { clear_lo = max(clear_lo, keys[nh][x].lo); clear_hi = min(clear_hi, keys[nh][x].hi); }
                 m_run[nh][x] = kLowest;
                 l_run[nh][x] = 0.f;
-            }
-            const int f = nh * 8 + g;
-            if (f < width) {
-                const E* row_q = q + (size_t)(seq.row + (f0 + f) / c.ratio) * a.q_stride + (size_t)(cur.head * c.ratio + (f0 + f) % c.ratio) * D + 8 * t;
-#pragma unroll
-                for (int j = 0; j < KJ; ++j) {
-                    const uint4 v = *reinterpret_cast<const uint4*>(row_q + 32 * j);
-                    qf[nh][4 * j] = v.x; qf[nh][4 * j + 1] = v.y; qf[nh][4 * j + 2] = v.z; qf[nh][4 * j + 3] = v.w;
-                }
-            } else {
-#pragma unroll
-                for (int j = 0; j < D / 8; ++j) qf[nh][j] = 0u;
             }
 #pragma unroll
             for (int i = 0; i < MT; ++i) o[nh][i][0] = o[nh][i][1] = o[nh][i][2] = o[nh][i][3] = 0.f;
@@ -208,53 +224,76 @@ __global__ void __launch_bounds__(kWarps<D> * 32, 1) paged_narrow_kernel(const P
             clear_hi = min(clear_hi, __shfl_xor_sync(0xffffffffu, clear_hi, off));
         }
         const Cursor item = cur;
-        const long long item_at = pos - cur.step;  // the item's first step on the line
+        const int item_at = pos - cur.step;  // the item's first step on the line
 
         // ── its steps in this CTA's stretch ──
+#pragma unroll 1
         for (;;) {
             const int k0 = (cur.first + cur.step) * KEYS + warp * 16;
-            const int u = 2 * (int)used;
-            const unsigned char *ku = ring + (size_t)(u % NU) * UNIT, *vu = ring + (size_t)((u + 1) % NU) * UNIT;
             const bool active = k0 < cur.keys.hi && k0 + 16 > cur.keys.lo;
             uint32_t pb[NH][4];
-            // K half
-            if (issued < n_units) issue_unit(issued);
-            else cp_async_commit();
-            ++issued;
-            cp_async_wait<NU - 1>();
-            __syncwarp();
             bool clear = true;
+            const uint32_t ku = k_lane + arrived() * UNIT;
             if (active) {
-                float s[NH][4];
-                tile_scores<D, NH, E>(ku, qf, s);
+                float s[NH][2][4];
+#pragma unroll
+                for (int nh = 0; nh < NH; ++nh)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) s[nh][0][i] = s[nh][1][i] = 0.f;
+#pragma unroll
+                for (int j = 0; j < MT; ++j) {
+                    uint32_t k[4];
+                    ldmatrix4(k, ku + 32 * j);
+#pragma unroll
+                    for (int nh = 0; nh < NH; ++nh) TileElem<E>::mma(s[nh][j & 1], k[0], k[1], k[2], k[3], qf[nh][2 * j], qf[nh][2 * j + 1]);
+                }
                 clear = k0 >= clear_lo && k0 + 16 <= clear_hi;
+                float v[NH][4], top[NH][2];
+                bool valid[NH][4];
 #pragma unroll
                 for (int nh = 0; nh < NH; ++nh) {
-                    bool valid[4] = {true, true, true, true};
-                    float v[4];
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
+                        valid[nh][i] = true;
                         if (!clear) {
                             const int k = k0 + g + 8 * (i >> 1);
-                            valid[i] = k >= keys[nh][i & 1].lo && k < keys[nh][i & 1].hi;
+                            valid[nh][i] = k >= keys[nh][i & 1].lo && k < keys[nh][i & 1].hi;
                         }
-                        v[i] = valid[i] ? s[nh][i] * a.scale2 : kLowest;
+                        v[nh][i] = valid[nh][i] ? (s[nh][0][i] + s[nh][1][i]) * a.scale2 : kLowest;
                     }
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) top[nh][x] = fmaxf(v[nh][x], v[nh][2 + x]);
+                }
+                bool moved = false;
+#pragma unroll
+                for (int off = 4; off < 32; off <<= 1)
+#pragma unroll
+                    for (int nh = 0; nh < NH; ++nh)
+#pragma unroll
+                        for (int x = 0; x < 2; ++x) top[nh][x] = fmaxf(top[nh][x], __shfl_xor_sync(0xffffffffu, top[nh][x], off));
+#pragma unroll
+                for (int nh = 0; nh < NH; ++nh)
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) moved = moved || top[nh][x] > m_run[nh][x];
+                if (__any_sync(0xffffffffu, moved)) {  // a new maximum: rare behind the first tiles
+#pragma unroll
+                    for (int nh = 0; nh < NH; ++nh)
+#pragma unroll
+                        for (int x = 0; x < 2; ++x) {
+                            const float m = fmaxf(top[nh][x], m_run[nh][x]), keep = exp2_approx(m_run[nh][x] - m);
+                            m_run[nh][x] = m;
+                            l_run[nh][x] *= keep;
+#pragma unroll
+                            for (int i = 0; i < MT; ++i) { o[nh][i][x] *= keep; o[nh][i][2 + x] *= keep; }
+                        }
+                }
+#pragma unroll
+                for (int nh = 0; nh < NH; ++nh) {
                     float p[4];
 #pragma unroll
-                    for (int x = 0; x < 2; ++x) {
-                        float top = fmaxf(v[x], v[2 + x]);
-#pragma unroll
-                        for (int off = 4; off < 32; off <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-                        top = fmaxf(top, m_run[nh][x]);
-                        const float keep = exp2f(m_run[nh][x] - top);
-                        m_run[nh][x] = top;
-                        p[x] = valid[x] ? exp2f(v[x] - top) : 0.f;
-                        p[2 + x] = valid[2 + x] ? exp2f(v[2 + x] - top) : 0.f;
-                        l_run[nh][x] = l_run[nh][x] * keep + (p[x] + p[2 + x]);
-#pragma unroll
-                        for (int i = 0; i < MT; ++i) { o[nh][i][x] *= keep; o[nh][i][2 + x] *= keep; }
-                    }
+                    for (int i = 0; i < 4; ++i) p[i] = valid[nh][i] ? exp2_approx(v[nh][i] - m_run[nh][i & 1]) : 0.f;
+                    l_run[nh][0] += p[0] + p[2];
+                    l_run[nh][1] += p[1] + p[3];
                     const uint32_t pa = TileElem<E>::pack(p[0], p[1]), pc = TileElem<E>::pack(p[2], p[3]);
                     const float2 fa = TileElem<E>::unpack(pa), fc = TileElem<E>::unpack(pc);
                     pb[nh][0] = movmatrix_trans(pa);
@@ -263,19 +302,16 @@ __global__ void __launch_bounds__(kWarps<D> * 32, 1) paged_narrow_kernel(const P
                     pb[nh][3] = movmatrix_trans(TileElem<E>::pack(p[2] - fc.x, p[3] - fc.y));
                 }
             }
-            // V half
-            if (issued < n_units) issue_unit(issued);
-            else cp_async_commit();
-            ++issued;
-            cp_async_wait<NU - 1>();
-            __syncwarp();
+            issue_next();  // into the place of the values of the tile before, which are used up
+            const uint32_t vu = v_lane + arrived() * UNIT;
             if (active) {
                 bool odd = false;
                 if (!clear) {
-#pragma unroll
-                    for (int i = 0; i < 4 * VC; ++i) {
-                        const uint4 v = *reinterpret_cast<const uint4*>(vu + i * 512);
-                        odd = odd || pair_not_finite<E>(v.x) || pair_not_finite<E>(v.y) || pair_not_finite<E>(v.z) || pair_not_finite<E>(v.w);
+#pragma unroll 1
+                    for (int i = 0; i < MT; ++i) {
+                        uint32_t v[4];
+                        ldmatrix4_trans(v, vu + 32 * i);
+                        odd = odd || pair_not_finite<E>(v[0]) || pair_not_finite<E>(v[1]) || pair_not_finite<E>(v[2]) || pair_not_finite<E>(v[3]);
                     }
                     odd = __any_sync(0xffffffffu, odd);
                 }
@@ -300,43 +336,40 @@ __global__ void __launch_bounds__(kWarps<D> * 32, 1) paged_narrow_kernel(const P
 #pragma unroll
                             for (int e = 0; e < 4; ++e) o[nh][i][e] = rare.o[nh][i][e];
                 } else {
-                    uint32_t b0[NH], b1[NH], l0[NH], l1[NH];
 #pragma unroll
-                    for (int nh = 0; nh < NH; ++nh) { b0[nh] = pb[nh][0]; b1[nh] = pb[nh][1]; l0[nh] = pb[nh][2]; l1[nh] = pb[nh][3]; }
-                    tile_weighted_sum<D, NH, E>(vu, o, b0, b1, l0, l1);
+                    for (int i = 0; i < MT; ++i) {
+                        uint32_t v[4];
+                        ldmatrix4_trans(v, vu + 32 * i);
+#pragma unroll
+                        for (int nh = 0; nh < NH; ++nh) {
+                            TileElem<E>::mma(o[nh][i], v[0], v[1], v[2], v[3], pb[nh][0], pb[nh][1]);
+                            TileElem<E>::mma(o[nh][i], v[0], v[1], v[2], v[3], pb[nh][2], pb[nh][3]);
+                        }
+                    }
                 }
             }
-            ++used;
-            ++pos;
-            if (pos >= end) break;
+            issue_next();  // into the place of this tile's keys
+            if (++pos >= end) break;
             cur.advance(c, line, a.window, batch);
             if (!cur.same_item(item)) break;
         }
 
         // ── the warps' sums, eight columns at a time ──
         const bool here = item_at >= begin && item_at + item.steps <= end;
-        const int slot = 2 * blockIdx.x + (item_at < begin ? 0 : 1);
+        const size_t slot_at = (size_t)(2 * blockIdx.x + (item_at < begin ? 0 : 1)) << line.columns;
+#pragma unroll
         for (int nh = 0; nh < NH; ++nh) {
             if (nh * 8 >= width) break;
 #pragma unroll
-            for (int n2 = 0; n2 < NH; ++n2)
-                if (n2 == nh) {
+            for (int x = 0; x < 2; ++x) {
+                float l = l_run[nh][x];
 #pragma unroll
-                    for (int x = 0; x < 2; ++x) {
-                        float l = l_run[n2][x];
+                for (int off = 4; off < 32; off <<= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
+                if (g == 0) state[warp * 8 + 2 * t + x] = make_float2(m_run[nh][x], l);
+                float* to = sums + (warp * 8 + 2 * t + x) * (D + 1) + g;
 #pragma unroll
-                        for (int off = 4; off < 32; off <<= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
-                        if (g == 0) state[warp * 8 + 2 * t + x] = make_float2(m_run[n2][x], l);
-                        float* to = sums + (size_t)(warp * 8 + 2 * t + x) * D;
-#pragma unroll
-                        for (int i = 0; i < MT; ++i)
-#pragma unroll
-                            for (int h = 0; h < 2; ++h) {
-                                const int j = 2 * i + h;
-                                to[64 * (j >> 3) + 8 * g + (j & 7)] = o[n2][i][2 * h + x];
-                            }
-                    }
-                }
+                for (int i = 0; i < MT; ++i) { to[16 * i] = o[nh][i][x]; to[16 * i + 8] = o[nh][i][2 + x]; }
+            }
             __syncthreads();
             const int n = min(8, width - nh * 8);
             for (int i = tid; i < n * D; i += THREADS) {
@@ -346,14 +379,16 @@ __global__ void __launch_bounds__(kWarps<D> * 32, 1) paged_narrow_kernel(const P
                 for (int w = 0; w < W; ++w) top = fmaxf(top, state[w * 8 + col].x);
 #pragma unroll
                 for (int w = 0; w < W; ++w) {
-                    const float keep = exp2f(state[w * 8 + col].x - top);
-                    l += state[w * 8 + col].y * keep;
-                    sum += sums[(size_t)(w * 8 + col) * D + d] * keep;
+                    const float2 ml = state[w * 8 + col];
+                    const float keep = exp2_approx(ml.x - top);
+                    l += ml.y * keep;
+                    sum += sums[(w * 8 + col) * (D + 1) + d] * keep;
                 }
-                const size_t out_row = seq.row + (f0 + f) / c.ratio, out_head = item.head * c.ratio + (f0 + f) % c.ratio;
+                const int ri = divide(f0 + f, c.ratio_div);
+                const size_t out_row = seq.row + ri, out_head = item.head * c.ratio + f0 + f - ri * c.ratio;
                 if (!here) {
-                    line.slot_o[((size_t)slot * line.columns + f) * D + d] = sum;
-                    if (d == 0) line.slot_ml[(size_t)slot * line.columns + f] = make_float2(top, l);
+                    line.slot_o[(slot_at + f) * D + d] = sum;
+                    if (d == 0) line.slot_ml[slot_at + f] = make_float2(top, l);
                 } else if (a.whole_o) {
                     const size_t at_row = ((item.source == 0 ? (size_t)c.rows : 0) + out_row) * c.n_q + out_head;
                     a.whole_o[at_row * D + d] = sum;
@@ -365,92 +400,119 @@ __global__ void __launch_bounds__(kWarps<D> * 32, 1) paged_narrow_kernel(const P
             __syncthreads();
         }
     }
-    cp_async_wait<0>();
+    if (!alive && lane == 0 && c.err) atomicOr(c.err, 0x1000u);
 }
 
 // ── the join ────────────────────────────────────────────────────────────────
-// A warp a row and query head: the parts of its item of the sequence and of its item of the prefix, in the order of the line.
+// A warp a row and query head: the parts of its item of the sequence and of its item of the prefix, in the order of the line.  A lane
+// fetches a part's maximum and sum; then the parts' sums are added with their factors, eight on their way at a time.
 constexpr int kMergeWarps = 4;
 
-template <int D>
-struct Joined {
-    float top = kLowest, l = 0.f, o[D / 32];
-    __device__ __forceinline__ Joined() {
+template <int D> struct Sums { float v[D / 32]; };
+template <int D> __device__ __forceinline__ Sums<D> load_part(const float* at, int lane) {  // a lane's values lie side by side
+    Sums<D> s;
+    if constexpr (D == 64) {
+        const float2 x = __ldcg(reinterpret_cast<const float2*>(at) + lane);
+        s.v[0] = x.x; s.v[1] = x.y;
+    } else {
 #pragma unroll
-        for (int i = 0; i < D / 32; ++i) o[i] = 0.f;
+        for (int i = 0; i < D / 128; ++i) {
+            const float4 x = __ldcg(reinterpret_cast<const float4*>(at) + lane * (D / 128) + i);
+            s.v[4 * i] = x.x; s.v[4 * i + 1] = x.y; s.v[4 * i + 2] = x.z; s.v[4 * i + 3] = x.w;
+        }
     }
-    __device__ __forceinline__ void add(const float2 ml, const float* part, int lane) {
-        if (ml.y == 0.f) return;  // sees nothing of the part, whatever its sums are
-        float v[D / 32];
-#pragma unroll
-        for (int i = 0; i < D / 32; ++i) v[i] = __ldcg(part + lane + 32 * i);
-        const float m = fmaxf(top, ml.x), mine = exp2f(top - m), theirs = exp2f(ml.x - m);
-        top = m;
-        l = l * mine + ml.y * theirs;
-#pragma unroll
-        for (int i = 0; i < D / 32; ++i) o[i] = o[i] * mine + v[i] * theirs;
-    }
-};
+    return s;
+}
 
 template <int D, class E>
-__global__ void __launch_bounds__(kMergeWarps * 32) paged_merge_kernel(const PagedAttentionArgs a) {
+__global__ void __launch_bounds__(kMergeWarps * 32) paged_merge_kernel(const __grid_constant__ PagedAttentionArgs a) {
     const PagedArgs& c = a.c;
     const int lane = threadIdx.x & 31;
-    const long long id = (long long)blockIdx.x * kMergeWarps + (threadIdx.x >> 5);
+    const int id = blockIdx.x * kMergeWarps + (threadIdx.x >> 5), r = id / c.n_q, h = id - r * c.n_q, head = divide(h, c.ratio_div);
     pdl_trigger();
     pdl_wait();
-    if (id >= (long long)c.rows * c.n_q) return;
-    const int r = (int)(id / c.n_q), h = (int)(id % c.n_q), head = h / c.ratio;
-    if (r >= first_row(c, c.n_seqs)) return;
+    if (r >= c.rows || r >= first_row(c, c.n_seqs)) return;
     int start = 0;
     const int s = warp_find_seq(c.row_start, c.n_seqs, c.rows, r, &start);
     if (s < 0) return;
-    const Seq seq = load_seq(c, s);
-    const int i = r - seq.row;
+    const Seq seq = {start, max(first_row(c, s + 1) - start, 0), tokens_of(c, s)};
+    const int i = r - start;
     if (i >= seq.n) return;
-    Joined<D> sum;
+    float top = kLowest, l = 0.f, o[D / 32];
+#pragma unroll
+    for (int k = 0; k < D / 32; ++k) o[k] = 0.f;
+#pragma unroll 1
     for (int x = 0; x < a.lines; ++x) {
         const PagedLine& line = a.line[x];
-        const long long total = line.cum[c.n_seqs + 1];
-        const int ctas = line_ctas(total, line.ctas);
-        for (int prefix = line.with_prefix ? 1 : 0; prefix >= 0; --prefix) {
-            if (!prefix && !line.with_own) continue;
+        const Share share(line.cum[c.n_seqs + 1], line.ctas);
+#pragma unroll 1
+        for (int prefix = line.with_prefix ? 1 : 0; prefix >= (line.with_own ? 0 : 1); --prefix) {
             // the item of this row and head: its first step on the line, and its steps
-            const int f = prefix ? r * c.ratio + h % c.ratio : i * c.ratio + h % c.ratio;
-            const int block = f / line.columns, col = f % line.columns;
-            long long at = prefix ? 0 : line.cum[s + 1];
-            int steps;
+            const int f = (prefix ? r : i) * c.ratio + h - head * c.ratio, block = f >> line.columns, col = f & ((1 << line.columns) - 1);
+            int at = prefix ? 0 : line.cum[s + 1], steps;
             if (prefix) {
-                steps = steps_of({(int)line.cum[c.n_seqs + 2], c.prefix_length}, line.keys);
-                at += (long long)block * c.n_kv * steps;
+                steps = steps_of({line.cum[c.n_seqs + 2], c.prefix_length}, line.keys);
+                at += block * c.n_kv * steps;
             } else {
-                for (int b = lane; b < block; b += 32) at += (long long)c.n_kv * steps_of(block_keys(seq, b, line.columns, c.ratio, a.window), line.keys);
-                const long long base = line.cum[s + 1];
-                at -= base;
+                int before = 0;
+                for (int b = lane; b < block; b += 32) before += c.n_kv * steps_of(block_keys(c, seq, b, line.columns, a.window), line.keys);
+                if (block) {
 #pragma unroll
-                for (int o = 16; o > 0; o >>= 1) at += __shfl_xor_sync(0xffffffffu, at, o);
-                at += base;
-                steps = steps_of(block_keys(seq, block, line.columns, c.ratio, a.window), line.keys);
+                    for (int k = 16; k > 0; k >>= 1) before += __shfl_xor_sync(0xffffffffu, before, k);
+                }
+                at += before;
+                steps = steps_of(block_keys(c, seq, block, line.columns, a.window), line.keys);
             }
             if (steps == 0) continue;
-            at += (long long)head * steps;
-            const int first = line_owner(total, at, ctas), last = line_owner(total, at + steps - 1, ctas);
-            if (first == last) {
-                if (!a.whole_o) return;  // written by the CTA that finished it
-                const size_t row = ((prefix ? (size_t)c.rows : 0) + r) * c.n_q + h;
-                sum.add(__ldcg(a.whole_ml + row), a.whole_o + row * D, lane);
-                continue;
-            }
-#pragma unroll 4
-            for (int cta = first; cta <= last; ++cta) {
-                const size_t slot = (size_t)(2 * cta + (at < line_begin(total, cta, ctas) ? 0 : 1)) * line.columns + col;
-                sum.add(__ldcg(line.slot_ml + slot), line.slot_o + slot * D, lane);
+            at += head * steps;
+            const int first = share.owner(at), last = share.owner(at + steps - 1);
+            const bool whole = first == last;
+            if (whole && !a.whole_o) return;  // written by the CTA that finished it
+            const size_t whole_at = ((prefix ? (size_t)c.rows : 0) + r) * c.n_q + h;
+            const int parts = last - first + 1;
+            const float* part0 = whole ? a.whole_o + whole_at * D : line.slot_o + (((size_t)(2 * first + (at < share.begin(first) ? 0 : 1)) << line.columns) + col) * D;
+            // every part but the first begins in front of its CTA's stretch: slot 0
+            const float* part1 = line.slot_o + (((size_t)(2 * (first + 1)) << line.columns) + col) * D;
+            const size_t stride = ((size_t)2 << line.columns) * D;
+#pragma unroll 1
+            for (int base = 0; base < parts; base += 32) {
+                const int k = base + lane;
+                float2 ml = make_float2(kLowest, 0.f);
+                if (k < parts) ml = whole ? __ldcg(a.whole_ml + whole_at) : __ldcg(line.slot_ml + ((size_t)(2 * (first + k) + (k == 0 && at >= share.begin(first) ? 1 : 0)) << line.columns) + col);
+                const bool counts = ml.y != 0.f;  // a part that the row sees nothing of adds nothing, whatever its sums are
+                const float here = counts ? ml.x : kLowest, m = fmaxf(top, warp_max(here)), mine = exp2_approx(top - m), factor = counts ? exp2_approx(here - m) : 0.f;
+                top = m;
+                l = l * mine + warp_sum(counts ? ml.y * factor : 0.f);
+#pragma unroll
+                for (int k2 = 0; k2 < D / 32; ++k2) o[k2] *= mine;
+                const uint32_t used = __ballot_sync(0xffffffffu, counts);
+                const int n = min(32, parts - base);
+#pragma unroll 1
+                for (int p = 0; p < n; p += 8) {
+                    Sums<D> v[8];
+#pragma unroll
+                    for (int y = 0; y < 8; ++y)
+                        if (p + y < n && (used >> (p + y) & 1u)) v[y] = load_part<D>(base + p + y == 0 ? part0 : part1 + (size_t)(base + p + y - 1) * stride, lane);
+#pragma unroll
+                    for (int y = 0; y < 8; ++y) {
+                        const float w = __shfl_sync(0xffffffffu, factor, (p + y) & 31);
+                        if (p + y < n && (used >> (p + y) & 1u)) {
+#pragma unroll
+                            for (int k2 = 0; k2 < D / 32; ++k2) o[k2] += v[y].v[k2] * w;
+                        }
+                    }
+                }
             }
         }
     }
-    E* out = static_cast<E*>(a.out) + (size_t)r * a.out_stride + (size_t)h * D;
+    const float rate = l > 0.f ? 1.f / l : l;  // l = 0: nothing was seen; NaN: what was seen is not a number
+    uint32_t w[D / 64];
 #pragma unroll
-    for (int k = 0; k < D / 32; ++k) out[lane + 32 * k] = round_to<E>(sum.l > 0.f ? sum.o[k] / sum.l : (sum.l == 0.f ? 0.f : sum.l));
+    for (int k = 0; k < D / 64; ++k) w[k] = l == 0.f ? 0u : TileElem<E>::pack(o[2 * k] * rate, o[2 * k + 1] * rate);
+    E* out = static_cast<E*>(a.out) + (size_t)r * a.out_stride + (size_t)h * D + lane * (D / 32);
+    if constexpr (D == 64) *reinterpret_cast<uint32_t*>(out) = w[0];
+    else if constexpr (D == 128) *reinterpret_cast<uint2*>(out) = make_uint2(w[0], w[1]);
+    else *reinterpret_cast<uint4*>(out) = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
 template <class Kernel, class... Args>
@@ -480,22 +542,18 @@ cudaError_t narrow(const Launch& l, PagedType type, const PagedAttentionArgs& a,
 
 }  // namespace
 
-int paged_narrow_columns(int head_dim, int64_t columns) {
-    const int most = head_dim == 256 ? 16 : 32;
-    return columns <= 8 ? 8 : columns <= 16 ? 16 : most;
-}
-int paged_narrow_keys(int head_dim) { return (head_dim == 256 ? kWarps<256> : head_dim == 128 ? kWarps<128> : kWarps<64>) * 16; }
+int paged_narrow_columns(int head_dim, int64_t columns) { return columns <= 8 ? 3 : columns <= 16 || head_dim == 256 ? 4 : 5; }
+int paged_narrow_keys(int head_dim) { return head_dim == 256 ? 6 : 7; }  // 16 a warp
 
 cudaError_t launch_paged_narrow(const Launch& l, PagedType type, int head_dim, const PagedAttentionArgs& a, int line) {
-    const int groups = a.line[line].columns / 8;
+    const int groups = 1 << (a.line[line].columns - 3);
     if (head_dim == 64) return groups == 1 ? narrow<64, 1>(l, type, a, line) : groups == 2 ? narrow<64, 2>(l, type, a, line) : narrow<64, 4>(l, type, a, line);
     if (head_dim == 128) return groups == 1 ? narrow<128, 1>(l, type, a, line) : groups == 2 ? narrow<128, 2>(l, type, a, line) : narrow<128, 4>(l, type, a, line);
     return groups == 1 ? narrow<256, 1>(l, type, a, line) : narrow<256, 2>(l, type, a, line);
 }
 
 cudaError_t launch_paged_merge(const Launch& l, PagedType type, int head_dim, const PagedAttentionArgs& a) {
-    const long long warps = (long long)a.c.rows * a.c.n_q;
-    const int grid = (int)((warps + kMergeWarps - 1) / kMergeWarps);
+    const int grid = (a.c.rows * a.c.n_q + kMergeWarps - 1) / kMergeWarps;
     auto go = [&](auto f16, auto bf16) { return type == kPagedF16 ? launch(l, f16, grid, kMergeWarps * 32, 0, a) : launch(l, bf16, grid, kMergeWarps * 32, 0, a); };
     if (head_dim == 64) return go(paged_merge_kernel<64, __half>, paged_merge_kernel<64, __nv_bfloat16>);
     if (head_dim == 128) return go(paged_merge_kernel<128, __half>, paged_merge_kernel<128, __nv_bfloat16>);

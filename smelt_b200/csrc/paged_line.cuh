@@ -13,84 +13,88 @@ struct Range { int lo, hi; };  // keys [lo, hi)
 struct Seq { int row, n, length; };
 
 __device__ __forceinline__ int first_row(const PagedArgs& c, int s) { return min(max(c.row_start[s], 0), c.rows); }
-__device__ __forceinline__ Seq load_seq(const PagedArgs& c, int s) {
-    const int r0 = first_row(c, s), r1 = first_row(c, s + 1);
-    return {r0, max(r1 - r0, 0), min(max(c.length[s], 0), c.table_tokens)};
-}
-// Keys of its own pages that row i of a sequence sees.
+__device__ __forceinline__ int tokens_of(const PagedArgs& c, int s) { return min(max(c.length[s], 0), c.table_tokens); }
+// Keys of its own pages that row i of a sequence sees.  (Tokens and rows are below 2^30; a window beyond that is none.)
 __device__ __forceinline__ Range own_keys(const Seq& s, int i, uint32_t window) {
-    const int token = s.length - s.n + i, hi = max(token + 1, 0);
-    return {window ? (int)max(0ll, (long long)hi - (long long)window) : 0, hi};
+    const int hi = max(s.length - s.n + i + 1, 0);
+    return {window ? max(0, hi - (int)window) : 0, hi};
 }
 // Keys of a prefix of P tokens that row i sees; a row without a token of its own sees nothing.
 __device__ __forceinline__ Range prefix_keys(const Seq& s, int i, int P, uint32_t window) {
-    if (s.length - s.n + i < 0) return {0, 0};
-    if (!window) return {0, P};
-    const long long lo = (long long)P + (s.length - s.n + i) + 1 - (long long)window;
-    return {(int)min((long long)P, max(0ll, lo)), P};
+    const int token = s.length - s.n + i;
+    if (token < 0) return {0, 0};
+    return {window ? min(P, max(0, P - (int)window + token + 1)) : 0, P};
 }
 // Keys that some row of a block of a sequence sees.
-__device__ __forceinline__ Range block_keys(const Seq& s, int block, int columns, int ratio, uint32_t window) {
-    const int f0 = block * columns, f1 = min(s.n * ratio, f0 + columns) - 1;
-    const Range a = own_keys(s, f0 / ratio, window), b = own_keys(s, f1 / ratio, window);
-    return {a.lo, b.hi};
+__device__ __forceinline__ Range block_keys(const PagedArgs& c, const Seq& s, int block, int columns, uint32_t window) {
+    const int f0 = block << columns, f1 = min(s.n * c.ratio, f0 + (1 << columns)) - 1;
+    return {own_keys(s, divide(f0, c.ratio_div), window).lo, own_keys(s, divide(f1, c.ratio_div), window).hi};
 }
-__device__ __forceinline__ int blocks_of(int rows, int ratio, int columns) { return (rows * ratio + columns - 1) / columns; }
-__device__ __forceinline__ int steps_of(const Range& r, int keys) { return r.hi > r.lo ? (r.hi - 1) / keys - r.lo / keys + 1 : 0; }
+__device__ __forceinline__ int blocks_of(const PagedArgs& c, int rows, int columns) { return (rows * c.ratio + (1 << columns) - 1) >> columns; }
+__device__ __forceinline__ int steps_of(const Range& r, int keys) { return r.hi > r.lo ? ((r.hi - 1) >> keys) - (r.lo >> keys) + 1 : 0; }
+// Steps of all blocks of a sequence, those of one key head.
+__device__ __forceinline__ int steps_of_seq(const PagedArgs& c, const PagedLine& line, const Seq& s, int blocks, uint32_t window) {
+    int sum = 0;
+    for (int k = 0; k < blocks; ++k) sum += steps_of(block_keys(c, s, k, line.columns, window), line.keys);
+    return sum;
+}
 
 // What a CTA holds of the batch in shared memory.
 struct Batch {
-    long long* cum;  // [n_seqs + 2]: steps in front of source 0 (the prefix), 1 (sequence 0), ..., and all of them
-    int* row;        // [n_seqs + 1]
-    int* length;     // [n_seqs]
+    int* cum;     // [n_seqs + 2]: steps in front of source 0 (the prefix), 1 (sequence 0), ..., and all of them
+    int* row;     // [n_seqs + 1]
+    int* length;  // [n_seqs]
     int prefix_lo;
     __device__ __forceinline__ Seq seq(int s) const { return {row[s], max(row[s + 1] - row[s], 0), length[s]}; }
 };
-__host__ __device__ constexpr size_t batch_bytes(int n_seqs) { return ((size_t)(n_seqs + 2) * 8 + (size_t)(2 * n_seqs + 1) * 4 + 15) & ~(size_t)15; }
+__host__ __device__ constexpr size_t batch_bytes(int n_seqs) { return ((size_t)(3 * n_seqs + 3) * 4 + 15) & ~(size_t)15; }
 
 // Fills `b` (every thread of the CTA calls it; the sums end behind a barrier).
 template <int THREADS>
 __device__ __forceinline__ void scan_line(const PagedArgs& c, const PagedLine& line, uint32_t window, Batch& b, unsigned char* memory) {
-    __shared__ long long warp_sums[THREADS / 32];
+    __shared__ int warp_sums[THREADS / 32];
     __shared__ int lowest;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n = c.n_seqs;
-    b.cum = reinterpret_cast<long long*>(memory);
-    b.row = reinterpret_cast<int*>(b.cum + n + 2);
+    b.cum = reinterpret_cast<int*>(memory);
+    b.row = b.cum + n + 2;
     b.length = b.row + n + 1;
     if (tid == 0) lowest = c.prefix_length;
     for (int s = tid; s <= n; s += THREADS) {
         b.row[s] = first_row(c, s);
-        if (s < n) b.length[s] = min(max(c.length[s], 0), c.table_tokens);
+        if (s < n) b.length[s] = tokens_of(c, s);
     }
     __syncthreads();
-    const int per = (n + THREADS - 1) / THREADS, s0 = tid * per, s1 = min(n, s0 + per);
-    long long mine = 0;
+    const int per = (n + THREADS - 1) / THREADS, s0 = min(n, tid * per), s1 = min(n, s0 + per);
+    int mine = 0;
     for (int s = s0; s < s1; ++s) {
         const Seq q = b.seq(s);
-        if (line.with_own)
-            for (int k = 0, nb = blocks_of(q.n, c.ratio, line.columns); k < nb; ++k) mine += (long long)c.n_kv * steps_of(block_keys(q, k, line.columns, c.ratio, window), line.keys);
+        if (line.with_own) mine += c.n_kv * steps_of_seq(c, line, q, blocks_of(c, q.n, line.columns), window);
         if (line.with_prefix && window && q.n) atomicMin(&lowest, prefix_keys(q, 0, c.prefix_length, window).lo);
     }
-    long long run = mine;
+    int run = mine;
+    if (n > 1) {
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const long long v = __shfl_up_sync(0xffffffffu, run, o);
-        if (lane >= o) run += v;
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, run, o);
+            if (lane >= o) run += v;
+        }
     }
     if (lane == 31) warp_sums[warp] = run;
     __syncthreads();
     b.prefix_lo = window ? lowest : 0;
-    long long before = run - mine;
-    for (int w = 0; w < warp; ++w) before += warp_sums[w];
-    const int total_rows = b.row[n];
-    if (line.with_prefix)
-        before += (long long)c.n_kv * blocks_of(total_rows, c.ratio, line.columns) * steps_of({b.prefix_lo, c.prefix_length}, line.keys);
+    int before = run - mine;
+    if (n > 32 * per)
+        for (int w = 0; w < warp; ++w) before += warp_sums[w];
+    if (line.with_prefix) before += c.n_kv * blocks_of(c, b.row[n], line.columns) * steps_of({b.prefix_lo, c.prefix_length}, line.keys);
     if (tid == 0) { b.cum[0] = 0; b.cum[1] = before; }
-    for (int s = s0; s < s1; ++s) {
-        const Seq q = b.seq(s);
-        if (line.with_own)
-            for (int k = 0, nb = blocks_of(q.n, c.ratio, line.columns); k < nb; ++k) before += (long long)c.n_kv * steps_of(block_keys(q, k, line.columns, c.ratio, window), line.keys);
-        b.cum[s + 2] = before;
+    if (per == 1) {
+        if (s0 < s1) b.cum[s0 + 2] = before + mine;
+    } else {
+        for (int s = s0; s < s1; ++s) {
+            const Seq q = b.seq(s);
+            if (line.with_own) before += c.n_kv * steps_of_seq(c, line, q, blocks_of(c, q.n, line.columns), window);
+            b.cum[s + 2] = before;
+        }
     }
     __syncthreads();
     if (blockIdx.x == 0) {
@@ -99,6 +103,18 @@ __device__ __forceinline__ void scan_line(const PagedArgs& c, const PagedLine& l
     }
 }
 
+// Who has which steps of the line: the first `more` CTAs have each + 1, the others `each`; CTAs beyond `ctas` have none, so that none between
+// two owners of an item is without.
+struct Share {
+    int ctas, each, more;
+    __device__ __forceinline__ Share(int total, int most) : ctas(min(total, most)), each(ctas ? total / ctas : 0), more(total - each * ctas) {}
+    __device__ __forceinline__ int begin(int cta) const { return each * cta + min(cta, more); }
+    __device__ __forceinline__ int owner(int at) const {
+        const int first = more * (each + 1);
+        return at < first ? at / (each + 1) : more + (at - first) / each;
+    }
+};
+
 // A place on the line: a step of an item.
 struct Cursor {
     int source, block, head, step, steps, first;  // source 0: the prefix, s + 1: sequence s; first: step of the item's first key
@@ -106,15 +122,15 @@ struct Cursor {
     int n_blocks;
 
     __device__ __forceinline__ void load_block(const PagedArgs& c, const PagedLine& line, uint32_t window, const Batch& b) {
-        keys = source == 0 ? Range{b.prefix_lo, c.prefix_length} : block_keys(b.seq(source - 1), block, line.columns, c.ratio, window);
+        keys = source == 0 ? Range{b.prefix_lo, c.prefix_length} : block_keys(c, b.seq(source - 1), block, line.columns, window);
         steps = steps_of(keys, line.keys);
-        first = keys.lo / line.keys;
+        first = keys.lo >> line.keys;
     }
     __device__ __forceinline__ void load_source(const PagedArgs& c, const PagedLine& line, const Batch& b) {
-        n_blocks = source == 0 ? blocks_of(b.row[c.n_seqs], c.ratio, line.columns) : blocks_of(b.seq(source - 1).n, c.ratio, line.columns);
+        n_blocks = blocks_of(c, source == 0 ? b.row[c.n_seqs] : b.seq(source - 1).n, line.columns);
     }
     // at < cum[n_seqs + 1]
-    __device__ __forceinline__ void seek(const PagedArgs& c, const PagedLine& line, uint32_t window, const Batch& b, long long at) {
+    __device__ __forceinline__ void seek(const PagedArgs& c, const PagedLine& line, uint32_t window, const Batch& b, int at) {
         int lo = 0, hi = c.n_seqs;  // the last source with cum <= at
         while (lo < hi) {
             const int mid = (lo + hi + 1) >> 1;
@@ -123,15 +139,15 @@ struct Cursor {
         }
         source = lo;
         load_source(c, line, b);
-        long long rest = at - b.cum[source];
+        int rest = at - b.cum[source];
         for (block = 0;; ++block) {
             load_block(c, line, window, b);
-            const long long here = (long long)c.n_kv * steps;
+            const int here = c.n_kv * steps;
             if (rest < here || block + 1 >= n_blocks) break;
             rest -= here;
         }
-        head = (int)(rest / steps);
-        step = (int)(rest - (long long)head * steps);
+        head = rest / steps;
+        step = rest - head * steps;
     }
     // To the next step; there is one.
     __device__ __forceinline__ void advance(const PagedArgs& c, const PagedLine& line, uint32_t window, const Batch& b) {
@@ -150,17 +166,6 @@ struct Cursor {
     }
     __device__ __forceinline__ bool same_item(const Cursor& o) const { return source == o.source && block == o.block && head == o.head; }
 };
-
-// The CTAs that have work: with fewer steps than CTAs one step each, so that none between two owners of an item is without.
-__device__ __forceinline__ int line_ctas(long long total, int ctas) { return total < ctas ? (int)total : ctas; }
-__device__ __forceinline__ long long line_begin(long long total, int cta, int ctas) { return total * cta / ctas; }
-// The CTA that has step `at` of the line.
-__device__ __forceinline__ int line_owner(long long total, long long at, int ctas) {
-    int c = (int)(at * ctas / total);
-    while (c + 1 < ctas && line_begin(total, c + 1, ctas) <= at) ++c;
-    while (c > 0 && line_begin(total, c, ctas) > at) --c;
-    return c;
-}
 
 // The sequence of a packed row, from row starts in shared memory.
 __device__ __forceinline__ int seq_of_row(const Batch& b, int n_seqs, int row) {

@@ -30,7 +30,6 @@ struct Cfg {
     static constexpr int kSets = D == 256 ? 1 : 2;   // of four softmax warps, each with an accumulator of its own
     static constexpr int kKeys = D == 256 ? 64 : 128;
     static constexpr int kStages = D == 64 ? 3 : 2;
-    static constexpr int kColumns = kSets * 128;
     static constexpr int kQTile = 128 * D * 2, kTile = kKeys * D * 2;
     static constexpr int kLoadWarp = kSets * 4, kMmaWarp = kLoadWarp + 4, kThreads = (kMmaWarp + 1) * 32;
     static constexpr int kSum = 2 * kKeys;  // first column of the accumulators: behind two of scores
@@ -42,7 +41,7 @@ struct Shared {  // behind the tiles
     uint32_t keep[2];    // the first product of an item adds to what its set has put into the accumulator
     uint32_t odd[3][4];  // keys of a stage's step whose values are not finite, and were taken out
     float2 ml[2][128];
-    long long row[128];  // of a step's keys in the pools, in elements (head 0); -1: none
+    long long row[2][128];  // of a step's keys in the pools, in elements (head 0); -1: none
 };
 template <int D>
 constexpr size_t wide_shared(int n_seqs) {
@@ -133,10 +132,10 @@ struct Item {
 __device__ __forceinline__ Item item_of(const PagedArgs& c, const PagedLine& line, uint32_t window, const Batch& b, const Cursor& cur) {
     Item it;
     it.seq = cur.source == 0 ? Seq{0, b.row[c.n_seqs], 0} : b.seq(cur.source - 1);
-    it.f0 = cur.block * line.columns;
-    it.width = min(line.columns, it.seq.n * c.ratio - it.f0);
+    it.f0 = cur.block << line.columns;
+    it.width = min(1 << line.columns, it.seq.n * c.ratio - it.f0);
     // of the prefix: without a window all columns, but for rows without a token, whose sums are dropped
-    it.clear = cur.source ? Range{own_keys(it.seq, (it.f0 + it.width - 1) / c.ratio, window).lo, own_keys(it.seq, it.f0 / c.ratio, window).hi} : window ? Range{0, 0} : Range{0, c.prefix_length};
+    it.clear = cur.source ? Range{own_keys(it.seq, divide(it.f0 + it.width - 1, c.ratio_div), window).lo, own_keys(it.seq, divide(it.f0, c.ratio_div), window).hi} : window ? Range{0, 0} : Range{0, c.prefix_length};
     return it;
 }
 
@@ -172,9 +171,8 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_wide_kernel(const P
     scan_line<C::kThreads>(c, line, a.window, batch, reinterpret_cast<unsigned char*>(&sh) + ((sizeof(Shared) + 15) & ~(size_t)15));
     tc_fence_after();
     const uint32_t tmem = (uint32_t)uniform((int)sh.tmem);
-    const long long total = batch.cum[c.n_seqs + 1];
-    const int ctas = line_ctas(total, line.ctas);
-    const long long begin = (int)blockIdx.x < ctas ? line_begin(total, blockIdx.x, ctas) : 0, end = (int)blockIdx.x < ctas ? line_begin(total, blockIdx.x + 1, ctas) : 0;
+    const Share share(batch.cum[c.n_seqs + 1], line.ctas);
+    const int begin = (int)blockIdx.x < share.ctas ? share.begin(blockIdx.x) : 0, end = (int)blockIdx.x < share.ctas ? share.begin(blockIdx.x + 1) : 0;
     // A role that gives up a wait goes through the rest of its schedule without work, so that no barrier is short of a thread.
     bool alive = true;
     // An item's steps in this CTA: tasks, one a step, or with two tiles one a tile and step; task T of the CTA has score buffer T & 1.
@@ -183,8 +181,8 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_wide_kernel(const P
         Cursor cur;
         cur.seek(c, line, a.window, batch, begin);
         uint32_t task = 0, step = 0;
-        for (long long pos = begin; pos < end;) {
-            const int n = (int)min((long long)(cur.steps - cur.step), end - pos);
+        for (int pos = begin; pos < end;) {
+            const int n = min(cur.steps - cur.step, end - pos);
             const Item it = item_of(c, line, a.window, batch, cur);
             const bool pair = it.width > 128;
             const int tasks = pair ? 2 * n : n;
@@ -211,7 +209,6 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_wide_kernel(const P
             __syncwarp();
             if (lane == 0) mbar_arrive(bar);
         };
-        const uint32_t flip = a.scale2 < 0.f ? 0x80008000u : 0u;  // the softmax wants a positive scale
         uint32_t items = 0;
         int v_behind = -1;        // stage of the values that were asked for last and not handed over yet
         bool v_check = false;     // ... that not every column sees all of
@@ -231,48 +228,57 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_wide_kernel(const P
             arrive(&sh.v_full[v_behind]);
             v_behind = -1;
         };
-        each_item([&](const Cursor& cur, const Item& it, bool pair, int n, int, uint32_t, uint32_t step0, long long) {
+        each_item([&](const Cursor& cur, const Item& it, bool pair, int n, int, uint32_t, uint32_t step0, int) {
             // queries, behind everything that was asked for before them
             cp_async_wait<0>();
             hand_over_values();
             if (items > 0) warp_wait(&sh.q_empty, (items - 1) & 1);
             ++items;
             if (alive) {
-                for (int f = r_first; f < (pair ? 256 : 128); f += ROWS)
-                    for (int k = ch; k < CHUNKS; k += LANES) {
-                        uint4 v = make_uint4(0, 0, 0, 0);
-                        if (f < it.width) {
-                            const int ff = it.f0 + f;
-                            v = *reinterpret_cast<const uint4*>(static_cast<const E*>(a.q) + (size_t)(it.seq.row + ff / c.ratio) * a.q_stride + (size_t)(cur.head * c.ratio + ff % c.ratio) * D + 8 * k);
-                            v.x ^= flip; v.y ^= flip; v.z ^= flip; v.w ^= flip;
+                for (int f = r_first; f < (pair ? 256 : 128); f += ROWS) {
+                    const int ff = it.f0 + f, i = divide(ff, c.ratio_div);
+                    const bool live = f < it.width;
+                    const E* from = static_cast<const E*>(a.q) + (live ? (size_t)(it.seq.row + i) * a.q_stride + (size_t)(cur.head * c.ratio + ff - i * c.ratio) * D : 0);
+                    const uint32_t to = smem_u32(q_tiles + (f >> 7) * C::kQTile);
+                    for (int k = ch; k < CHUNKS; k += LANES) copy16(to + place(128, f & 127, k), from + 8 * k, live);
+                }
+                cp_async_commit();
+                cp_async_wait<0>();
+                if (a.scale2 < 0.f)  // the softmax wants a positive scale
+                    for (int f = r_first; f < (pair ? 256 : 128); f += ROWS)
+                        for (int k = ch; k < CHUNKS; k += LANES) {
+                            uint4* v = reinterpret_cast<uint4*>(q_tiles + (f >> 7) * C::kQTile + place(128, f & 127, k));
+                            *v = make_uint4(v->x ^ 0x80008000u, v->y ^ 0x80008000u, v->z ^ 0x80008000u, v->w ^ 0x80008000u);
                         }
-                        *reinterpret_cast<uint4*>(q_tiles + (f >> 7) * C::kQTile + place(128, f & 127, k)) = v;
-                    }
             }
             arrive(&sh.q_full);
             const int32_t* table = cur.source == 0 ? c.prefix_table : c.table + (size_t)(cur.source - 1) * c.table_stride;
             const long long head_at = (long long)cur.head * c.head_stride;
+            // where the key of this thread lies, a step ahead
+            auto look_up = [&](int i) {
+                const int key = (cur.first + cur.step + i) * KEYS + lt;
+                long long at = -1;
+                if (lt < KEYS && i < n && key >= cur.keys.lo && key < cur.keys.hi) {
+                    const int p = divide(key, c.page_div), page = table[p];
+                    if ((uint32_t)page < (uint32_t)c.n_pages) at = (long long)page * c.page_stride + (long long)(key - p * c.page_size) * c.token_stride + head_at;
+                    else if (c.err) atomicOr(c.err, KERR_BAD_PAGE);
+                }
+                return at;
+            };
+            long long ahead = look_up(0);
             for (int i = 0; i < n; ++i) {
                 const uint32_t step = step0 + i, s = step % S, use = step / S;
                 const int k0 = (cur.first + cur.step + i) * KEYS;
-                barrier(1, 128);  // the rows of the step before have been read
-                if (lt < KEYS) {
-                    const int key = k0 + lt;
-                    long long at = -1;
-                    if (key >= cur.keys.lo && key < cur.keys.hi) {
-                        const int p = divide(key, c.page_div), page = table[p];
-                        if ((uint32_t)page < (uint32_t)c.n_pages) at = (long long)page * c.page_stride + (long long)(key - p * c.page_size) * c.token_stride + head_at;
-                        else if (c.err) atomicOr(c.err, KERR_BAD_PAGE);
-                    }
-                    sh.row[lt] = at;
-                }
-                barrier(1, 128);
+                long long* rows = sh.row[step & 1];
+                if (lt < KEYS) rows[lt] = ahead;
+                barrier(1, 128);  // ... and the rows of the step before have been read: the other half may be written
+                ahead = look_up(i + 1);
                 auto copy = [&](const void* pool, unsigned char* tiles) {
                     const uint32_t dst = smem_u32(tiles + s * C::kTile);
                     if (alive) {
 #pragma unroll 4
                         for (int r = r_first; r < KEYS; r += ROWS) {
-                            const long long at = sh.row[r];
+                            const long long at = rows[r];
                             for (int k = ch; k < CHUNKS; k += LANES) copy16(dst + place(KEYS, r, k), static_cast<const E*>(pool) + max(at, 0ll) + 8 * k, at >= 0);
                         }
                     }
@@ -303,7 +309,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_wide_kernel(const P
             tc_fence_after();
         };
         uint32_t items = 0, done = 0;
-        each_item([&](const Cursor&, const Item&, bool pair, int, int tasks, uint32_t task0, uint32_t step0, long long) {
+        each_item([&](const Cursor&, const Item&, bool pair, int, int tasks, uint32_t task0, uint32_t step0, int) {
             wait(&sh.q_full, items & 1);
             ++items;
             auto scores = [&](int t) {
@@ -351,11 +357,11 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_wide_kernel(const P
             alive = __all_sync(0xffffffffu, alive && wait_alive(bar, parity, dead)) != 0;
             tc_fence_after();
         };
-        each_item([&](const Cursor& cur, const Item& it, bool pair, int n, int tasks, uint32_t task0, uint32_t step0, long long pos) {
+        each_item([&](const Cursor& cur, const Item& it, bool pair, int n, int tasks, uint32_t task0, uint32_t step0, int pos) {
             const int t_first = C::kSets == 1 ? 0 : (int)((task0 & 1) ^ set), f = (pair ? t_first * 128 : 0) + me, ff = it.f0 + f;
             Range keys = {0, 0};
             if (f < it.width) {
-                const int i = ff / c.ratio;
+                const int i = divide(ff, c.ratio_div);
                 if (cur.source) {
                     keys = own_keys(it.seq, i, a.window);
                 } else {
@@ -487,7 +493,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_wide_kernel(const P
             }
             // ── the item's sums ──
             if (any) wait(&sh.pv_done[last & 1], (last >> 1) & 1);
-            const long long item_at = pos - cur.step;
+            const int item_at = pos - cur.step;
             const bool here = item_at >= begin && item_at + cur.steps <= end;
             const bool both = C::kSets == 2 && !pair;
             float mine = 1.f;
@@ -501,11 +507,11 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_wide_kernel(const P
                 m = top;
             }
             const bool writer = !both || t_first == 0;
-            const size_t row = (size_t)it.seq.row + ff / c.ratio, head = (size_t)cur.head * c.ratio + ff % c.ratio;
+            const size_t row = (size_t)it.seq.row + divide(ff, c.ratio_div), head = (size_t)cur.head * c.ratio + ff - divide(ff, c.ratio_div) * c.ratio;
             float* part = nullptr;
             float2* part_ml = nullptr;
             if (!here) {
-                const size_t at = (size_t)(2 * blockIdx.x + (item_at < begin ? 0 : 1)) * line.columns + f;
+                const size_t at = ((size_t)(2 * blockIdx.x + (item_at < begin ? 0 : 1)) << line.columns) + f;
                 part = line.slot_o + at * D;
                 part_ml = line.slot_ml + at;
             } else if (a.whole_o) {
@@ -593,8 +599,8 @@ cudaError_t go(const Launch& l, const PagedAttentionArgs& a, int line) {
 
 }  // namespace
 
-int paged_wide_columns(int head_dim) { return head_dim == 256 ? Cfg<256>::kColumns : Cfg<128>::kColumns; }
-int paged_wide_keys(int head_dim) { return head_dim == 256 ? Cfg<256>::kKeys : Cfg<128>::kKeys; }
+int paged_wide_columns(int head_dim) { return head_dim == 256 ? 7 : 8; }
+int paged_wide_keys(int head_dim) { return head_dim == 256 ? 6 : 7; }
 bool paged_wide_takes(int head_dim, int n_seqs) {
     const size_t most = 227 * 1024 - 1024;  // less what the scan of the batch holds, up to the tiles' alignment
     return (head_dim == 64 ? wide_shared<64>(n_seqs) : head_dim == 128 ? wide_shared<128>(n_seqs) : wide_shared<256>(n_seqs)) <= most;
