@@ -7,15 +7,13 @@
 //
 // paged_narrow_kernel: one CTA a SM, each with as many steps of the line of work (paged.h).  A warp takes 16 keys of a step at a time as
 // S^T = K Q^T and O^T += V^T P^T on mma.sync: the columns of the block are the narrow side of the product, so eight columns cost what one
-// costs.  A lane brings a key's row with one bulk copy for K and one for V, wherever its page is, into a ring of the warp's own; rows lie 16
-// bytes more than their length apart, so that ldmatrix reads them without conflicts, and the warp waits on its own barriers
-// only.  The ring runs on across items, so that the pages of the next sequence are on their way while this one's warps join their sums.
+// costs.  Rows come with cp.async, wherever their pages are, into a ring of the warp's own, 16 bytes more than their length apart, so
+// that ldmatrix reads them without conflicts.  The ring runs on across items, so that the pages of the next sequence are on their way while this one's warps join their sums.
 // P goes into the product as two 16-bit parts: the kernel waits for memory, and rounding P once would cost up to half a step of the
 // 16-bit type.  Keys outside an item are not read (zeros), and a value row that is not finite reaches only the columns that see it.
 // paged_merge_kernel joins the items that several CTAs share, and the prefix with the sequences.
 #include "attention.cuh"
 #include "paged_line.cuh"
-#include "tcgen05.cuh"
 
 namespace smelt {
 namespace {
@@ -30,8 +28,8 @@ template <int D> constexpr int kPitch = D * 2 + 16;
 template <int D> constexpr int kUnitBytes = 16 * kPitch<D>;
 
 template <int D>
-constexpr size_t narrow_shared(int n_seqs) {  // rings, one column group's sums of all warps, their maxima and sums, barriers, the batch
-    return (size_t)kWarps<D> * kUnits<D> * kUnitBytes<D> + (size_t)kWarps<D> * 8 * (D + 1) * 4 + (size_t)kWarps<D> * 8 * 8 + (size_t)kWarps<D> * kUnits<D> * 8 + batch_bytes(n_seqs);
+constexpr size_t narrow_shared(int n_seqs) {  // rings, one column group's sums of all warps, their maxima and sums, rows of keys, the batch
+    return (size_t)kWarps<D> * kUnits<D> * kUnitBytes<D> + (size_t)kWarps<D> * 8 * (D + 1) * 4 + (size_t)kWarps<D> * 8 * 8 + (size_t)kWarps<D> * 16 * 8 + batch_bytes(n_seqs);
 }
 
 __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t at) {
@@ -44,6 +42,10 @@ __device__ __forceinline__ float exp2_approx(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+
+__device__ __forceinline__ void cp_async16_or_zero(uint32_t dst, const void* src, bool take) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(take ? 16 : 0) : "memory");
 }
 
 template <class E> __device__ __forceinline__ E round_to(float v);
@@ -89,18 +91,15 @@ __global__ void __launch_bounds__(kWarps<D> * 32, 1) paged_narrow_kernel(const _
     extern __shared__ __align__(16) unsigned char smem[];
     float* sums = reinterpret_cast<float*>(smem + (size_t)W * NU * UNIT);     // [W][8][D + 1]
     float2* state = reinterpret_cast<float2*>(sums + W * 8 * (D + 1));        // [W][8]
-    uint64_t* bars = reinterpret_cast<uint64_t*>(state + W * 8);              // [W][NU]
+    long long* rows_of = reinterpret_cast<long long*>(state + W * 8);         // [W][16]
     const PagedArgs& c = a.c;
     const PagedLine& line = a.line[which];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-    uint64_t* bar = bars + warp * NU;
-    if (lane < NU) mbar_init(bar + lane, 1);
-    mbar_fence_init();
-    fence_async_smem();
+    long long* rows = rows_of + warp * 16;
     pdl_trigger();
     pdl_wait();
     Batch batch;
-    scan_line<THREADS>(c, line, a.window, batch, reinterpret_cast<unsigned char*>(bars + W * NU));
+    scan_line<THREADS>(c, line, a.window, batch, reinterpret_cast<unsigned char*>(rows_of + W * 16));
     const Share share(batch.cum[c.n_seqs + 1], line.ctas);
     if ((int)blockIdx.x >= share.ctas) return;
     const int begin = share.begin(blockIdx.x), end = share.begin(blockIdx.x + 1);
@@ -127,34 +126,33 @@ __global__ void __launch_bounds__(kWarps<D> * 32, 1) paged_narrow_kernel(const _
         }
         if (++at < end) ahead.advance(c, line, a.window, batch);
     };
-    long long row = -1;  // of lane's key in the pools, in elements; -1: none
-    int rows = 0;        // of the tile that there are
+    constexpr int LANES = D / 8 < 32 ? D / 8 : 32, TURN = 32 / LANES;  // lanes of a row of 16-byte pieces, rows of a turn of the warp
+    const int piece = lane % LANES * 8, turn_row = lane / LANES;
     auto issue_unit = [&](int u, int place) {
-        unsigned char* dst = ring + place * UNIT + (lane & 15) * PITCH;
         if ((u & 1) == 0) {
-            row = -1;
+            long long row = -1;  // of lane's key in the pools, in elements; -1: none
             if (inside) {
                 if ((uint32_t)page < (uint32_t)c.n_pages) row = (long long)page * c.page_stride + (long long)slot * c.token_stride + (long long)head * c.head_stride;
                 else if (c.err && lane < 16) atomicOr(c.err, KERR_BAD_PAGE);
             }
-            rows = __popc(__ballot_sync(0xffffffffu, row >= 0) & 0xffffu);
+            if (lane < 16) rows[lane] = row;
             look_up();
         }
-        __syncwarp();  // the unit's last readers are through
-        if (rows < 16) {
-            if (row < 0 && lane < 16)
-                for (int i = 0; i < D * 2; i += 16) *reinterpret_cast<uint4*>(dst + i) = make_uint4(0, 0, 0, 0);
-            fence_async_smem();  // a copy writes there later
+        __syncwarp();  // the rows are there, and the unit's last readers are through
+        const E* pool = static_cast<const E*>((u & 1) == 0 ? c.k : c.v) + piece;
+        const uint32_t dst = smem_u32(ring + place * UNIT) + turn_row * PITCH + piece * 2;
+#pragma unroll
+        for (int i = 0; i < 16; i += TURN) {
+            const long long row = rows[i + turn_row];
+            cp_async16_or_zero(dst + i * PITCH, pool + max(row, 0ll), row >= 0);
         }
-        if (lane == 0) mbar_arrive_expect_tx(bar + place, rows * D * 2);
-        __syncwarp();
-        if (row >= 0 && lane < 16) bulk_g2s(dst, static_cast<const E*>((u & 1) == 0 ? c.k : c.v) + row, D * 2, bar + place);
     };
     look_up();
     const int n_units = 2 * (end - begin);
     int issued = 0, issue_place = 0;  // the next unit to issue, and its place in the ring
     auto issue_next = [&]() {
         if (issued < n_units) issue_unit(issued, issue_place);
+        cp_async_commit();
         ++issued;
         if (++issue_place == NU) issue_place = 0;
     };
@@ -169,15 +167,14 @@ __global__ void __launch_bounds__(kWarps<D> * 32, 1) paged_narrow_kernel(const _
     Seq seq{0, 0, 0};
     int width = 0;  // columns of the block
     int use_place = 0;
-    uint32_t use_phase = 0;
-    bool alive = true;
     // ldmatrix: this lane's row of a tile of keys (as they are) and of values (turned)
     const uint32_t k_lane = smem_u32(ring) + ((lane & 7) + ((lane >> 3) & 1) * 8) * PITCH + (lane >> 4) * 16;
     const uint32_t v_lane = smem_u32(ring) + ((lane & 7) + (lane >> 4) * 8) * PITCH + ((lane >> 3) & 1) * 16;
-    auto arrived = [&]() {  // the unit at use_place, which it leaves in `place`
-        alive = alive && mbar_poll_bounded(bar + use_place, use_phase);
+    auto arrived = [&]() {  // the place of the next unit, which is there; as many have been asked for behind it as the ring holds less two
+        cp_async_wait<NU - 2>();
+        __syncwarp();
         const int place = use_place;
-        if (++use_place == NU) { use_place = 0; use_phase ^= 1u; }
+        if (++use_place == NU) use_place = 0;
         return place;
     };
 
@@ -400,7 +397,7 @@ __global__ void __launch_bounds__(kWarps<D> * 32, 1) paged_narrow_kernel(const _
             __syncthreads();
         }
     }
-    if (!alive && lane == 0 && c.err) atomicOr(c.err, 0x1000u);
+    cp_async_wait<0>();
 }
 
 // ── the join ────────────────────────────────────────────────────────────────
