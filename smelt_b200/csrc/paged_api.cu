@@ -62,11 +62,11 @@ size_t attention_plan(const smelt_cuda_ctx* ctx, const smelt_paged_cache* k, con
         at += (bytes + 15) & ~(size_t)15;
         return p;
     };
-    // Columns of a source: up to 32 on the streaming kernel (16 with heads of 256), more on the tensor core.  A launch takes sequences and
+    // Columns of a source: up to 2048 / head_dim on the streaming kernel, more on the tensor core.  A launch takes sequences and
     // prefix together where they go to the same kernel.
     const int64_t own = (int64_t)(b->max_rows > 0 ? b->max_rows : 1) * a->c.ratio, prefix = b->prefix_length > 0 ? (int64_t)b->rows * a->c.ratio : 0;
     const bool can = paged_wide_takes(D, b->n_seqs);
-    const int64_t most = D == 256 ? 16 : 32;
+    const int64_t most = 2048 / D;
     const bool own_wide = can && own > most, prefix_wide = can && prefix > most;
     a->lines = 0;
     auto add = [&](bool wide, bool with_own, bool with_prefix) {

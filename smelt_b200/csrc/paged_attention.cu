@@ -5,7 +5,7 @@
 // with the running maximum and sum of the softmax, so that keys and values are read once.  This file has the streaming kernel for blocks
 // of few columns (a column is a row and a query head of the group that shares a key head) and the kernel that joins shared items.
 //
-// paged_narrow_kernel: one CTA a SM, each with as many steps of the line of work (paged.h).  A warp takes 16 keys of a step at a time as
+// paged_narrow_kernel: one CTA a SM, each with as many steps of the line of work (paged.h).  A warp takes 32 keys of a step at a time as
 // S^T = K Q^T and O^T += V^T P^T on mma.sync: the columns of the block are the narrow side of the product, so eight columns cost what one
 // costs.  Rows come with cp.async, wherever their pages are, into a ring of the warp's own, 16 bytes more than their length apart, so
 // that ldmatrix reads them without conflicts.  The ring runs on across items, so that the pages of the next sequence are on their way while this one's warps join their sums.
@@ -23,13 +23,14 @@ using attn::movmatrix_trans;
 using attn::TileElem;
 
 template <int D> constexpr int kWarps = D == 256 ? 4 : 8;
+constexpr int kGroups = 2;                                 // of 16 keys a tile: a chain of products, exchange and exponentials takes two as fast as one
 template <int D> constexpr int kUnits = D == 64 ? 10 : 5;  // of a warp's ring: the K or V rows of 16 keys each
 template <int D> constexpr int kPitch = D * 2 + 16;
 template <int D> constexpr int kUnitBytes = 16 * kPitch<D>;
 
 template <int D>
 constexpr size_t narrow_shared(int n_seqs) {  // rings, one column group's sums of all warps, their maxima and sums, rows of keys, the batch
-    return (size_t)kWarps<D> * kUnits<D> * kUnitBytes<D> + (size_t)kWarps<D> * 8 * (D + 1) * 4 + (size_t)kWarps<D> * 8 * 8 + (size_t)kWarps<D> * 16 * 8 + batch_bytes(n_seqs);
+    return (size_t)kWarps<D> * kUnits<D> * kUnitBytes<D> + (size_t)kWarps<D> * 8 * (D + 1) * 4 + (size_t)kWarps<D> * 8 * 8 + (size_t)kWarps<D> * 16 * kGroups * 8 + batch_bytes(n_seqs);
 }
 
 __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t at) {
@@ -44,6 +45,9 @@ __device__ __forceinline__ float exp2_approx(float x) {
     return y;
 }
 
+constexpr uint32_t kHidden = 0x7FFFF00Du;  // a NaN of our own
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory"); }
 __device__ __forceinline__ void cp_async16_or_zero(uint32_t dst, const void* src, bool take) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(take ? 16 : 0) : "memory");
 }
@@ -87,35 +91,36 @@ __device__ __noinline__ void weighted_sum_masked(uint32_t values, MaskedTile<D, 
 
 template <int D, int NH, class E>
 __global__ void __launch_bounds__(kWarps<D> * 32, 1) paged_narrow_kernel(const __grid_constant__ PagedAttentionArgs a, const int which) {
-    constexpr int W = kWarps<D>, THREADS = W * 32, NU = kUnits<D>, UNIT = kUnitBytes<D>, PITCH = kPitch<D>, KEYS = W * 16, MT = D / 16;
+    constexpr int W = kWarps<D>, THREADS = W * 32, NU = kUnits<D>, UNIT = kUnitBytes<D>, PITCH = kPitch<D>, TILE = 16 * kGroups, KEYS = W * TILE, MT = D / 16;
     extern __shared__ __align__(16) unsigned char smem[];
     float* sums = reinterpret_cast<float*>(smem + (size_t)W * NU * UNIT);     // [W][8][D + 1]
     float2* state = reinterpret_cast<float2*>(sums + W * 8 * (D + 1));        // [W][8]
-    long long* rows_of = reinterpret_cast<long long*>(state + W * 8);         // [W][16]
+    long long* rows_of = reinterpret_cast<long long*>(state + W * 8);         // [W][TILE]
     const PagedArgs& c = a.c;
     const PagedLine& line = a.line[which];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-    long long* rows = rows_of + warp * 16;
+    long long* rows = rows_of + warp * TILE;
     pdl_trigger();
     pdl_wait();
     Batch batch;
-    scan_line<THREADS>(c, line, a.window, batch, reinterpret_cast<unsigned char*>(rows_of + W * 16));
+    scan_line<THREADS>(c, line, a.window, batch, reinterpret_cast<unsigned char*>(rows_of + W * TILE));
     const Share share(batch.cum[c.n_seqs + 1], line.ctas);
     if ((int)blockIdx.x >= share.ctas) return;
     const int begin = share.begin(blockIdx.x), end = share.begin(blockIdx.x + 1);
 
-    // ── the ring: unit u holds K (even) or V (odd) of this warp's tile of step begin + u / 2 ──
+    // ── the ring: of every tile kGroups units of keys, then kGroups of values ──
+    static_assert(TILE == 32, "a lane a key");
     unsigned char* ring = smem + (size_t)warp * NU * UNIT;
     Cursor cur;
     cur.seek(c, line, a.window, batch, begin);
-    Cursor ahead = cur;  // the step whose page is looked up next
+    Cursor ahead = cur;  // the step whose pages are looked up next
     int at = begin;
-    int page = 0, slot = 0, head = 0;  // lane i (and i + 16): page and place of key i of the tile that is issued next
+    int page = 0, slot = 0, head = 0;  // page and place of the lane's key of the tile that is issued next
     bool inside = false;               // ... which is one of the item's
     auto look_up = [&]() {
         inside = false;
         if (at >= end) return;
-        const int key = (ahead.first + ahead.step) * KEYS + warp * 16 + (lane & 15);
+        const int key = (ahead.first + ahead.step) * KEYS + warp * TILE + lane;
         head = ahead.head;
         inside = key >= ahead.keys.lo && key < ahead.keys.hi;
         if (inside) {
@@ -127,37 +132,42 @@ __global__ void __launch_bounds__(kWarps<D> * 32, 1) paged_narrow_kernel(const _
         if (++at < end) ahead.advance(c, line, a.window, batch);
     };
     constexpr int LANES = D / 8 < 32 ? D / 8 : 32, TURN = 32 / LANES;  // lanes of a row of 16-byte pieces, rows of a turn of the warp
-    const int piece = lane % LANES * 8, turn_row = lane / LANES;
-    auto issue_unit = [&](int u, int place) {
-        if ((u & 1) == 0) {
-            long long row = -1;  // of lane's key in the pools, in elements; -1: none
-            if (inside) {
-                if ((uint32_t)page < (uint32_t)c.n_pages) row = (long long)page * c.page_stride + (long long)slot * c.token_stride + (long long)head * c.head_stride;
-                else if (c.err && lane < 16) atomicOr(c.err, KERR_BAD_PAGE);
-            }
-            if (lane < 16) rows[lane] = row;
+    const int turn_row = lane / LANES;
+    const E *k_pool = static_cast<const E*>(c.k) + lane % LANES * 8, *v_pool = static_cast<const E*>(c.v) + lane % LANES * 8;
+    const uint32_t ring_at = smem_u32(ring) + turn_row * PITCH + lane % LANES * 16;
+    uint32_t there = 0;  // keys of the tile that are read; the others' rows are zeros
+    auto issue_unit = [&](int w, int place) {  // unit w of a tile
+        if (w == 0) {
+            bool take = inside && (uint32_t)page < (uint32_t)c.n_pages;
+            if (inside && !take && c.err) atomicOr(c.err, KERR_BAD_PAGE);
+            rows[lane] = take ? (long long)page * c.page_stride + (long long)slot * c.token_stride + (long long)head * c.head_stride : 0;
+            there = __ballot_sync(0xffffffffu, take);
             look_up();
         }
         __syncwarp();  // the rows are there, and the unit's last readers are through
-        const E* pool = static_cast<const E*>((u & 1) == 0 ? c.k : c.v) + piece;
-        const uint32_t dst = smem_u32(ring + place * UNIT) + turn_row * PITCH + piece * 2;
+        const E* pool = w < kGroups ? k_pool : v_pool;
+        const uint32_t dst = ring_at + place * UNIT;
+        const long long* row = rows + w % kGroups * 16 + turn_row;
+        const uint32_t mine = there >> (w % kGroups * 16) & 0xffffu;
+        if (mine == 0xffffu) {
 #pragma unroll
-        for (int i = 0; i < 16; i += TURN) {
-            const long long row = rows[i + turn_row];
-            cp_async16_or_zero(dst + i * PITCH, pool + max(row, 0ll), row >= 0);
+            for (int i = 0; i < 16; i += TURN) cp_async16(dst + i * PITCH, pool + row[i]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 16; i += TURN) cp_async16_or_zero(dst + i * PITCH, pool + row[i], mine >> (i + turn_row) & 1u);
         }
     };
     look_up();
-    const int n_units = 2 * (end - begin);
+    const int n_units = 2 * kGroups * (end - begin);
     int issued = 0, issue_place = 0;  // the next unit to issue, and its place in the ring
     auto issue_next = [&]() {
-        if (issued < n_units) issue_unit(issued, issue_place);
+        if (issued < n_units) issue_unit(issued % (2 * kGroups), issue_place);
         cp_async_commit();
         ++issued;
         if (++issue_place == NU) issue_place = 0;
     };
 #pragma unroll 1
-    for (int i = 0; i < NU - 1; ++i) issue_next();
+    for (int i = 0; i < NU; ++i) issue_next();
 
     const E* q = static_cast<const E*>(a.q);
     uint32_t qf[NH][D / 8];
@@ -170,12 +180,15 @@ __global__ void __launch_bounds__(kWarps<D> * 32, 1) paged_narrow_kernel(const _
     // ldmatrix: this lane's row of a tile of keys (as they are) and of values (turned)
     const uint32_t k_lane = smem_u32(ring) + ((lane & 7) + ((lane >> 3) & 1) * 8) * PITCH + (lane >> 4) * 16;
     const uint32_t v_lane = smem_u32(ring) + ((lane & 7) + (lane >> 4) * 8) * PITCH + ((lane >> 3) & 1) * 16;
-    auto arrived = [&]() {  // the place of the next unit, which is there; as many have been asked for behind it as the ring holds less two
-        cp_async_wait<NU - 2>();
+    int unit[kGroups];  // places of the next units, which are there
+    auto arrived = [&]() {
+        cp_async_wait<NU - kGroups>();
         __syncwarp();
-        const int place = use_place;
-        if (++use_place == NU) use_place = 0;
-        return place;
+#pragma unroll
+        for (int z = 0; z < kGroups; ++z) {
+            unit[z] = use_place * UNIT;
+            if (++use_place == NU) use_place = 0;
+        }
     };
 
     for (int pos = begin; pos < end;) {
@@ -226,40 +239,48 @@ __global__ void __launch_bounds__(kWarps<D> * 32, 1) paged_narrow_kernel(const _
         // ── its steps in this CTA's stretch ──
 #pragma unroll 1
         for (;;) {
-            const int k0 = (cur.first + cur.step) * KEYS + warp * 16;
-            const bool active = k0 < cur.keys.hi && k0 + 16 > cur.keys.lo;
-            uint32_t pb[NH][4];
+            const int k0 = (cur.first + cur.step) * KEYS + warp * TILE;
+            const bool active = k0 < cur.keys.hi && k0 + TILE > cur.keys.lo;
+            uint32_t pb[kGroups][NH][4];
             bool clear = true;
-            const uint32_t ku = k_lane + arrived() * UNIT;
+            arrived();
             if (active) {
-                float s[NH][2][4];
+                float s[kGroups][NH][4];
 #pragma unroll
-                for (int nh = 0; nh < NH; ++nh)
+                for (int z = 0; z < kGroups; ++z)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) s[nh][0][i] = s[nh][1][i] = 0.f;
+                    for (int nh = 0; nh < NH; ++nh)
 #pragma unroll
-                for (int j = 0; j < MT; ++j) {
-                    uint32_t k[4];
-                    ldmatrix4(k, ku + 32 * j);
+                        for (int i = 0; i < 4; ++i) s[z][nh][i] = 0.f;
 #pragma unroll
-                    for (int nh = 0; nh < NH; ++nh) TileElem<E>::mma(s[nh][j & 1], k[0], k[1], k[2], k[3], qf[nh][2 * j], qf[nh][2 * j + 1]);
-                }
-                clear = k0 >= clear_lo && k0 + 16 <= clear_hi;
-                float v[NH][4], top[NH][2];
-                bool valid[NH][4];
+                for (int j = 0; j < MT; ++j)
+#pragma unroll
+                    for (int z = 0; z < kGroups; ++z) {
+                        uint32_t k[4];
+                        ldmatrix4(k, k_lane + unit[z] + 32 * j);
+#pragma unroll
+                        for (int nh = 0; nh < NH; ++nh) TileElem<E>::mma(s[z][nh], k[0], k[1], k[2], k[3], qf[nh][2 * j], qf[nh][2 * j + 1]);
+                    }
+                clear = k0 >= clear_lo && k0 + TILE <= clear_hi;
+                float top[NH][2];
 #pragma unroll
                 for (int nh = 0; nh < NH; ++nh) {
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        valid[nh][i] = true;
-                        if (!clear) {
-                            const int k = k0 + g + 8 * (i >> 1);
-                            valid[nh][i] = k >= keys[nh][i & 1].lo && k < keys[nh][i & 1].hi;
-                        }
-                        v[nh][i] = valid[nh][i] ? (s[nh][0][i] + s[nh][1][i]) * a.scale2 : kLowest;
-                    }
+                    for (int z = 0; z < kGroups; ++z)
 #pragma unroll
-                    for (int x = 0; x < 2; ++x) top[nh][x] = fmaxf(v[nh][x], v[nh][2 + x]);
+                        for (int i = 0; i < 4; ++i) {
+                            s[z][nh][i] *= a.scale2;
+                            if (!clear) {  // NaN marks a key that the column does not see: a maximum passes it over
+                                const int k = k0 + 16 * z + g + 8 * (i >> 1);
+                                if (k < keys[nh][i & 1].lo || k >= keys[nh][i & 1].hi) s[z][nh][i] = __uint_as_float(kHidden);
+                            }
+                        }
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        top[nh][x] = fmaxf(s[0][nh][x], s[0][nh][2 + x]);
+#pragma unroll
+                        for (int z = 1; z < kGroups; ++z) top[nh][x] = fmaxf(top[nh][x], fmaxf(s[z][nh][x], s[z][nh][2 + x]));
+                    }
                 }
                 bool moved = false;
 #pragma unroll
@@ -285,67 +306,78 @@ __global__ void __launch_bounds__(kWarps<D> * 32, 1) paged_narrow_kernel(const _
                         }
                 }
 #pragma unroll
-                for (int nh = 0; nh < NH; ++nh) {
-                    float p[4];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) p[i] = valid[nh][i] ? exp2_approx(v[nh][i] - m_run[nh][i & 1]) : 0.f;
-                    l_run[nh][0] += p[0] + p[2];
-                    l_run[nh][1] += p[1] + p[3];
-                    const uint32_t pa = TileElem<E>::pack(p[0], p[1]), pc = TileElem<E>::pack(p[2], p[3]);
-                    const float2 fa = TileElem<E>::unpack(pa), fc = TileElem<E>::unpack(pc);
-                    pb[nh][0] = movmatrix_trans(pa);
-                    pb[nh][1] = movmatrix_trans(pc);
-                    pb[nh][2] = movmatrix_trans(TileElem<E>::pack(p[0] - fa.x, p[1] - fa.y));
-                    pb[nh][3] = movmatrix_trans(TileElem<E>::pack(p[2] - fc.x, p[3] - fc.y));
-                }
-            }
-            issue_next();  // into the place of the values of the tile before, which are used up
-            const uint32_t vu = v_lane + arrived() * UNIT;
-            if (active) {
-                bool odd = false;
-                if (!clear) {
-#pragma unroll 1
-                    for (int i = 0; i < MT; ++i) {
-                        uint32_t v[4];
-                        ldmatrix4_trans(v, vu + 32 * i);
-                        odd = odd || pair_not_finite<E>(v[0]) || pair_not_finite<E>(v[1]) || pair_not_finite<E>(v[2]) || pair_not_finite<E>(v[3]);
-                    }
-                    odd = __any_sync(0xffffffffu, odd);
-                }
-                if (odd) {
-                    MaskedTile<D, NH> rare;  // a copy: what is passed by address does not stay in registers
+                for (int z = 0; z < kGroups; ++z)
 #pragma unroll
                     for (int nh = 0; nh < NH; ++nh) {
-                        rare.keys[nh][0] = keys[nh][0];
-                        rare.keys[nh][1] = keys[nh][1];
+                        float p[4];
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) rare.p[nh][i] = pb[nh][i];
-#pragma unroll
-                        for (int i = 0; i < MT; ++i)
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) rare.o[nh][i][e] = o[nh][i][e];
+                        for (int i = 0; i < 4; ++i) {
+                            p[i] = exp2_approx(s[z][nh][i] - m_run[nh][i & 1]);
+                            if (!clear && __float_as_uint(s[z][nh][i]) == kHidden) p[i] = 0.f;
+                        }
+                        l_run[nh][0] += p[0] + p[2];
+                        l_run[nh][1] += p[1] + p[3];
+                        const uint32_t pa = TileElem<E>::pack(p[0], p[1]), pc = TileElem<E>::pack(p[2], p[3]);
+                        const float2 fa = TileElem<E>::unpack(pa), fc = TileElem<E>::unpack(pc);
+                        pb[z][nh][0] = movmatrix_trans(pa);
+                        pb[z][nh][1] = movmatrix_trans(pc);
+                        pb[z][nh][2] = movmatrix_trans(TileElem<E>::pack(p[0] - fa.x, p[1] - fa.y));
+                        pb[z][nh][3] = movmatrix_trans(TileElem<E>::pack(p[2] - fc.x, p[3] - fc.y));
                     }
-                    weighted_sum_masked<D, NH, E>(vu, rare, k0, t);
+            }
 #pragma unroll
-                    for (int nh = 0; nh < NH; ++nh)
+            for (int z = 0; z < kGroups; ++z) issue_next();  // into the places of the keys
+            arrived();
+            if (active) {
 #pragma unroll
-                        for (int i = 0; i < MT; ++i)
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) o[nh][i][e] = rare.o[nh][i][e];
-                } else {
-#pragma unroll
-                    for (int i = 0; i < MT; ++i) {
-                        uint32_t v[4];
-                        ldmatrix4_trans(v, vu + 32 * i);
+                for (int z = 0; z < kGroups; ++z) {
+                    const uint32_t vu = v_lane + unit[z];
+                    bool odd = false;
+                    if (!clear) {
+#pragma unroll 1
+                        for (int i = 0; i < MT; ++i) {
+                            uint32_t v[4];
+                            ldmatrix4_trans(v, vu + 32 * i);
+                            odd = odd || pair_not_finite<E>(v[0]) || pair_not_finite<E>(v[1]) || pair_not_finite<E>(v[2]) || pair_not_finite<E>(v[3]);
+                        }
+                        odd = __any_sync(0xffffffffu, odd);
+                    }
+                    if (odd) {
+                        MaskedTile<D, NH> rare;  // a copy: what is passed by address does not stay in registers
 #pragma unroll
                         for (int nh = 0; nh < NH; ++nh) {
-                            TileElem<E>::mma(o[nh][i], v[0], v[1], v[2], v[3], pb[nh][0], pb[nh][1]);
-                            TileElem<E>::mma(o[nh][i], v[0], v[1], v[2], v[3], pb[nh][2], pb[nh][3]);
+                            rare.keys[nh][0] = keys[nh][0];
+                            rare.keys[nh][1] = keys[nh][1];
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) rare.p[nh][i] = pb[z][nh][i];
+#pragma unroll
+                            for (int i = 0; i < MT; ++i)
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) rare.o[nh][i][e] = o[nh][i][e];
+                        }
+                        weighted_sum_masked<D, NH, E>(vu, rare, k0 + 16 * z, t);
+#pragma unroll
+                        for (int nh = 0; nh < NH; ++nh)
+#pragma unroll
+                            for (int i = 0; i < MT; ++i)
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) o[nh][i][e] = rare.o[nh][i][e];
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < MT; ++i) {
+                            uint32_t v[4];
+                            ldmatrix4_trans(v, vu + 32 * i);
+#pragma unroll
+                            for (int nh = 0; nh < NH; ++nh) {
+                                TileElem<E>::mma(o[nh][i], v[0], v[1], v[2], v[3], pb[z][nh][0], pb[z][nh][1]);
+                                TileElem<E>::mma(o[nh][i], v[0], v[1], v[2], v[3], pb[z][nh][2], pb[z][nh][3]);
+                            }
                         }
                     }
                 }
             }
-            issue_next();  // into the place of this tile's keys
+#pragma unroll
+            for (int z = 0; z < kGroups; ++z) issue_next();  // into the places of the values
             if (++pos >= end) break;
             cur.advance(c, line, a.window, batch);
             if (!cur.same_item(item)) break;
@@ -539,14 +571,14 @@ cudaError_t narrow(const Launch& l, PagedType type, const PagedAttentionArgs& a,
 
 }  // namespace
 
-int paged_narrow_columns(int head_dim, int64_t columns) { return columns <= 8 ? 3 : columns <= 16 || head_dim == 256 ? 4 : 5; }
-int paged_narrow_keys(int head_dim) { return head_dim == 256 ? 6 : 7; }  // 16 a warp
+int paged_narrow_columns(int head_dim, int64_t columns) { return columns <= 8 || head_dim == 256 ? 3 : columns <= 16 || head_dim == 128 ? 4 : 5; }
+int paged_narrow_keys(int head_dim) { return head_dim == 256 ? 7 : 8; }  // 32 a warp
 
 cudaError_t launch_paged_narrow(const Launch& l, PagedType type, int head_dim, const PagedAttentionArgs& a, int line) {
     const int groups = 1 << (a.line[line].columns - 3);
     if (head_dim == 64) return groups == 1 ? narrow<64, 1>(l, type, a, line) : groups == 2 ? narrow<64, 2>(l, type, a, line) : narrow<64, 4>(l, type, a, line);
-    if (head_dim == 128) return groups == 1 ? narrow<128, 1>(l, type, a, line) : groups == 2 ? narrow<128, 2>(l, type, a, line) : narrow<128, 4>(l, type, a, line);
-    return groups == 1 ? narrow<256, 1>(l, type, a, line) : narrow<256, 2>(l, type, a, line);
+    if (head_dim == 128) return groups == 1 ? narrow<128, 1>(l, type, a, line) : narrow<128, 2>(l, type, a, line);
+    return narrow<256, 1>(l, type, a, line);
 }
 
 cudaError_t launch_paged_merge(const Launch& l, PagedType type, int head_dim, const PagedAttentionArgs& a) {
