@@ -76,8 +76,9 @@ size_t attention_plan(const smelt_cuda_ctx* ctx, const smelt_paged_cache* k, con
         line.with_prefix = with_prefix;
         const int64_t columns = with_own && with_prefix ? (own > prefix ? own : prefix) : with_own ? own : prefix;
         line.columns = wide ? paged_wide_columns(D) : paged_narrow_columns(D, columns);
-        line.keys = wide ? paged_wide_keys(D) : paged_narrow_keys(D);
+        line.keys = wide ? paged_wide_keys(D) : paged_narrow_keys();
         line.ctas = ctx->sm_count;
+        line.workers = wide ? 1 : paged_narrow_workers(D);
         line.cum = (int32_t*)room((size_t)(b->n_seqs + 3) * sizeof(int32_t));
         line.slot_o = (float*)room(((size_t)2 * line.ctas << line.columns) * D * sizeof(float));
         line.slot_ml = (float2*)room(((size_t)2 * line.ctas << line.columns) * sizeof(float2));

@@ -5,10 +5,12 @@
 // with the running maximum and sum of the softmax, so that keys and values are read once.  This file has the streaming kernel for blocks
 // of few columns (a column is a row and a query head of the group that shares a key head) and the kernel that joins shared items.
 //
-// paged_narrow_kernel: one CTA a SM, each with as many steps of the line of work (paged.h).  A warp takes 32 keys of a step at a time as
+// paged_narrow_kernel: one CTA a SM, each warp with a stretch of the line of work (paged.h) of its own.  It takes 32 keys at a time as
 // S^T = K Q^T and O^T += V^T P^T on mma.sync: the columns of the block are the narrow side of the product, so eight columns cost what one
 // costs.  Rows come with cp.async, wherever their pages are, into a ring of the warp's own, 16 bytes more than their length apart, so
-// that ldmatrix reads them without conflicts.  The ring runs on across items, so that the pages of the next sequence are on their way while this one's warps join their sums.
+// that ldmatrix reads them without conflicts.  Nothing but the end of the stretch makes a warp wait for another: the ring runs on across
+// items, and while one warp writes down an item or waits for the next one's queries the others keep the memory busy.  At the end the
+// CTA joins what its warps have of the same item.
 // P goes into the product as two 16-bit parts: the kernel waits for memory, and rounding P once would cost up to half a step of the
 // 16-bit type.  Keys outside an item are not read (zeros), and a value row that is not finite reaches only the columns that see it.
 // paged_merge_kernel joins the items that several CTAs share, and the prefix with the sequences.
@@ -23,14 +25,17 @@ using attn::movmatrix_trans;
 using attn::TileElem;
 
 template <int D> constexpr int kWarps = D == 256 ? 4 : 8;
-constexpr int kGroups = 2;                                 // of 16 keys a tile: a chain of products, exchange and exponentials takes two as fast as one
-template <int D> constexpr int kUnits = D == 64 ? 10 : 5;  // of a warp's ring: the K or V rows of 16 keys each
+constexpr int kGroups = 2, kTile = 16 * kGroups;  // of 16 keys a tile: a chain of products, exchange and exponentials takes two as fast as one
+template <int D, int NH> constexpr int kUnits = D == 64 ? (NH == 1 ? 10 : NH == 2 ? 8 : 6) : D == 128 ? (NH == 1 ? 5 : 4) : 5;  // of a warp's ring: the K or V rows of 16 keys each
 template <int D> constexpr int kPitch = D * 2 + 16;
 template <int D> constexpr int kUnitBytes = 16 * kPitch<D>;
 
-template <int D>
-constexpr size_t narrow_shared(int n_seqs) {  // rings, one column group's sums of all warps, their maxima and sums, rows of keys, the batch
-    return (size_t)kWarps<D> * kUnits<D> * kUnitBytes<D> + (size_t)kWarps<D> * 8 * (D + 1) * 4 + (size_t)kWarps<D> * 8 * 8 + (size_t)kWarps<D> * 16 * kGroups * 8 + batch_bytes(n_seqs);
+// A warp's part of an item that it has not all of: from the steps before its stretch (0) or into those behind it (1).
+struct Part { int valid, source, block, head, at, steps; };
+
+template <int D, int NH>
+constexpr size_t narrow_shared(int n_seqs) {  // rings (and at the end parts 1), parts 0, maxima and sums of both, rows of keys, parts, the batch
+    return (size_t)kWarps<D> * (kUnits<D, NH> * kUnitBytes<D> + NH * 8 * (D + 1) * 4 + 2 * NH * 8 * 8 + kTile * 8 + 2 * sizeof(Part)) + batch_bytes(n_seqs);
 }
 
 __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t at) {
@@ -91,25 +96,29 @@ __device__ __noinline__ void weighted_sum_masked(uint32_t values, MaskedTile<D, 
 
 template <int D, int NH, class E>
 __global__ void __launch_bounds__(kWarps<D> * 32, 1) paged_narrow_kernel(const __grid_constant__ PagedAttentionArgs a, const int which) {
-    constexpr int W = kWarps<D>, THREADS = W * 32, NU = kUnits<D>, UNIT = kUnitBytes<D>, PITCH = kPitch<D>, TILE = 16 * kGroups, KEYS = W * TILE, MT = D / 16;
+    constexpr int W = kWarps<D>, THREADS = W * 32, NU = kUnits<D, NH>, UNIT = kUnitBytes<D>, PITCH = kPitch<D>, MT = D / 16, C = NH * 8;
+    static_assert(kTile == 32, "a lane a key");
+    static_assert(C * (D + 1) * 4 <= NU * UNIT && UNIT % 16 == 0, "parts 1 lie in the rings");
     extern __shared__ __align__(16) unsigned char smem[];
-    float* sums = reinterpret_cast<float*>(smem + (size_t)W * NU * UNIT);     // [W][8][D + 1]
-    float2* state = reinterpret_cast<float2*>(sums + W * 8 * (D + 1));        // [W][8]
-    long long* rows_of = reinterpret_cast<long long*>(state + W * 8);         // [W][TILE]
+    float* fronts = reinterpret_cast<float*>(smem + (size_t)W * NU * UNIT);     // [W][C][D + 1]
+    float2* state = reinterpret_cast<float2*>(fronts + W * C * (D + 1));        // [W][2][C]
+    long long* rows_of = reinterpret_cast<long long*>(state + W * 2 * C);       // [W][kTile]
+    Part* parts = reinterpret_cast<Part*>(rows_of + W * kTile);                 // [W][2]
     const PagedArgs& c = a.c;
     const PagedLine& line = a.line[which];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-    long long* rows = rows_of + warp * TILE;
+    long long* rows = rows_of + warp * kTile;
     pdl_trigger();
     pdl_wait();
     Batch batch;
-    scan_line<THREADS>(c, line, a.window, batch, reinterpret_cast<unsigned char*>(rows_of + W * TILE));
-    const Share share(batch.cum[c.n_seqs + 1], line.ctas);
-    if ((int)blockIdx.x >= share.ctas) return;
-    const int begin = share.begin(blockIdx.x), end = share.begin(blockIdx.x + 1);
+    scan_line<THREADS>(c, line, a.window, batch, reinterpret_cast<unsigned char*>(parts + W * 2));
+    const Share share(batch.cum[c.n_seqs + 1], line);
+    if ((int)blockIdx.x * W >= share.used) return;
+    const int begin = share.begin(blockIdx.x * W + warp), end = share.begin(blockIdx.x * W + warp + 1);
+    if (lane < 2) parts[warp * 2 + lane].valid = 0;
 
+    if (begin < end) {
     // ── the ring: of every tile kGroups units of keys, then kGroups of values ──
-    static_assert(TILE == 32, "a lane a key");
     unsigned char* ring = smem + (size_t)warp * NU * UNIT;
     Cursor cur;
     cur.seek(c, line, a.window, batch, begin);
@@ -120,7 +129,7 @@ __global__ void __launch_bounds__(kWarps<D> * 32, 1) paged_narrow_kernel(const _
     auto look_up = [&]() {
         inside = false;
         if (at >= end) return;
-        const int key = (ahead.first + ahead.step) * KEYS + warp * TILE + lane;
+        const int key = (ahead.first + ahead.step) * kTile + lane;
         head = ahead.head;
         inside = key >= ahead.keys.lo && key < ahead.keys.hi;
         if (inside) {
@@ -159,29 +168,39 @@ __global__ void __launch_bounds__(kWarps<D> * 32, 1) paged_narrow_kernel(const _
     };
     look_up();
     const int n_units = 2 * kGroups * (end - begin);
-    int issued = 0, issue_place = 0;  // the next unit to issue, and its place in the ring
-    auto issue_next = [&]() {
-        if (issued < n_units) issue_unit(issued % (2 * kGroups), issue_place);
-        cp_async_commit();
-        ++issued;
-        if (++issue_place == NU) issue_place = 0;
-    };
-#pragma unroll 1
-    for (int i = 0; i < NU; ++i) issue_next();
+    int issued = 0, issue_place = 0, freed = NU;  // the next unit to issue, its place in the ring, and up to which unit there is room
 
     const E* q = static_cast<const E*>(a.q);
     uint32_t qf[NH][D / 8];
     float m_run[NH][2], l_run[NH][2], o[NH][MT][4];
     Range keys[NH][2];  // of this thread's columns 2t, 2t + 1
     int clear_lo = 0, clear_hi = 0;  // every column of the block sees the keys [clear_lo, clear_hi)
-    Seq seq{0, 0, 0};
-    int width = 0;  // columns of the block
     int use_place = 0;
     // ldmatrix: this lane's row of a tile of keys (as they are) and of values (turned)
     const uint32_t k_lane = smem_u32(ring) + ((lane & 7) + ((lane >> 3) & 1) * 8) * PITCH + (lane >> 4) * 16;
     const uint32_t v_lane = smem_u32(ring) + ((lane & 7) + (lane >> 4) * 8) * PITCH + ((lane >> 3) & 1) * 16;
+    auto seq_of = [&](int source) { return source == 0 ? Seq{0, batch.row[c.n_seqs], 0} : batch.seq(source - 1); };
+    auto width_of = [&](const Cursor& x, const Seq& s) { return min(1 << line.columns, s.n * c.ratio - (x.block << line.columns)); };
+    auto load_queries = [&](const Cursor& x) {
+        const Seq s = seq_of(x.source);
+        const int width = width_of(x, s);
+#pragma unroll
+        for (int nh = 0; nh < NH; ++nh) {
+            const int f = (x.block << line.columns) + nh * 8 + g, i = divide(f, c.ratio_div);
+            const E* row_q = q + (size_t)(s.row + i) * a.q_stride + (size_t)(x.head * c.ratio + f - i * c.ratio) * D + 2 * t;
+            const bool live = nh * 8 + g < width;
+#pragma unroll
+            for (int j = 0; j < D / 8; ++j) qf[nh][j] = live ? *reinterpret_cast<const uint32_t*>(row_q + 8 * j) : 0u;
+        }
+    };
     int unit[kGroups];  // places of the next units, which are there
-    auto arrived = [&]() {
+    auto arrived = [&]() {  // in one place of the code: it is long, and short calls wait for instructions as for anything else
+#pragma unroll 1
+        for (; issued < freed; ++issued) {
+            if (issued < n_units) issue_unit(issued % (2 * kGroups), issue_place);
+            cp_async_commit();
+            if (++issue_place == NU) issue_place = 0;
+        }
         cp_async_wait<NU - kGroups>();
         __syncwarp();
 #pragma unroll
@@ -189,14 +208,14 @@ __global__ void __launch_bounds__(kWarps<D> * 32, 1) paged_narrow_kernel(const _
             unit[z] = use_place * UNIT;
             if (++use_place == NU) use_place = 0;
         }
+        freed += kGroups;
     };
 
+    load_queries(cur);
     for (int pos = begin; pos < end;) {
-        // ── an item: its columns' queries and key ranges ──
-        const int f0 = cur.block << line.columns;
-        if (cur.source == 0) seq = {0, batch.row[c.n_seqs], 0};
-        else seq = batch.seq(cur.source - 1);
-        width = min(1 << line.columns, seq.n * c.ratio - f0);
+        // ── an item: its columns' key ranges ──
+        const Seq seq = seq_of(cur.source);
+        const int f0 = cur.block << line.columns, width = width_of(cur, seq);
         auto range_of = [&](int f) -> Range {
             if (f >= width) return {0, 0};
             const int i = divide(f0 + f, c.ratio_div);
@@ -208,16 +227,6 @@ __global__ void __launch_bounds__(kWarps<D> * 32, 1) paged_narrow_kernel(const _
         clear_hi = 0x7fffffff;
 #pragma unroll
         for (int nh = 0; nh < NH; ++nh) {
-            const int f = nh * 8 + g;
-            if (f < width) {
-                const int i = divide(f0 + f, c.ratio_div);
-                const E* row_q = q + (size_t)(seq.row + i) * a.q_stride + (size_t)(cur.head * c.ratio + f0 + f - i * c.ratio) * D + 2 * t;
-#pragma unroll
-                for (int j = 0; j < D / 8; ++j) qf[nh][j] = *reinterpret_cast<const uint32_t*>(row_q + 8 * j);
-            } else {
-#pragma unroll
-                for (int j = 0; j < D / 8; ++j) qf[nh][j] = 0u;
-            }
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
                 keys[nh][x] = range_of(nh * 8 + 2 * t + x);
@@ -236,15 +245,15 @@ __global__ void __launch_bounds__(kWarps<D> * 32, 1) paged_narrow_kernel(const _
         const Cursor item = cur;
         const int item_at = pos - cur.step;  // the item's first step on the line
 
-        // ── its steps in this CTA's stretch ──
+        // ── its steps in this warp's stretch: keys, then values ──
+        uint32_t pb[kGroups][NH][4];
+        bool clear = true, last = false;
+        int k0 = 0;
 #pragma unroll 1
-        for (;;) {
-            const int k0 = (cur.first + cur.step) * KEYS + warp * TILE;
-            const bool active = k0 < cur.keys.hi && k0 + TILE > cur.keys.lo;
-            uint32_t pb[kGroups][NH][4];
-            bool clear = true;
+        for (int phase = 0;; phase ^= 1) {
             arrived();
-            if (active) {
+            if (phase == 0) {
+                k0 = (cur.first + cur.step) * kTile;
                 float s[kGroups][NH][4];
 #pragma unroll
                 for (int z = 0; z < kGroups; ++z)
@@ -261,7 +270,7 @@ __global__ void __launch_bounds__(kWarps<D> * 32, 1) paged_narrow_kernel(const _
 #pragma unroll
                         for (int nh = 0; nh < NH; ++nh) TileElem<E>::mma(s[z][nh], k[0], k[1], k[2], k[3], qf[nh][2 * j], qf[nh][2 * j + 1]);
                     }
-                clear = k0 >= clear_lo && k0 + TILE <= clear_hi;
+                clear = k0 >= clear_lo && k0 + kTile <= clear_hi;
                 float top[NH][2];
 #pragma unroll
                 for (int nh = 0; nh < NH; ++nh) {
@@ -324,11 +333,12 @@ __global__ void __launch_bounds__(kWarps<D> * 32, 1) paged_narrow_kernel(const _
                         pb[z][nh][2] = movmatrix_trans(TileElem<E>::pack(p[0] - fa.x, p[1] - fa.y));
                         pb[z][nh][3] = movmatrix_trans(TileElem<E>::pack(p[2] - fc.x, p[3] - fc.y));
                     }
-            }
-#pragma unroll
-            for (int z = 0; z < kGroups; ++z) issue_next();  // into the places of the keys
-            arrived();
-            if (active) {
+                last = cur.step + 1 == cur.steps || pos + 1 == end;
+                if (++pos < end) {
+                    cur.advance(c, line, a.window, batch);
+                    if (last) load_queries(cur);  // of the next item, on their way meanwhile
+                }
+            } else {
 #pragma unroll
                 for (int z = 0; z < kGroups; ++z) {
                     const uint32_t vu = v_lane + unit[z];
@@ -375,61 +385,113 @@ __global__ void __launch_bounds__(kWarps<D> * 32, 1) paged_narrow_kernel(const _
                         }
                     }
                 }
+                if (last) break;
             }
-#pragma unroll
-            for (int z = 0; z < kGroups; ++z) issue_next();  // into the places of the values
-            if (++pos >= end) break;
-            cur.advance(c, line, a.window, batch);
-            if (!cur.same_item(item)) break;
         }
 
-        // ── the warps' sums, eight columns at a time ──
-        const bool here = item_at >= begin && item_at + item.steps <= end;
-        const size_t slot_at = (size_t)(2 * blockIdx.x + (item_at < begin ? 0 : 1)) << line.columns;
+        // ── the item's sums ──
 #pragma unroll
-        for (int nh = 0; nh < NH; ++nh) {
-            if (nh * 8 >= width) break;
+        for (int nh = 0; nh < NH; ++nh)
 #pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                float l = l_run[nh][x];
+            for (int x = 0; x < 2; ++x)
 #pragma unroll
-                for (int off = 4; off < 32; off <<= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
-                if (g == 0) state[warp * 8 + 2 * t + x] = make_float2(m_run[nh][x], l);
-                float* to = sums + (warp * 8 + 2 * t + x) * (D + 1) + g;
+                for (int off = 4; off < 32; off <<= 1) l_run[nh][x] += __shfl_xor_sync(0xffffffffu, l_run[nh][x], off);
+        const bool before = item_at < begin, behind = item_at + item.steps > end;
+        if (before || behind) {
+            __syncwarp();  // behind: the ring has been read for the last time
+            const int which_part = before ? 0 : 1;
+            float* to = before ? fronts + warp * C * (D + 1) : reinterpret_cast<float*>(ring);
+            if (lane == 0) parts[warp * 2 + which_part] = {1, item.source, item.block, item.head, item_at, item.steps};
 #pragma unroll
-                for (int i = 0; i < MT; ++i) { to[16 * i] = o[nh][i][x]; to[16 * i + 8] = o[nh][i][2 + x]; }
-            }
-            __syncthreads();
-            const int n = min(8, width - nh * 8);
-            for (int i = tid; i < n * D; i += THREADS) {
-                const int col = i / D, d = i % D, f = nh * 8 + col;
-                float top = kLowest, sum = 0.f, l = 0.f;
+            for (int nh = 0; nh < NH; ++nh)
 #pragma unroll
-                for (int w = 0; w < W; ++w) top = fmaxf(top, state[w * 8 + col].x);
+                for (int x = 0; x < 2; ++x) {
+                    const int col = nh * 8 + 2 * t + x;
+                    if (g == 0) state[(warp * 2 + which_part) * C + col] = make_float2(m_run[nh][x], l_run[nh][x]);
+                    if (col < width)
 #pragma unroll
-                for (int w = 0; w < W; ++w) {
-                    const float2 ml = state[w * 8 + col];
-                    const float keep = exp2_approx(ml.x - top);
-                    l += ml.y * keep;
-                    sum += sums[(w * 8 + col) * (D + 1) + d] * keep;
+                        for (int i = 0; i < MT; ++i) { to[col * (D + 1) + 16 * i + g] = o[nh][i][x]; to[col * (D + 1) + 16 * i + 8 + g] = o[nh][i][2 + x]; }
                 }
-                const int ri = divide(f0 + f, c.ratio_div);
-                const size_t out_row = seq.row + ri, out_head = item.head * c.ratio + f0 + f - ri * c.ratio;
-                if (!here) {
-                    line.slot_o[(slot_at + f) * D + d] = sum;
-                    if (d == 0) line.slot_ml[slot_at + f] = make_float2(top, l);
-                } else if (a.whole_o) {
-                    const size_t at_row = ((item.source == 0 ? (size_t)c.rows : 0) + out_row) * c.n_q + out_head;
-                    a.whole_o[at_row * D + d] = sum;
-                    if (d == 0) a.whole_ml[at_row] = make_float2(top, l);
-                } else {
-                    static_cast<E*>(a.out)[out_row * a.out_stride + out_head * D + d] = round_to<E>(l > 0.f ? sum / l : (l == 0.f ? 0.f : l));
+        } else if (a.whole_o) {
+#pragma unroll
+            for (int nh = 0; nh < NH; ++nh)
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    const int f = nh * 8 + 2 * t + x, i = divide(f0 + f, c.ratio_div);
+                    if (f >= width) continue;
+                    const size_t to = ((item.source == 0 ? (size_t)c.rows : 0) + seq.row + i) * c.n_q + item.head * c.ratio + f0 + f - i * c.ratio;
+                    if (g == 0) a.whole_ml[to] = make_float2(m_run[nh][x], l_run[nh][x]);
+#pragma unroll
+                    for (int k = 0; k < MT; ++k) { a.whole_o[to * D + 16 * k + g] = o[nh][k][x]; a.whole_o[to * D + 16 * k + 8 + g] = o[nh][k][2 + x]; }
+                }
+        } else {
+#pragma unroll
+            for (int nh = 0; nh < NH; ++nh) {
+                float rate[2];
+#pragma unroll
+                for (int x = 0; x < 2; ++x) rate[x] = l_run[nh][x] > 0.f ? 1.f / l_run[nh][x] : l_run[nh][x];
+                const int f = nh * 8 + g, i = divide(f0 + f, c.ratio_div);  // after the turn this lane has two values of column g
+                E* to = static_cast<E*>(a.out) + (size_t)(seq.row + i) * a.out_stride + (size_t)(item.head * c.ratio + f0 + f - i * c.ratio) * D + 2 * t;
+#pragma unroll
+                for (int k = 0; k < 2 * MT; ++k) {
+                    const float v0 = o[nh][k >> 1][2 * (k & 1)], v1 = o[nh][k >> 1][2 * (k & 1) + 1];
+                    const uint32_t w = movmatrix_trans(TileElem<E>::pack(l_run[nh][0] == 0.f ? 0.f : v0 * rate[0], l_run[nh][1] == 0.f ? 0.f : v1 * rate[1]));
+                    if (f < width) *reinterpret_cast<uint32_t*>(to + 8 * k) = w;
                 }
             }
-            __syncthreads();
         }
     }
     cp_async_wait<0>();
+    }
+    __syncthreads();
+
+    // ── what the warps have of the same item, in order: a warp a column of an item ──
+    const int cta_begin = share.cta_begin(blockIdx.x), cta_end = share.cta_begin(blockIdx.x + 1);
+    const bool mine = lane < 2 * W && parts[lane & (2 * W - 1)].valid;  // lane p: part p
+    const int at_mine = parts[lane & (2 * W - 1)].at;
+    const uint32_t valid = __ballot_sync(0xffffffffu, mine), ahead_of_me = valid & ((1u << lane) - 1u);
+    const int at_before = __shfl_sync(0xffffffffu, at_mine, ahead_of_me ? 31 - __clz(ahead_of_me) : 0);
+    int turn = 0;
+    for (uint32_t first = __ballot_sync(0xffffffffu, mine && (!ahead_of_me || at_before != at_mine)); first; first &= first - 1u) {  // the first part of each item
+        const int p0 = __ffs(first) - 1, p1 = first & (first - 1u) ? __ffs(first & (first - 1u)) - 1 : 32;
+        const uint32_t members = valid & ~((1u << p0) - 1u) & (p1 < 32 ? (1u << p1) - 1u : 0xffffffffu);
+        const Part part = parts[p0];
+        const Seq seq = part.source == 0 ? Seq{0, batch.row[c.n_seqs], 0} : batch.seq(part.source - 1);
+        const int f0 = part.block << line.columns, width = min(1 << line.columns, seq.n * c.ratio - f0);
+        const bool here = part.at >= cta_begin && part.at + part.steps <= cta_end;
+        for (int f = 0; f < width; ++f) {
+            if ((turn++ & (W - 1)) != warp) continue;
+            const float2 ml = members >> lane & 1u ? state[lane * C + f] : make_float2(kLowest, 0.f);
+            const bool counts = ml.y != 0.f;  // a part that the column sees nothing of adds nothing, whatever its sums are
+            const float top = warp_max(counts ? ml.x : kLowest), factor = counts ? exp2_approx(ml.x - top) : 0.f, l = warp_sum(counts ? ml.y * factor : 0.f);
+            float sum[D / 32];
+#pragma unroll
+            for (int k = 0; k < D / 32; ++k) sum[k] = 0.f;
+            const uint32_t used = __ballot_sync(0xffffffffu, counts);
+#pragma unroll 2
+            for (uint32_t left = used; left; left &= left - 1u) {
+                const int p = __ffs(left) - 1;
+                const float w = __shfl_sync(0xffffffffu, factor, p);
+                const float* from = (p & 1 ? reinterpret_cast<const float*>(smem + (size_t)(p >> 1) * NU * UNIT) : fronts + (p >> 1) * C * (D + 1)) + f * (D + 1) + lane;
+#pragma unroll
+                for (int k = 0; k < D / 32; ++k) sum[k] += from[32 * k] * w;
+            }
+            const int ri = divide(f0 + f, c.ratio_div);
+            const size_t out_row = seq.row + ri, out_head = part.head * c.ratio + f0 + f - ri * c.ratio;
+            if (here && !a.whole_o) {
+                const float rate = l > 0.f ? 1.f / l : l;  // l = 0: nothing was seen
+                E* to = static_cast<E*>(a.out) + out_row * a.out_stride + out_head * D + lane;
+#pragma unroll
+                for (int k = 0; k < D / 32; ++k) to[32 * k] = round_to<E>(sum[k] * rate);
+            } else {
+                const size_t to = here ? ((part.source == 0 ? (size_t)c.rows : 0) + out_row) * c.n_q + out_head : ((size_t)(2 * blockIdx.x + (part.at < cta_begin ? 0 : 1)) << line.columns) + f;
+                float* o_to = (here ? a.whole_o : line.slot_o) + to * D + lane;
+#pragma unroll
+                for (int k = 0; k < D / 32; ++k) o_to[32 * k] = sum[k];
+                if (lane == 0) (here ? a.whole_ml : line.slot_ml)[to] = make_float2(top, l);
+            }
+        }
+    }
 }
 
 // ── the join ────────────────────────────────────────────────────────────────
@@ -473,7 +535,7 @@ __global__ void __launch_bounds__(kMergeWarps * 32) paged_merge_kernel(const __g
 #pragma unroll 1
     for (int x = 0; x < a.lines; ++x) {
         const PagedLine& line = a.line[x];
-        const Share share(line.cum[c.n_seqs + 1], line.ctas);
+        const Share share(line.cum[c.n_seqs + 1], line);
 #pragma unroll 1
         for (int prefix = line.with_prefix ? 1 : 0; prefix >= (line.with_own ? 0 : 1); --prefix) {
             // the item of this row and head: its first step on the line, and its steps
@@ -494,12 +556,12 @@ __global__ void __launch_bounds__(kMergeWarps * 32) paged_merge_kernel(const __g
             }
             if (steps == 0) continue;
             at += head * steps;
-            const int first = share.owner(at), last = share.owner(at + steps - 1);
+            const int first = share.cta_of(at), last = share.cta_of(at + steps - 1);
             const bool whole = first == last;
             if (whole && !a.whole_o) return;  // written by the CTA that finished it
             const size_t whole_at = ((prefix ? (size_t)c.rows : 0) + r) * c.n_q + h;
             const int parts = last - first + 1;
-            const float* part0 = whole ? a.whole_o + whole_at * D : line.slot_o + (((size_t)(2 * first + (at < share.begin(first) ? 0 : 1)) << line.columns) + col) * D;
+            const float* part0 = whole ? a.whole_o + whole_at * D : line.slot_o + (((size_t)(2 * first + (at < share.cta_begin(first) ? 0 : 1)) << line.columns) + col) * D;
             // every part but the first begins in front of its CTA's stretch: slot 0
             const float* part1 = line.slot_o + (((size_t)(2 * (first + 1)) << line.columns) + col) * D;
             const size_t stride = ((size_t)2 << line.columns) * D;
@@ -507,7 +569,7 @@ __global__ void __launch_bounds__(kMergeWarps * 32) paged_merge_kernel(const __g
             for (int base = 0; base < parts; base += 32) {
                 const int k = base + lane;
                 float2 ml = make_float2(kLowest, 0.f);
-                if (k < parts) ml = whole ? __ldcg(a.whole_ml + whole_at) : __ldcg(line.slot_ml + ((size_t)(2 * (first + k) + (k == 0 && at >= share.begin(first) ? 1 : 0)) << line.columns) + col);
+                if (k < parts) ml = whole ? __ldcg(a.whole_ml + whole_at) : __ldcg(line.slot_ml + ((size_t)(2 * (first + k) + (k == 0 && at >= share.cta_begin(first) ? 1 : 0)) << line.columns) + col);
                 const bool counts = ml.y != 0.f;  // a part that the row sees nothing of adds nothing, whatever its sums are
                 const float here = counts ? ml.x : kLowest, m = fmaxf(top, warp_max(here)), mine = exp2_approx(top - m), factor = counts ? exp2_approx(here - m) : 0.f;
                 top = m;
@@ -564,7 +626,7 @@ cudaError_t launch(const Launch& l, Kernel kernel, int grid, int threads, size_t
 
 template <int D, int NH>
 cudaError_t narrow(const Launch& l, PagedType type, const PagedAttentionArgs& a, int line) {
-    const size_t shared = narrow_shared<D>(a.c.n_seqs);
+    const size_t shared = narrow_shared<D, NH>(a.c.n_seqs);
     if (type == kPagedF16) return launch(l, paged_narrow_kernel<D, NH, __half>, a.line[line].ctas, kWarps<D> * 32, shared, a, line);
     return launch(l, paged_narrow_kernel<D, NH, __nv_bfloat16>, a.line[line].ctas, kWarps<D> * 32, shared, a, line);
 }
@@ -572,7 +634,8 @@ cudaError_t narrow(const Launch& l, PagedType type, const PagedAttentionArgs& a,
 }  // namespace
 
 int paged_narrow_columns(int head_dim, int64_t columns) { return columns <= 8 || head_dim == 256 ? 3 : columns <= 16 || head_dim == 128 ? 4 : 5; }
-int paged_narrow_keys(int head_dim) { return head_dim == 256 ? 7 : 8; }  // 32 a warp
+int paged_narrow_keys() { return 5; }
+int paged_narrow_workers(int head_dim) { return head_dim == 256 ? kWarps<256> : kWarps<128>; }
 
 cudaError_t launch_paged_narrow(const Launch& l, PagedType type, int head_dim, const PagedAttentionArgs& a, int line) {
     const int groups = 1 << (a.line[line].columns - 3);

@@ -103,15 +103,17 @@ __device__ __forceinline__ void scan_line(const PagedArgs& c, const PagedLine& l
     }
 }
 
-// Who has which steps of the line: the first `more` CTAs have each + 1, the others `each`; CTAs beyond `ctas` have none, so that none between
-// two owners of an item is without.
+// Who has which steps of the line: the first `more` workers have each + 1, the others `each`; workers from `used` on have none, so that none
+// between two owners of an item is without.
 struct Share {
-    int ctas, each, more;
-    __device__ __forceinline__ Share(int total, int most) : ctas(min(total, most)), each(ctas ? total / ctas : 0), more(total - each * ctas) {}
-    __device__ __forceinline__ int begin(int cta) const { return each * cta + min(cta, more); }
-    __device__ __forceinline__ int owner(int at) const {
-        const int first = more * (each + 1);
-        return at < first ? at / (each + 1) : more + (at - first) / each;
+    int workers, used, each, more;
+    __device__ __forceinline__ Share(int total, const PagedLine& line)
+        : workers(line.workers), used(min(total, line.ctas * line.workers)), each(used ? total / used : 0), more(total - each * used) {}
+    __device__ __forceinline__ int begin(int worker) const { const int w = min(worker, used); return each * w + min(w, more); }
+    __device__ __forceinline__ int cta_begin(int cta) const { return begin(cta * workers); }
+    __device__ __forceinline__ int cta_of(int at) const {  // the CTA that has a step
+        const int first = more * (each + 1), w = at < first ? at / (each + 1) : more + (at - first) / each;
+        return w / workers;
     }
 };
 

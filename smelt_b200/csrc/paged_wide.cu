@@ -171,8 +171,8 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_wide_kernel(const P
     scan_line<C::kThreads>(c, line, a.window, batch, reinterpret_cast<unsigned char*>(&sh) + ((sizeof(Shared) + 15) & ~(size_t)15));
     tc_fence_after();
     const uint32_t tmem = (uint32_t)uniform((int)sh.tmem);
-    const Share share(batch.cum[c.n_seqs + 1], line.ctas);
-    const int begin = (int)blockIdx.x < share.ctas ? share.begin(blockIdx.x) : 0, end = (int)blockIdx.x < share.ctas ? share.begin(blockIdx.x + 1) : 0;
+    const Share share(batch.cum[c.n_seqs + 1], line);
+    const int begin = share.cta_begin(blockIdx.x), end = share.cta_begin(blockIdx.x + 1);
     // A role that gives up a wait goes through the rest of its schedule without work, so that no barrier is short of a thread.
     bool alive = true;
     // An item's steps in this CTA: tasks, one a step, or with two tiles one a tile and step; task T of the CTA has score buffer T & 1.
