@@ -31,7 +31,10 @@ struct Cfg {
     static constexpr int kKeys = D == 256 ? 64 : 128;
     static constexpr int kStages = D == 64 ? 3 : 2;
     static constexpr int kQTile = 128 * D * 2, kTile = kKeys * D * 2;
-    static constexpr int kLoadWarp = kSets * 4, kMmaWarp = kLoadWarp + 4, kThreads = (kMmaWarp + 1) * 32;
+    static constexpr int kLoadWarp = kSets * 4, kMmaWarp = kLoadWarp + 4, kThreads = (kMmaWarp + 4) * 32;
+    // registers of a thread: the softmax holds a column's scores; 512 threads (384) are launched with 128 (168)
+    static constexpr int kMany = kSets == 2 ? 192 : 232, kFew = kSets == 2 ? 64 : 120;
+    static_assert(kSets * 128 * kMany + 256 * kFew <= kThreads * (65536 / kThreads / 8 * 8), "registers");
     static constexpr int kSum = 2 * kKeys;  // first column of the accumulators: behind two of scores
 };
 
@@ -97,12 +100,38 @@ __device__ __forceinline__ void tmem_ld32(uint32_t t, uint32_t (&v)[32]) {
                  : "r"(t)
                  : "memory");
 }
+// Two fp32 values side by side, and both operations on them in one instruction.
+__device__ __forceinline__ uint64_t pair_of(float x, float y) {
+    uint64_t v;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(x), "f"(y));
+    return v;
+}
+__device__ __forceinline__ void split(uint64_t v, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t v;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(a), "l"(b), "l"(c));
+    return v;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t v;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
+    return v;
+}
+constexpr uint32_t kHidden = 0x7FFFF00Du;  // a NaN of our own
 // The loads behind v have arrived (v is named so that nothing is read of it earlier).
 __device__ __forceinline__ void tmem_wait_ld32(uint32_t (&v)[32]) {
     asm volatile("tcgen05.wait::ld.sync.aligned;"
                  : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]), "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]),
                    "+r"(v[15]), "+r"(v[16]), "+r"(v[17]), "+r"(v[18]), "+r"(v[19]), "+r"(v[20]), "+r"(v[21]), "+r"(v[22]), "+r"(v[23]), "+r"(v[24]), "+r"(v[25]), "+r"(v[26]), "+r"(v[27]), "+r"(v[28]),
                    "+r"(v[29]), "+r"(v[30]), "+r"(v[31])::"memory");
+}
+// A column's scores, all on their way at once.
+template <int KEYS> __device__ __forceinline__ void load_scores(uint32_t at, uint32_t (&v)[KEYS]) {
+    uint32_t(&a)[KEYS / 32][32] = reinterpret_cast<uint32_t(&)[KEYS / 32][32]>(v);
+#pragma unroll
+    for (int x = 0; x < KEYS / 32; ++x) tmem_ld32(at + 32 * x, a[x]);
+#pragma unroll
+    for (int x = 0; x < KEYS / 32; ++x) tmem_wait_ld32(a[x]);
 }
 __device__ __forceinline__ void tmem_st16(uint32_t t, const uint32_t (&v)[16]) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(t), "r"(v[0]), "r"(v[1]), "r"(v[2]),
@@ -139,8 +168,11 @@ __device__ __forceinline__ Item item_of(const PagedArgs& c, const PagedLine& lin
     return it;
 }
 
+template <int REGS> __device__ __forceinline__ void registers_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS)); }
+template <int REGS> __device__ __forceinline__ void registers_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS)); }
+
 template <int D, class E>
-__global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_wide_kernel(const PagedAttentionArgs a, const int which) {
+__global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_wide_kernel(const __grid_constant__ PagedAttentionArgs a, const int which) {
     using C = Cfg<D>;
     constexpr int KEYS = C::kKeys, S = C::kStages, CHUNKS = D / 8;  // 16-byte chunks of a row
     extern __shared__ __align__(1024) unsigned char raw[];
@@ -197,7 +229,9 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_wide_kernel(const P
         }
     };
 
-    if (warp >= C::kLoadWarp && warp < C::kMmaWarp) {
+    if (warp >= C::kLoadWarp) {
+    registers_down<C::kFew>();
+    if (warp < C::kMmaWarp) {
         // ── pages to shared memory ──
         const int lt = tid - C::kLoadWarp * 32;
         constexpr int LANES = CHUNKS < 32 ? CHUNKS : 32, ROWS = 128 / LANES;  // lanes of a row, rows of a turn of the four warps
@@ -235,6 +269,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_wide_kernel(const P
             if (items > 0) warp_wait(&sh.q_empty, (items - 1) & 1);
             ++items;
             if (alive) {
+#pragma unroll 4
                 for (int f = r_first; f < (pair ? 256 : 128); f += ROWS) {
                     const int ff = it.f0 + f, i = divide(ff, c.ratio_div);
                     const bool live = f < it.width;
@@ -242,16 +277,17 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_wide_kernel(const P
                     const uint32_t to = smem_u32(q_tiles + (f >> 7) * C::kQTile);
                     for (int k = ch; k < CHUNKS; k += LANES) copy16(to + place(128, f & 127, k), from + 8 * k, live);
                 }
-                cp_async_commit();
-                cp_async_wait<0>();
-                if (a.scale2 < 0.f)  // the softmax wants a positive scale
+            }
+            cp_async_commit();
+            auto hand_over_queries = [&] {
+                if (a.scale2 < 0.f && alive)  // the softmax wants a positive scale
                     for (int f = r_first; f < (pair ? 256 : 128); f += ROWS)
                         for (int k = ch; k < CHUNKS; k += LANES) {
                             uint4* v = reinterpret_cast<uint4*>(q_tiles + (f >> 7) * C::kQTile + place(128, f & 127, k));
                             *v = make_uint4(v->x ^ 0x80008000u, v->y ^ 0x80008000u, v->z ^ 0x80008000u, v->w ^ 0x80008000u);
                         }
-            }
-            arrive(&sh.q_full);
+                arrive(&sh.q_full);
+            };
             const int32_t* table = cur.source == 0 ? c.prefix_table : c.table + (size_t)(cur.source - 1) * c.table_stride;
             const long long head_at = (long long)cur.head * c.head_stride;
             // where the key of this thread lies, a step ahead
@@ -286,8 +322,9 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_wide_kernel(const P
                 };
                 if (use > 0) warp_wait(&sh.k_empty[s], (use - 1) & 1);
                 copy(c.k, k_tiles);
-                cp_async_wait<1>();  // the values of the step before have arrived
-                hand_over_values();
+                cp_async_wait<1>();  // the values of the step before (or the queries) have arrived
+                if (i == 0) hand_over_queries();
+                else hand_over_values();
                 if (use > 0) warp_wait(&sh.v_empty[s], (use - 1) & 1);
                 if (lt < 4) sh.odd[s][lt] = 0;
                 copy(c.v, v_tiles);
@@ -348,7 +385,9 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_wide_kernel(const P
         // the products in flight read shared memory and write tensor memory
         if (done > 0) mbar_poll_bounded(&sh.pv_done[(done - 1) & 1], ((done - 1) >> 1) & 1);
         if (done > 1) mbar_poll_bounded(&sh.pv_done[done & 1], ((done - 2) >> 1) & 1);
+    }
     } else {
+        registers_up<C::kMany>();
         // ── softmax: a thread a column ──
         const int set = warp >> 2, me = (warp & 3) * 32 + lane;
         const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16), o_at = lanes + C::kSum + set * D;
@@ -381,22 +420,21 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_wide_kernel(const P
                 const uint32_t s_at = lanes + b * KEYS;
                 wait(&sh.s_full[b], use & 1);
                 if (alive) {
+                    uint32_t v[KEYS];
+                    load_scores<KEYS>(s_at, v);
                     float top = kLowest;
+                    if (!clear) {  // NaN marks a key that the column does not see: a maximum passes it over
 #pragma unroll
-                    for (int x = 0; x < KEYS; x += 32) {
-                        uint32_t v[32];
-                        tmem_ld32(s_at + x, v);
-                        tmem_wait_ld32(v);
-                        float t0 = kLowest, t1 = kLowest;
-                        if (clear) {
+                        for (int e = 0; e < KEYS; ++e)
+                            if (k0 + e < keys.lo || k0 + e >= keys.hi) v[e] = kHidden;
+                    }
+                    {
+                        float most[4] = {kLowest, kLowest, kLowest, kLowest};
 #pragma unroll
-                            for (int e = 0; e < 32; e += 2) { t0 = fmaxf(t0, __uint_as_float(v[e])); t1 = fmaxf(t1, __uint_as_float(v[e + 1])); }
-                        } else {
+                        for (int e = 0; e < KEYS; e += 8)
 #pragma unroll
-                            for (int e = 0; e < 32; ++e)
-                                if (k0 + x + e >= keys.lo && k0 + x + e < keys.hi) t0 = fmaxf(t0, __uint_as_float(v[e]));
-                        }
-                        top = fmaxf(top, fmaxf(t0, t1));
+                            for (int i = 0; i < 4; ++i) most[i] = fmaxf(most[i], fmaxf(__uint_as_float(v[e + 2 * i]), __uint_as_float(v[e + 2 * i + 1])));
+                        top = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
                     }
                     top = top == kLowest ? kLowest : top * scale2;
                     const bool begun = any;
@@ -420,28 +458,30 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_wide_kernel(const P
                             }
                         }
                     }
-                    const float minus = -m;
-                    float l0 = 0.f, l1 = 0.f;
+                    const uint64_t scales = pair_of(scale2, scale2), minus = pair_of(-m, -m);
+                    uint64_t sums[2] = {0ull, 0ull};
 #pragma unroll
                     for (int x = 0; x < KEYS; x += 32) {
-                        uint32_t v[32], p[16];
-                        tmem_ld32(s_at + x, v);
-                        tmem_wait_ld32(v);
+                        uint32_t p[16];
 #pragma unroll
                         for (int e = 0; e < 32; e += 2) {
-                            float p0 = exp2_approx(fmaf(__uint_as_float(v[e]), scale2, minus)), p1 = exp2_approx(fmaf(__uint_as_float(v[e + 1]), scale2, minus));
+                            float y0, y1;
+                            split(fma2(pair_of(__uint_as_float(v[x + e]), __uint_as_float(v[x + e + 1])), scales, minus), y0, y1);
+                            float p0 = exp2_approx(y0), p1 = exp2_approx(y1);
                             if (!clear) {
-                                const int k = k0 + x + e;
-                                if (k < keys.lo || k >= keys.hi) p0 = 0.f;
-                                if (k + 1 < keys.lo || k + 1 >= keys.hi) p1 = 0.f;
+                                if (v[x + e] == kHidden) p0 = 0.f;
+                                if (v[x + e + 1] == kHidden) p1 = 0.f;
                             }
-                            l0 += p0;
-                            l1 += p1;
+                            sums[e >> 1 & 1] = add2(sums[e >> 1 & 1], pair_of(p0, p1));
                             p[e / 2] = Pack<E>::two(p0, p1);
                         }
                         tmem_st16(s_at + x / 2, p);
                     }
-                    l += l0 + l1;
+                    {
+                        float l0, l1;
+                        split(add2(sums[0], sums[1]), l0, l1);
+                        l += l0 + l1;
+                    }
                     tmem_wait_st();
                     uint32_t keep_sum = 0;
                     if (checked) {  // values that were taken out of this step's product
