@@ -39,7 +39,7 @@ struct Cfg {
 };
 
 struct Shared {  // behind the tiles
-    uint64_t k_full[3], k_empty[3], v_full[3], v_empty[3], s_full[2], p_ready[2], pv_done[2], q_full, q_empty;
+    uint64_t k_full[3], k_empty[3], v_full[3], v_empty[3], v_raw[3], s_full[2], p_ready[2], pv_done[2], q_full, q_empty;
     uint32_t tmem, dead;
     uint32_t keep[2];    // the first product of an item adds to what its set has put into the accumulator
     uint32_t odd[3][4];  // keys of a stage's step whose values are not finite, and were taken out
@@ -171,8 +171,15 @@ __device__ __forceinline__ Item item_of(const PagedArgs& c, const PagedLine& lin
 template <int REGS> __device__ __forceinline__ void registers_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS)); }
 template <int REGS> __device__ __forceinline__ void registers_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS)); }
 
-template <int D, class E>
-__global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_wide_kernel(const __grid_constant__ PagedAttentionArgs a, const int which) {
+// What the tensor map reads: boxes of `tokens` tokens, and how many of them make a step.
+struct Pages {
+    CUtensorMap k, v;
+    int tokens, boxes;
+};
+
+// TILED: pages come as boxes of a tensor map; else row by row.
+template <int D, class E, bool TILED>
+__global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_wide_kernel(const __grid_constant__ PagedAttentionArgs a, const int which, const __grid_constant__ Pages pages) {
     using C = Cfg<D>;
     constexpr int KEYS = C::kKeys, S = C::kStages, CHUNKS = D / 8;  // 16-byte chunks of a row
     extern __shared__ __align__(1024) unsigned char raw[];
@@ -185,7 +192,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_wide_kernel(const _
     volatile uint32_t* dead = &sh.dead;
     if (tid == 0) {
         for (int i = 0; i < S; ++i) {
-            mbar_init(&sh.k_full[i], 4); mbar_init(&sh.v_full[i], 4);
+            mbar_init(&sh.k_full[i], TILED ? 1 : 4); mbar_init(&sh.v_full[i], TILED ? 1 : 4); mbar_init(&sh.v_raw[i], 1);
             mbar_init(&sh.k_empty[i], 1); mbar_init(&sh.v_empty[i], 1);
         }
         for (int i = 0; i < 2; ++i) { mbar_init(&sh.s_full[i], 1); mbar_init(&sh.p_ready[i], 4); mbar_init(&sh.pv_done[i], 1); }
@@ -246,22 +253,40 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_wide_kernel(const _
         uint32_t items = 0;
         int v_behind = -1;        // stage of the values that were asked for last and not handed over yet
         bool v_check = false;     // ... that not every column sees all of
+        Range v_rows = {0, KEYS}; // ... rows that are the item's (TILED)
+        uint32_t v_bad = 0, raw_uses = 0;  // ... boxes whose page is none; parity of v_raw by stage
+        auto zero_row = [&](unsigned char* tile, int r) {
+            for (int k = ch; k < CHUNKS; k += LANES) *reinterpret_cast<uint4*>(tile + place(KEYS, r, k)) = make_uint4(0, 0, 0, 0);
+        };
         auto hand_over_values = [&] {
             if (v_behind < 0) return;
+            unsigned char* tile = v_tiles + v_behind * C::kTile;
+            if (TILED) {
+                warp_wait(&sh.v_raw[v_behind], raw_uses >> v_behind & 1u);
+                raw_uses ^= 1u << v_behind;
+                if (v_rows.lo > 0 || v_rows.hi < KEYS || v_bad)
+                    for (int r = r_first; r < KEYS; r += ROWS)
+                        if (r < v_rows.lo || r >= v_rows.hi || (v_bad >> (r / pages.tokens) & 1u)) zero_row(tile, r);
+            }
             if (v_check) {
-                unsigned char* tile = v_tiles + v_behind * C::kTile;
                 barrier(1, 128);  // the stage's words of odd keys are zero
                 for (int r = r_first; r < KEYS; r += ROWS)
                     for (int k = ch; k < CHUNKS; k += LANES)
                         if (word_not_finite<E>(*reinterpret_cast<const uint4*>(tile + place(KEYS, r, k)))) atomicOr(&sh.odd[v_behind][r >> 5], 1u << (r & 31));
                 barrier(1, 128);
                 for (int r = r_first; r < KEYS; r += ROWS)
-                    if (sh.odd[v_behind][r >> 5] >> (r & 31) & 1u)
-                        for (int k = ch; k < CHUNKS; k += LANES) *reinterpret_cast<uint4*>(tile + place(KEYS, r, k)) = make_uint4(0, 0, 0, 0);
+                    if (sh.odd[v_behind][r >> 5] >> (r & 31) & 1u) zero_row(tile, r);
             }
-            arrive(&sh.v_full[v_behind]);
+            if (TILED) {
+                fence_async_smem();
+                barrier(1, 128);
+                if (lt == 0) mbar_arrive(&sh.v_full[v_behind]);
+            } else {
+                arrive(&sh.v_full[v_behind]);
+            }
             v_behind = -1;
         };
+        uint32_t all_steps = 0;
         each_item([&](const Cursor& cur, const Item& it, bool pair, int n, int, uint32_t, uint32_t step0, int) {
             // queries, behind everything that was asked for before them
             cp_async_wait<0>();
@@ -290,6 +315,59 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_wide_kernel(const _
             };
             const int32_t* table = cur.source == 0 ? c.prefix_table : c.table + (size_t)(cur.source - 1) * c.table_stride;
             const long long head_at = (long long)cur.head * c.head_stride;
+            if constexpr (TILED) {
+                // lane p of each warp: the page of box p, a step ahead
+                auto look_up = [&](int i) {
+                    const int key = (cur.first + cur.step + i) * KEYS + lane * pages.tokens;
+                    return lane < pages.boxes && i < n && key < cur.keys.hi && key + pages.tokens > cur.keys.lo ? table[divide(key, c.page_div)] : -1;
+                };
+                int ahead = look_up(0);
+                for (int i = 0; i < n; ++i) {
+                    const uint32_t step = step0 + i, s = step % S, use = step / S;
+                    const int k0 = (cur.first + cur.step + i) * KEYS, key = k0 + lane * pages.tokens, page = ahead;
+                    const bool in = lane < pages.boxes && key < cur.keys.hi && key + pages.tokens > cur.keys.lo, take = in && (uint32_t)page < (uint32_t)c.n_pages;
+                    const uint32_t taken = __ballot_sync(0xffffffffu, take), bad = __ballot_sync(0xffffffffu, in && !take);
+                    if (bad && lt == 0 && c.err) atomicOr(c.err, KERR_BAD_PAGE);
+                    ahead = look_up(i + 1);
+                    auto copy = [&](const CUtensorMap* map, unsigned char* tiles, uint64_t* bar) {
+                        if (warp != C::kLoadWarp || !alive) return;
+                        const uint32_t dst = smem_u32(tiles + s * C::kTile), at = smem_u32(bar);
+                        if (lane == 0) arrive_expect_at(at, __popc(taken) * pages.tokens * D * 2);
+                        __syncwarp();
+#pragma unroll 1
+                        for (uint32_t left = taken; left; left &= left - 1u) {
+                            const int p = __ffs(left) - 1, id = __shfl_sync(0xffffffffu, page, p);
+                            const int token = pages.boxes == 1 ? k0 - divide(k0, c.page_div) * c.page_size : 0;
+                            if (lane == 0)
+#pragma unroll
+                                for (int x = 0; x < D / 64; ++x) tma_load_4d_at(dst + x * (KEYS * 128) + p * pages.tokens * 128, map, 64 * x, token, cur.head, id, at);
+                        }
+                    };
+                    if (use > 0) warp_wait(&sh.k_empty[s], (use - 1) & 1);
+                    if (bad) {
+                        for (int r = r_first; r < KEYS; r += ROWS)
+                            if (bad >> (r / pages.tokens) & 1u) zero_row(k_tiles + s * C::kTile, r);
+                        fence_async_smem();
+                        barrier(1, 128);
+                    }
+                    copy(&pages.k, k_tiles, &sh.k_full[s]);
+                    if (i > 0) hand_over_values();
+                    if (use > 0) warp_wait(&sh.v_empty[s], (use - 1) & 1);
+                    if (lt < 4) sh.odd[s][lt] = 0;
+                    v_check = k0 < it.clear.lo || min(k0 + KEYS, cur.keys.hi) > it.clear.hi;
+                    v_rows = {max(cur.keys.lo - k0, 0), min(cur.keys.hi - k0, KEYS)};
+                    v_bad = bad;
+                    const bool fix = v_check || v_rows.lo > 0 || v_rows.hi < KEYS || bad;
+                    copy(&pages.v, v_tiles, fix ? &sh.v_raw[s] : &sh.v_full[s]);
+                    if (fix) v_behind = (int)s;
+                    if (i == 0) {
+                        cp_async_wait<0>();
+                        hand_over_queries();
+                    }
+                }
+                all_steps = step0 + n;
+                return;
+            }
             // where the key of this thread lies, a step ahead
             auto look_up = [&](int i) {
                 const int key = (cur.first + cur.step + i) * KEYS + lt;
@@ -336,6 +414,12 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_wide_kernel(const _
         });
         cp_async_wait<0>();
         hand_over_values();
+        if (TILED && !alive && warp == C::kLoadWarp)  // no copy may land after the CTA has left
+            for (uint32_t s = 0; s < S && s < all_steps; ++s) {
+                const uint32_t use = (all_steps - 1 - s) / S;
+                mbar_poll_bounded(&sh.k_full[s], use & 1);
+                mbar_poll_bounded(&sh.v_full[s], use & 1);
+            }
     } else if (warp == C::kMmaWarp) {
         // ── products ──
         constexpr uint32_t kScores = (1u << 4) | Pack<E>::kType | ((uint32_t)(KEYS >> 3) << 17) | ((128u >> 4) << 24);
@@ -617,9 +701,9 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_wide_kernel(const _
     }
 }
 
-template <int D, class E>
-cudaError_t go(const Launch& l, const PagedAttentionArgs& a, int line) {
-    auto kernel = paged_wide_kernel<D, E>;
+template <int D, class E, bool TILED>
+cudaError_t run(const Launch& l, const PagedAttentionArgs& a, int line, const Pages& pages) {
+    auto kernel = paged_wide_kernel<D, E, TILED>;
     const size_t shared = wide_shared<D>(a.c.n_seqs);
     cudaError_t e = allow_shared(kernel, shared);
     if (e == cudaSuccess) e = prefer_max_shared(kernel);
@@ -634,7 +718,21 @@ cudaError_t go(const Launch& l, const PagedAttentionArgs& a, int line) {
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = l.pdl ? 1 : 0;
-    return cudaLaunchKernelEx(&cfg, kernel, a, line);
+    return cudaLaunchKernelEx(&cfg, kernel, a, line, pages);
+}
+
+template <int D, class E>
+cudaError_t go(const Launch& l, const PagedAttentionArgs& a, int line) {
+    constexpr int KEYS = Cfg<D>::kKeys;
+    const PagedArgs& c = a.c;
+    // Boxes of a step: whole pages, or a part of one.  The swizzle's atoms are eight rows.
+    Pages pages = {};
+    pages.tokens = c.page_size < KEYS ? c.page_size : KEYS;
+    pages.boxes = KEYS / pages.tokens;
+    const bool tiled = pages.tokens % 8 == 0 && KEYS % pages.tokens == 0 && c.page_size % pages.tokens == 0 &&
+                       encode_pages(&pages.k, c.k, D, c.page_size, c.n_kv, c.n_pages, c.token_stride, c.head_stride, c.page_stride, pages.tokens) &&
+                       encode_pages(&pages.v, c.v, D, c.page_size, c.n_kv, c.n_pages, c.token_stride, c.head_stride, c.page_stride, pages.tokens);
+    return tiled ? run<D, E, true>(l, a, line, pages) : run<D, E, false>(l, a, line, pages);
 }
 
 }  // namespace

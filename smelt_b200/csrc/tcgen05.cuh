@@ -86,6 +86,10 @@ __device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, i
                  "r"(smem_u32(bar))
                  : "memory");
 }
+__device__ __forceinline__ void tma_load_4d_at(uint32_t dst, const CUtensorMap* map, int x, int y, int z, int w, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar)
+                 : "memory");
+}
 __device__ __forceinline__ void tma_load_2d_at(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
     asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(bar) : "memory");
 }
@@ -159,5 +163,7 @@ __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.
 // A row-major matrix of `width`-byte elements read in boxes of box_rows rows x 128 bytes, 128-byte swizzle; beyond its edges: zeros
 // (affine_line.cu).
 bool encode_rows(CUtensorMap* map, CUtensorMapDataType type, int width, const void* base, long rows, long cols, int box_rows);
+// Pages of 16-bit values [page][head][token][dim] with strides in values, read in boxes of 64 values of box_tokens tokens, 128-byte swizzle.
+bool encode_pages(CUtensorMap* map, const void* base, int dim, int tokens, int heads, int pages, int64_t token_stride, int64_t head_stride, int64_t page_stride, int box_tokens);
 
 }  // namespace smelt
