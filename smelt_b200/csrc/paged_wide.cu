@@ -48,7 +48,7 @@ struct Shared {  // behind the tiles
 };
 template <int D>
 constexpr size_t wide_shared(int n_seqs) {
-    return (size_t)Cfg<D>::kSets * Cfg<D>::kQTile + 2 * Cfg<D>::kStages * Cfg<D>::kTile + (Cfg<D>::kSets == 2 ? 128 * 32 * 4 : 0) + ((sizeof(Shared) + 15) & ~(size_t)15) + batch_bytes(n_seqs);
+    return (size_t)Cfg<D>::kSets * Cfg<D>::kQTile + 2 * Cfg<D>::kStages * Cfg<D>::kTile + Cfg<D>::kSets * 128 * 16 * 4 + ((sizeof(Shared) + 15) & ~(size_t)15) + batch_bytes(n_seqs);
 }
 
 template <class E> struct Pack;
@@ -184,8 +184,8 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_wide_kernel(const _
     constexpr int KEYS = C::kKeys, S = C::kStages, CHUNKS = D / 8;  // 16-byte chunks of a row
     extern __shared__ __align__(1024) unsigned char raw[];
     unsigned char *q_tiles = raw, *k_tiles = q_tiles + C::kSets * C::kQTile, *v_tiles = k_tiles + S * C::kTile;
-    float* joint = reinterpret_cast<float*>(v_tiles + S * C::kTile);  // [128][32] of the set that is added to the other
-    Shared& sh = *reinterpret_cast<Shared*>(reinterpret_cast<unsigned char*>(joint) + (C::kSets == 2 ? 128 * 32 * 4 : 0));
+    float* joint = reinterpret_cast<float*>(v_tiles + S * C::kTile);  // what the ends of items go through: [sets][128][16]
+    Shared& sh = *reinterpret_cast<Shared*>(reinterpret_cast<unsigned char*>(joint) + C::kSets * 128 * 16 * 4);
     const PagedArgs& c = a.c;
     const PagedLine& line = a.line[which];
     const int tid = threadIdx.x, warp = uniform(tid >> 5), lane = tid & 31;
@@ -199,6 +199,10 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_wide_kernel(const _
         mbar_init(&sh.q_full, 4);
         mbar_init(&sh.q_empty, 1);
         sh.dead = 0;
+        if (TILED) {
+            asm volatile("prefetch.tensormap [%0];" ::"l"(&pages.k) : "memory");
+            asm volatile("prefetch.tensormap [%0];" ::"l"(&pages.v) : "memory");
+        }
         mbar_fence_init();
         fence_async_smem();
     }
@@ -480,6 +484,71 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_wide_kernel(const _
             alive = __all_sync(0xffffffffu, alive && wait_alive(bar, parity, dead)) != 0;
             tc_fence_after();
         };
+        float m = kLowest, l = 0.f;  // of the column: what its weights are relative to, and their sum
+        // A task's scores to weights, in place.  all: every key is seen.
+        auto weigh = [&](auto all, uint32_t s_at, int k0, const Range& keys, bool begun, uint32_t last) {
+            uint32_t v[KEYS];
+            load_scores<KEYS>(s_at, v);
+            float top = kLowest;
+            if constexpr (!decltype(all)::value) {  // NaN marks a key that the column does not see: a maximum passes it over
+#pragma unroll
+                for (int e = 0; e < KEYS; ++e)
+                    if (k0 + e < keys.lo || k0 + e >= keys.hi) v[e] = kHidden;
+            }
+            {
+                float most[4] = {kLowest, kLowest, kLowest, kLowest};
+#pragma unroll
+                for (int e = 0; e < KEYS; e += 8)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) most[i] = fmaxf(most[i], fmaxf(__uint_as_float(v[e + 2 * i]), __uint_as_float(v[e + 2 * i + 1])));
+                top = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
+            }
+            top = top == kLowest ? kLowest : top * scale2;
+            const bool move = top > m + 8.f || !begun;
+            if (!begun) {
+                m = top;
+            } else if (__any_sync(0xffffffffu, move)) {
+                const float keep = move ? exp2_approx(m - top) : 1.f;
+                if (move) m = top;
+                l *= keep;
+                wait(&sh.pv_done[last & 1], (last >> 1) & 1);
+                if (alive) {
+#pragma unroll 1
+                    for (int x = 0; x < D; x += 16) {
+                        uint32_t v[16];
+                        tmem_ld16(o_at + x, v);
+                        tmem_wait_ld16(v);
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * keep);
+                        tmem_st16(o_at + x, v);
+                    }
+                }
+            }
+            const uint64_t scales = pair_of(scale2, scale2), minus = pair_of(-m, -m);
+            uint64_t sums[2] = {0ull, 0ull};
+#pragma unroll
+            for (int x = 0; x < KEYS; x += 32) {
+                uint32_t p[16];
+#pragma unroll
+                for (int e = 0; e < 32; e += 2) {
+                    float y0, y1;
+                    split(fma2(pair_of(__uint_as_float(v[x + e]), __uint_as_float(v[x + e + 1])), scales, minus), y0, y1);
+                    float p0 = exp2_approx(y0), p1 = exp2_approx(y1);
+                    if constexpr (!decltype(all)::value) {
+                        if (v[x + e] == kHidden) p0 = 0.f;
+                        if (v[x + e + 1] == kHidden) p1 = 0.f;
+                    }
+                    sums[e >> 1 & 1] = add2(sums[e >> 1 & 1], pair_of(p0, p1));
+                    p[e / 2] = Pack<E>::two(p0, p1);
+                }
+                tmem_st16(s_at + x / 2, p);
+            }
+            {
+                float l0, l1;
+                split(add2(sums[0], sums[1]), l0, l1);
+                l += l0 + l1;
+            }
+        };
         each_item([&](const Cursor& cur, const Item& it, bool pair, int n, int tasks, uint32_t task0, uint32_t step0, int pos) {
             const int t_first = C::kSets == 1 ? 0 : (int)((task0 & 1) ^ set), f = (pair ? t_first * 128 : 0) + me, ff = it.f0 + f;
             Range keys = {0, 0};
@@ -493,7 +562,8 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_wide_kernel(const _
                 }
             }
             const bool blind = __any_sync(0xffffffffu, f < it.width && keys.hi == 0);  // a row of the prefix's block that sees nothing
-            float m = kLowest, l = 0.f;
+            m = kLowest;
+            l = 0.f;
             uint32_t last = 0;
             bool any = false;
             for (int t = t_first; t < tasks; t += C::kSets) {
@@ -504,68 +574,9 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_wide_kernel(const _
                 const uint32_t s_at = lanes + b * KEYS;
                 wait(&sh.s_full[b], use & 1);
                 if (alive) {
-                    uint32_t v[KEYS];
-                    load_scores<KEYS>(s_at, v);
-                    float top = kLowest;
-                    if (!clear) {  // NaN marks a key that the column does not see: a maximum passes it over
-#pragma unroll
-                        for (int e = 0; e < KEYS; ++e)
-                            if (k0 + e < keys.lo || k0 + e >= keys.hi) v[e] = kHidden;
-                    }
-                    {
-                        float most[4] = {kLowest, kLowest, kLowest, kLowest};
-#pragma unroll
-                        for (int e = 0; e < KEYS; e += 8)
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) most[i] = fmaxf(most[i], fmaxf(__uint_as_float(v[e + 2 * i]), __uint_as_float(v[e + 2 * i + 1])));
-                        top = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
-                    }
-                    top = top == kLowest ? kLowest : top * scale2;
                     const bool begun = any;
-                    const bool move = top > m + 8.f || !begun;
-                    if (!begun) {
-                        m = top;
-                    } else if (__any_sync(0xffffffffu, move)) {
-                        const float keep = move ? exp2_approx(m - top) : 1.f;
-                        if (move) m = top;
-                        l *= keep;
-                        wait(&sh.pv_done[last & 1], (last >> 1) & 1);
-                        if (alive) {
-#pragma unroll 1
-                            for (int x = 0; x < D; x += 16) {
-                                uint32_t v[16];
-                                tmem_ld16(o_at + x, v);
-                                tmem_wait_ld16(v);
-#pragma unroll
-                                for (int e = 0; e < 16; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * keep);
-                                tmem_st16(o_at + x, v);
-                            }
-                        }
-                    }
-                    const uint64_t scales = pair_of(scale2, scale2), minus = pair_of(-m, -m);
-                    uint64_t sums[2] = {0ull, 0ull};
-#pragma unroll
-                    for (int x = 0; x < KEYS; x += 32) {
-                        uint32_t p[16];
-#pragma unroll
-                        for (int e = 0; e < 32; e += 2) {
-                            float y0, y1;
-                            split(fma2(pair_of(__uint_as_float(v[x + e]), __uint_as_float(v[x + e + 1])), scales, minus), y0, y1);
-                            float p0 = exp2_approx(y0), p1 = exp2_approx(y1);
-                            if (!clear) {
-                                if (v[x + e] == kHidden) p0 = 0.f;
-                                if (v[x + e + 1] == kHidden) p1 = 0.f;
-                            }
-                            sums[e >> 1 & 1] = add2(sums[e >> 1 & 1], pair_of(p0, p1));
-                            p[e / 2] = Pack<E>::two(p0, p1);
-                        }
-                        tmem_st16(s_at + x / 2, p);
-                    }
-                    {
-                        float l0, l1;
-                        split(add2(sums[0], sums[1]), l0, l1);
-                        l += l0 + l1;
-                    }
+                    if (clear) weigh(std::true_type{}, s_at, k0, keys, begun, last);
+                    else weigh(std::false_type{}, s_at, k0, keys, begun, last);
                     tmem_wait_st();
                     uint32_t keep_sum = 0;
                     if (checked) {  // values that were taken out of this step's product
@@ -646,47 +657,65 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_wide_kernel(const _
             const bool write = writer && f < it.width && alive;
             if (write && part) *part_ml = make_float2(m, l);
             const float rate = part ? 1.f : l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;
+            // 16 values of a column at a time, through shared memory: a store of the warp takes whole sectors of a few columns
+            float* exchange = joint;                                                 // [128][16] of the set that is added to the other
+            float* stage = joint + ((both ? 1 : set) * 4 + (warp & 3)) * (32 * 16);  // [32][16] of the warp
+            auto turned = [](int row, int piece) { return row * 16 + ((piece ^ (row >> 1 & 3)) << 2); };
+            const uint32_t stores = __ballot_sync(0xffffffffu, write);
+            char* dest = reinterpret_cast<char*>(part);  // the column's values in memory
+            if (!part) dest = reinterpret_cast<char*>(static_cast<E*>(a.out) + row * a.out_stride + head * D);
 #pragma unroll 1
-            for (int x = 0; x < D; x += 32) {
-                uint32_t v[32];
+            for (int x = 0; x < D; x += 16) {
+                uint32_t v[16];
                 if (any && alive) {
-                    tmem_ld32(o_at + x, v);
-                    tmem_wait_ld32(v);
+                    tmem_ld16(o_at + x, v);
+                    tmem_wait_ld16(v);
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * mine);
+                    for (int e = 0; e < 16; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * mine);
                 } else {
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) v[e] = 0u;
+                    for (int e = 0; e < 16; ++e) v[e] = 0u;
                 }
-                if (both) {  // [column][32 values], 16-byte groups turned by the column
-                    float* to = joint + me * 32;
+                if (both) {
                     if (!writer)
 #pragma unroll
-                        for (int e = 0; e < 32; e += 4) *reinterpret_cast<uint4*>(to + (((e >> 2) ^ (me & 7)) << 2)) = make_uint4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+                        for (int e = 0; e < 4; ++e) *reinterpret_cast<uint4*>(exchange + turned(me, e)) = make_uint4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
                     barrier(2, 256);
                     if (writer)
 #pragma unroll
-                        for (int e = 0; e < 32; e += 4) {
-                            const float4 w = *reinterpret_cast<const float4*>(to + (((e >> 2) ^ (me & 7)) << 2));
-                            v[e] = __float_as_uint(__uint_as_float(v[e]) + w.x); v[e + 1] = __float_as_uint(__uint_as_float(v[e + 1]) + w.y);
-                            v[e + 2] = __float_as_uint(__uint_as_float(v[e + 2]) + w.z); v[e + 3] = __float_as_uint(__uint_as_float(v[e + 3]) + w.w);
+                        for (int e = 0; e < 4; ++e) {
+                            const float4 w = *reinterpret_cast<const float4*>(exchange + turned(me, e));
+                            v[4 * e] = __float_as_uint(__uint_as_float(v[4 * e]) + w.x); v[4 * e + 1] = __float_as_uint(__uint_as_float(v[4 * e + 1]) + w.y);
+                            v[4 * e + 2] = __float_as_uint(__uint_as_float(v[4 * e + 2]) + w.z); v[4 * e + 3] = __float_as_uint(__uint_as_float(v[4 * e + 3]) + w.w);
                         }
                     barrier(2, 256);
                 }
-                if (write) {
-                    if (part) {
+                if (!stores) continue;
+                if (part) {  // 64 bytes a column
 #pragma unroll
-                        for (int e = 0; e < 32; e += 4) *reinterpret_cast<uint4*>(part + x + e) = make_uint4(v[e], v[e + 1], v[e + 2], v[e + 3]);
-                    } else {
-                        E* out = static_cast<E*>(a.out) + row * a.out_stride + head * D + x;
-                        uint32_t w[16];
+                    for (int e = 0; e < 4; ++e) *reinterpret_cast<uint4*>(stage + turned(lane, e)) = make_uint4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
+                    __syncwarp();
 #pragma unroll
-                        for (int e = 0; e < 32; e += 2)
-                            w[e / 2] = l == 0.f ? 0u : Pack<E>::two(__uint_as_float(v[e]) * rate, __uint_as_float(v[e + 1]) * rate);
+                    for (int i = 0; i < 4; ++i) {
+                        const int r = 8 * i + (lane >> 2);
+                        char* to = reinterpret_cast<char*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(dest), r));
+                        if (stores >> r & 1u) *reinterpret_cast<uint4*>(to + x * 4 + (lane & 3) * 16) = *reinterpret_cast<const uint4*>(stage + turned(r, lane & 3));
+                    }
+                } else {  // 32 bytes a column
+                    uint32_t w[8];
 #pragma unroll
-                        for (int e = 0; e < 16; e += 4) *reinterpret_cast<uint4*>(out + 2 * e) = make_uint4(w[e], w[e + 1], w[e + 2], w[e + 3]);
+                    for (int e = 0; e < 16; e += 2) w[e / 2] = l == 0.f ? 0u : Pack<E>::two(__uint_as_float(v[e]) * rate, __uint_as_float(v[e + 1]) * rate);
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) *reinterpret_cast<uint4*>(stage + turned(lane, e)) = make_uint4(w[4 * e], w[4 * e + 1], w[4 * e + 2], w[4 * e + 3]);
+                    __syncwarp();
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const int r = 16 * i + (lane >> 1);
+                        char* to = reinterpret_cast<char*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(dest), r));
+                        if (stores >> r & 1u) *reinterpret_cast<uint4*>(to + x * 2 + (lane & 1) * 16) = *reinterpret_cast<const uint4*>(stage + turned(r, lane & 1));
                     }
                 }
+                __syncwarp();
             }
             tc_fence_before();
         });
