@@ -78,11 +78,11 @@ bool encode_rows(CUtensorMap* map, CUtensorMapDataType type, int width, const vo
                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-bool encode_pages(CUtensorMap* map, const void* base, int dim, int tokens, int heads, int pages, int64_t token_stride, int64_t head_stride, int64_t page_stride, int box_tokens) {
+bool encode_pages(CUtensorMap* map, const void* base, int dim, int tokens, int heads, int pages, int64_t token_stride, int64_t head_stride, int64_t page_stride, int box_tokens, int box_heads) {
     auto bytes = [](int count, int64_t stride) { return (cuuint64_t)(count > 1 ? 2 * stride : 16); };  // (the stride of one is not used)
     const cuuint64_t dims[4] = {(cuuint64_t)dim, (cuuint64_t)tokens, (cuuint64_t)heads, (cuuint64_t)pages};
     const cuuint64_t strides[3] = {bytes(tokens, token_stride), bytes(heads, head_stride), bytes(pages, page_stride)};
-    const cuuint32_t box[4] = {64, (cuuint32_t)box_tokens, 1, 1}, step[4] = {1, 1, 1, 1};
+    const cuuint32_t box[4] = {64, (cuuint32_t)box_tokens, (cuuint32_t)box_heads, 1}, step[4] = {1, 1, 1, 1};
     const EncodeTiled fn = encode_tiled();
     return fn && fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 4, const_cast<void*>(base), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                     CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;

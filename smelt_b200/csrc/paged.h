@@ -59,18 +59,19 @@ struct PagedAppendArgs {
 cudaError_t launch_paged_append(const Launch& l, PagedType type, int head_dim, const PagedAppendArgs& a);
 
 // Work of an attention kernel as one line of steps.  A step is 2^keys keys of an item; an item is one key head of one block of
-// 2^columns (row, query head of the group) pairs of a source; sources are the shared prefix, whose rows are those of the whole batch, and
+// `columns` (row, query head of the group) pairs of a source; sources are the shared prefix, whose rows are those of the whole batch, and
 // the sequences.  Items follow one another source by source, block by block, key head by key head, and every worker (a CTA, or a warp of
 // it) takes as many steps in a row: as many keys, however uneven the lengths are, and no CTA has more than two items that it
 // shares with others, one at each end.  Lengths are read on the device, so that a captured call follows them.  The line is at most 2^30
 // steps (paged_api.cu).
 struct PagedLine {
-    int columns, keys;  // as powers of two
+    int columns, keys;  // keys as a power of two
+    Divisor column_div;
     int ctas, workers;  // workers of a CTA
     int with_prefix, with_own, wide;
     int32_t* cum;     // [n_seqs + 3] written by CTA 0: steps before each source, and the first prefix key that any row sees
-    float* slot_o;    // [2 ctas][2^columns][D] weighted sums of items shared by several CTAs
-    float2* slot_ml;  // [2 ctas][2^columns] their running maxima and sums
+    float* slot_o;    // [2 ctas][columns][D] weighted sums of items shared by several CTAs
+    float2* slot_ml;  // [2 ctas][columns] their running maxima and sums
 };
 struct PagedAttentionArgs {
     PagedArgs c;
@@ -84,12 +85,12 @@ struct PagedAttentionArgs {
     float scale2;  // scale log2(e)
     uint32_t window;
 };
-int paged_narrow_columns(int head_dim, int64_t columns);  // columns of a block of the streaming kernel for so many of a source, and keys of a step, as powers of two
+int paged_narrow_columns(int head_dim, int64_t columns);  // columns of a block of the streaming kernel for so many of a source; keys of a step, as a power of two
 int paged_narrow_keys();
 int paged_narrow_workers(int head_dim);
 cudaError_t launch_paged_narrow(const Launch& l, PagedType type, int head_dim, const PagedAttentionArgs& a, int line);
 // The tensor-core kernel (paged_wide.cu) and whether its shared memory holds a batch of n_seqs.
-int paged_wide_columns(int head_dim);
+int paged_wide_columns(int head_dim, int ratio);
 int paged_wide_keys(int head_dim);
 bool paged_wide_takes(int head_dim, int n_seqs);
 cudaError_t launch_paged_wide(const Launch& l, PagedType type, int head_dim, const PagedAttentionArgs& a, int line);

@@ -19,7 +19,7 @@ smelt_status enter(smelt_cuda_ctx* ctx, Launch* l) {
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 // Rows of `width` 16-bit values, `stride` apart, that 16-byte loads can take.
 bool rows_ok(const void* p, int64_t stride, int64_t width, int64_t rows) {
-    return p && aligned16(p) && stride % 8 == 0 && (rows <= 1 || stride >= width) && stride >= 0 && stride < ((int64_t)1 << 40);
+    return p && aligned16(p) && stride % 8 == 0 && (rows <= 1 || stride >= width) && stride >= 0 && stride < ((int64_t)1 << 38);
 }
 
 smelt_status cache_args(smelt_cuda_ctx* ctx, const smelt_paged_cache* k, const smelt_paged_batch* b, PagedArgs* c) {
@@ -75,13 +75,14 @@ size_t attention_plan(const smelt_cuda_ctx* ctx, const smelt_paged_cache* k, con
         line.with_own = with_own;
         line.with_prefix = with_prefix;
         const int64_t columns = with_own && with_prefix ? (own > prefix ? own : prefix) : with_own ? own : prefix;
-        line.columns = wide ? paged_wide_columns(D) : paged_narrow_columns(D, columns);
+        line.columns = wide ? paged_wide_columns(D, a->c.ratio) : paged_narrow_columns(D, columns);
+        line.column_div = Divisor::of((uint32_t)line.columns);
         line.keys = wide ? paged_wide_keys(D) : paged_narrow_keys();
         line.ctas = ctx->sm_count;
         line.workers = wide ? 1 : paged_narrow_workers(D);
         line.cum = (int32_t*)room((size_t)(b->n_seqs + 3) * sizeof(int32_t));
-        line.slot_o = (float*)room(((size_t)2 * line.ctas << line.columns) * D * sizeof(float));
-        line.slot_ml = (float2*)room(((size_t)2 * line.ctas << line.columns) * sizeof(float2));
+        line.slot_o = (float*)room((size_t)2 * line.ctas * line.columns * D * sizeof(float));
+        line.slot_ml = (float2*)room((size_t)2 * line.ctas * line.columns * sizeof(float2));
     };
     if (prefix == 0) {
         add(own_wide, true, false);
@@ -190,7 +191,7 @@ smelt_status smelt_cuda_paged_attention(smelt_cuda_ctx* ctx, const smelt_paged_c
         double steps = 0;
         for (int i = 0; i < a.lines; ++i) {
             const PagedLine& line = a.line[i];
-            const double blocks = (double)(rows * a.c.ratio >> line.columns) + 1;
+            const double blocks = (double)(rows * a.c.ratio / line.columns) + 1;
             if (line.with_own) steps += (blocks + batch->n_seqs) * cache->n_kv * ((a.c.table_tokens >> line.keys) + 2.0);
             if (line.with_prefix) steps += blocks * cache->n_kv * ((batch->prefix_length >> line.keys) + 2.0);
         }

@@ -180,13 +180,13 @@ __global__ void __launch_bounds__(kWarps<D> * 32, 1) paged_narrow_kernel(const _
     const uint32_t k_lane = smem_u32(ring) + ((lane & 7) + ((lane >> 3) & 1) * 8) * PITCH + (lane >> 4) * 16;
     const uint32_t v_lane = smem_u32(ring) + ((lane & 7) + (lane >> 4) * 8) * PITCH + ((lane >> 3) & 1) * 16;
     auto seq_of = [&](int source) { return source == 0 ? Seq{0, batch.row[c.n_seqs], 0} : batch.seq(source - 1); };
-    auto width_of = [&](const Cursor& x, const Seq& s) { return min(1 << line.columns, s.n * c.ratio - (x.block << line.columns)); };
+    auto width_of = [&](const Cursor& x, const Seq& s) { return min(line.columns, s.n * c.ratio - x.block * line.columns); };
     auto load_queries = [&](const Cursor& x) {
         const Seq s = seq_of(x.source);
         const int width = width_of(x, s);
 #pragma unroll
         for (int nh = 0; nh < NH; ++nh) {
-            const int f = (x.block << line.columns) + nh * 8 + g, i = divide(f, c.ratio_div);
+            const int f = x.block * line.columns + nh * 8 + g, i = divide(f, c.ratio_div);
             const E* row_q = q + (size_t)(s.row + i) * a.q_stride + (size_t)(x.head * c.ratio + f - i * c.ratio) * D + 2 * t;
             const bool live = nh * 8 + g < width;
 #pragma unroll
@@ -215,7 +215,7 @@ __global__ void __launch_bounds__(kWarps<D> * 32, 1) paged_narrow_kernel(const _
     for (int pos = begin; pos < end;) {
         // ── an item: its columns' key ranges ──
         const Seq seq = seq_of(cur.source);
-        const int f0 = cur.block << line.columns, width = width_of(cur, seq);
+        const int f0 = cur.block * line.columns, width = width_of(cur, seq);
         auto range_of = [&](int f) -> Range {
             if (f >= width) return {0, 0};
             const int i = divide(f0 + f, c.ratio_div);
@@ -457,7 +457,7 @@ __global__ void __launch_bounds__(kWarps<D> * 32, 1) paged_narrow_kernel(const _
         const uint32_t members = valid & ~((1u << p0) - 1u) & (p1 < 32 ? (1u << p1) - 1u : 0xffffffffu);
         const Part part = parts[p0];
         const Seq seq = part.source == 0 ? Seq{0, batch.row[c.n_seqs], 0} : batch.seq(part.source - 1);
-        const int f0 = part.block << line.columns, width = min(1 << line.columns, seq.n * c.ratio - f0);
+        const int f0 = part.block * line.columns, width = min(line.columns, seq.n * c.ratio - f0);
         const bool here = part.at >= cta_begin && part.at + part.steps <= cta_end;
         for (int f = 0; f < width; ++f) {
             if ((turn++ & (W - 1)) != warp) continue;
@@ -484,7 +484,7 @@ __global__ void __launch_bounds__(kWarps<D> * 32, 1) paged_narrow_kernel(const _
 #pragma unroll
                 for (int k = 0; k < D / 32; ++k) to[32 * k] = round_to<E>(sum[k] * rate);
             } else {
-                const size_t to = here ? ((part.source == 0 ? (size_t)c.rows : 0) + out_row) * c.n_q + out_head : ((size_t)(2 * blockIdx.x + (part.at < cta_begin ? 0 : 1)) << line.columns) + f;
+                const size_t to = here ? ((part.source == 0 ? (size_t)c.rows : 0) + out_row) * c.n_q + out_head : (size_t)(2 * blockIdx.x + (part.at < cta_begin ? 0 : 1)) * line.columns + f;
                 float* o_to = (here ? a.whole_o : line.slot_o) + to * D + lane;
 #pragma unroll
                 for (int k = 0; k < D / 32; ++k) o_to[32 * k] = sum[k];
@@ -539,20 +539,20 @@ __global__ void __launch_bounds__(kMergeWarps * 32) paged_merge_kernel(const __g
 #pragma unroll 1
         for (int prefix = line.with_prefix ? 1 : 0; prefix >= (line.with_own ? 0 : 1); --prefix) {
             // the item of this row and head: its first step on the line, and its steps
-            const int f = (prefix ? r : i) * c.ratio + h - head * c.ratio, block = f >> line.columns, col = f & ((1 << line.columns) - 1);
+            const int f = (prefix ? r : i) * c.ratio + h - head * c.ratio, block = divide(f, line.column_div), col = f - block * line.columns;
             int at = prefix ? 0 : line.cum[s + 1], steps;
             if (prefix) {
                 steps = steps_of({line.cum[c.n_seqs + 2], c.prefix_length}, line.keys);
                 at += block * c.n_kv * steps;
             } else {
                 int before = 0;
-                for (int b = lane; b < block; b += 32) before += c.n_kv * steps_of(block_keys(c, seq, b, line.columns, a.window), line.keys);
+                for (int b = lane; b < block; b += 32) before += c.n_kv * steps_of(block_keys(c, line, seq, b, a.window), line.keys);
                 if (block) {
 #pragma unroll
                     for (int k = 16; k > 0; k >>= 1) before += __shfl_xor_sync(0xffffffffu, before, k);
                 }
                 at += before;
-                steps = steps_of(block_keys(c, seq, block, line.columns, a.window), line.keys);
+                steps = steps_of(block_keys(c, line, seq, block, a.window), line.keys);
             }
             if (steps == 0) continue;
             at += head * steps;
@@ -561,15 +561,15 @@ __global__ void __launch_bounds__(kMergeWarps * 32) paged_merge_kernel(const __g
             if (whole && !a.whole_o) return;  // written by the CTA that finished it
             const size_t whole_at = ((prefix ? (size_t)c.rows : 0) + r) * c.n_q + h;
             const int parts = last - first + 1;
-            const float* part0 = whole ? a.whole_o + whole_at * D : line.slot_o + (((size_t)(2 * first + (at < share.cta_begin(first) ? 0 : 1)) << line.columns) + col) * D;
+            const float* part0 = whole ? a.whole_o + whole_at * D : line.slot_o + ((size_t)(2 * first + (at < share.cta_begin(first) ? 0 : 1)) * line.columns + col) * D;
             // every part but the first begins in front of its CTA's stretch: slot 0
-            const float* part1 = line.slot_o + (((size_t)(2 * (first + 1)) << line.columns) + col) * D;
-            const size_t stride = ((size_t)2 << line.columns) * D;
+            const float* part1 = line.slot_o + ((size_t)(2 * (first + 1)) * line.columns + col) * D;
+            const size_t stride = (size_t)2 * line.columns * D;
 #pragma unroll 1
             for (int base = 0; base < parts; base += 32) {
                 const int k = base + lane;
                 float2 ml = make_float2(kLowest, 0.f);
-                if (k < parts) ml = whole ? __ldcg(a.whole_ml + whole_at) : __ldcg(line.slot_ml + ((size_t)(2 * (first + k) + (k == 0 && at >= share.cta_begin(first) ? 1 : 0)) << line.columns) + col);
+                if (k < parts) ml = whole ? __ldcg(a.whole_ml + whole_at) : __ldcg(line.slot_ml + (size_t)(2 * (first + k) + (k == 0 && at >= share.cta_begin(first) ? 1 : 0)) * line.columns + col);
                 const bool counts = ml.y != 0.f;  // a part that the row sees nothing of adds nothing, whatever its sums are
                 const float here = counts ? ml.x : kLowest, m = fmaxf(top, warp_max(here)), mine = exp2_approx(top - m), factor = counts ? exp2_approx(here - m) : 0.f;
                 top = m;
@@ -633,12 +633,12 @@ cudaError_t narrow(const Launch& l, PagedType type, const PagedAttentionArgs& a,
 
 }  // namespace
 
-int paged_narrow_columns(int head_dim, int64_t columns) { return columns <= 8 || head_dim == 256 ? 3 : columns <= 16 || head_dim == 128 ? 4 : 5; }
+int paged_narrow_columns(int head_dim, int64_t columns) { return columns <= 8 || head_dim == 256 ? 8 : columns <= 16 || head_dim == 128 ? 16 : 32; }
 int paged_narrow_keys() { return 5; }
 int paged_narrow_workers(int head_dim) { return head_dim == 256 ? kWarps<256> : kWarps<128>; }
 
 cudaError_t launch_paged_narrow(const Launch& l, PagedType type, int head_dim, const PagedAttentionArgs& a, int line) {
-    const int groups = 1 << (a.line[line].columns - 3);
+    const int groups = a.line[line].columns / 8;
     if (head_dim == 64) return groups == 1 ? narrow<64, 1>(l, type, a, line) : groups == 2 ? narrow<64, 2>(l, type, a, line) : narrow<64, 4>(l, type, a, line);
     if (head_dim == 128) return groups == 1 ? narrow<128, 1>(l, type, a, line) : narrow<128, 2>(l, type, a, line);
     return narrow<256, 1>(l, type, a, line);

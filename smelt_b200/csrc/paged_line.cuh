@@ -26,16 +26,16 @@ __device__ __forceinline__ Range prefix_keys(const Seq& s, int i, int P, uint32_
     return {window ? min(P, max(0, P - (int)window + token + 1)) : 0, P};
 }
 // Keys that some row of a block of a sequence sees.
-__device__ __forceinline__ Range block_keys(const PagedArgs& c, const Seq& s, int block, int columns, uint32_t window) {
-    const int f0 = block << columns, f1 = min(s.n * c.ratio, f0 + (1 << columns)) - 1;
+__device__ __forceinline__ Range block_keys(const PagedArgs& c, const PagedLine& line, const Seq& s, int block, uint32_t window) {
+    const int f0 = block * line.columns, f1 = min(s.n * c.ratio, f0 + line.columns) - 1;
     return {own_keys(s, divide(f0, c.ratio_div), window).lo, own_keys(s, divide(f1, c.ratio_div), window).hi};
 }
-__device__ __forceinline__ int blocks_of(const PagedArgs& c, int rows, int columns) { return (rows * c.ratio + (1 << columns) - 1) >> columns; }
+__device__ __forceinline__ int blocks_of(const PagedArgs& c, const PagedLine& line, int rows) { return divide(rows * c.ratio + line.columns - 1, line.column_div); }
 __device__ __forceinline__ int steps_of(const Range& r, int keys) { return r.hi > r.lo ? ((r.hi - 1) >> keys) - (r.lo >> keys) + 1 : 0; }
 // Steps of all blocks of a sequence, those of one key head.
 __device__ __forceinline__ int steps_of_seq(const PagedArgs& c, const PagedLine& line, const Seq& s, int blocks, uint32_t window) {
     int sum = 0;
-    for (int k = 0; k < blocks; ++k) sum += steps_of(block_keys(c, s, k, line.columns, window), line.keys);
+    for (int k = 0; k < blocks; ++k) sum += steps_of(block_keys(c, line, s, k, window), line.keys);
     return sum;
 }
 
@@ -68,7 +68,7 @@ __device__ __forceinline__ void scan_line(const PagedArgs& c, const PagedLine& l
     int mine = 0;
     for (int s = s0; s < s1; ++s) {
         const Seq q = b.seq(s);
-        if (line.with_own) mine += c.n_kv * steps_of_seq(c, line, q, blocks_of(c, q.n, line.columns), window);
+        if (line.with_own) mine += c.n_kv * steps_of_seq(c, line, q, blocks_of(c, line, q.n), window);
         if (line.with_prefix && window && q.n) atomicMin(&lowest, prefix_keys(q, 0, c.prefix_length, window).lo);
     }
     int run = mine;
@@ -85,14 +85,14 @@ __device__ __forceinline__ void scan_line(const PagedArgs& c, const PagedLine& l
     int before = run - mine;
     if (n > 32 * per)
         for (int w = 0; w < warp; ++w) before += warp_sums[w];
-    if (line.with_prefix) before += c.n_kv * blocks_of(c, b.row[n], line.columns) * steps_of({b.prefix_lo, c.prefix_length}, line.keys);
+    if (line.with_prefix) before += c.n_kv * blocks_of(c, line, b.row[n]) * steps_of({b.prefix_lo, c.prefix_length}, line.keys);
     if (tid == 0) { b.cum[0] = 0; b.cum[1] = before; }
     if (per == 1) {
         if (s0 < s1) b.cum[s0 + 2] = before + mine;
     } else {
         for (int s = s0; s < s1; ++s) {
             const Seq q = b.seq(s);
-            if (line.with_own) before += c.n_kv * steps_of_seq(c, line, q, blocks_of(c, q.n, line.columns), window);
+            if (line.with_own) before += c.n_kv * steps_of_seq(c, line, q, blocks_of(c, line, q.n), window);
             b.cum[s + 2] = before;
         }
     }
@@ -124,12 +124,12 @@ struct Cursor {
     int n_blocks;
 
     __device__ __forceinline__ void load_block(const PagedArgs& c, const PagedLine& line, uint32_t window, const Batch& b) {
-        keys = source == 0 ? Range{b.prefix_lo, c.prefix_length} : block_keys(c, b.seq(source - 1), block, line.columns, window);
+        keys = source == 0 ? Range{b.prefix_lo, c.prefix_length} : block_keys(c, line, b.seq(source - 1), block, window);
         steps = steps_of(keys, line.keys);
         first = keys.lo >> line.keys;
     }
     __device__ __forceinline__ void load_source(const PagedArgs& c, const PagedLine& line, const Batch& b) {
-        n_blocks = blocks_of(c, source == 0 ? b.row[c.n_seqs] : b.seq(source - 1).n, line.columns);
+        n_blocks = blocks_of(c, line, source == 0 ? b.row[c.n_seqs] : b.seq(source - 1).n);
     }
     // at < cum[n_seqs + 1]
     __device__ __forceinline__ void seek(const PagedArgs& c, const PagedLine& line, uint32_t window, const Batch& b, int at) {

@@ -1,8 +1,8 @@
 // Attention over pages for blocks of many columns (prompt chunks, drafts of wide groups, a prefix that a whole batch shares): the
 // products on the fifth-generation tensor core.
 //
-// A block is 256 columns ((row, query head of the group) pairs of one key head; 128 with heads of 256) as two tiles of 128 lanes of tensor memory, a step
-// 128 keys (64).  Roles: four warps copy pages to shared memory (16-byte cp.async a row, so pages may have any size and strides;
+// A block is up to 256 columns ((row, query head of the group) pairs of one key head; 128 with heads of 256) as two tiles of up to 128 lanes of
+// tensor memory, whole rows where a group has no more than 128 heads, a step 128 keys (64).  Roles: four warps copy pages to shared memory (16-byte cp.async a row, so pages may have any size and strides;
 // 128-byte swizzle), one warp issues the products S = Q K^T and O += P V, and two sets of four warps take a tile each: a thread has
 // a column, so the softmax needs no exchange.  P overwrites S in tensor memory and is the product's operand from there.  While one
 // set is at its exponentials (128 x 128 of them take the SM's 16 a clock 1024 clocks) the tensor core works for the other (1024 clocks a
@@ -161,8 +161,8 @@ struct Item {
 __device__ __forceinline__ Item item_of(const PagedArgs& c, const PagedLine& line, uint32_t window, const Batch& b, const Cursor& cur) {
     Item it;
     it.seq = cur.source == 0 ? Seq{0, b.row[c.n_seqs], 0} : b.seq(cur.source - 1);
-    it.f0 = cur.block << line.columns;
-    it.width = min(1 << line.columns, it.seq.n * c.ratio - it.f0);
+    it.f0 = cur.block * line.columns;
+    it.width = min(line.columns, it.seq.n * c.ratio - it.f0);
     // of the prefix: without a window all columns, but for rows without a token, whose sums are dropped
     it.clear = cur.source ? Range{own_keys(it.seq, divide(it.f0 + it.width - 1, c.ratio_div), window).lo, own_keys(it.seq, divide(it.f0, c.ratio_div), window).hi} : window ? Range{0, 0} : Range{0, c.prefix_length};
     return it;
@@ -171,10 +171,11 @@ __device__ __forceinline__ Item item_of(const PagedArgs& c, const PagedLine& lin
 template <int REGS> __device__ __forceinline__ void registers_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS)); }
 template <int REGS> __device__ __forceinline__ void registers_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS)); }
 
-// What the tensor map reads: boxes of `tokens` tokens, and how many of them make a step.
+// What the tensor maps read: boxes of `tokens` tokens, of which `boxes` make a step, and all query heads of a group of q_rows rows, which
+// make a tile (0: a tile is 128 columns, from wherever in a row, and is copied column by column).
 struct Pages {
-    CUtensorMap k, v;
-    int tokens, boxes;
+    CUtensorMap k, v, q;
+    int tokens, boxes, q_rows;
 };
 
 // TILED: pages come as boxes of a tensor map; else row by row.
@@ -196,7 +197,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_wide_kernel(const _
             mbar_init(&sh.k_empty[i], 1); mbar_init(&sh.v_empty[i], 1);
         }
         for (int i = 0; i < 2; ++i) { mbar_init(&sh.s_full[i], 1); mbar_init(&sh.p_ready[i], 4); mbar_init(&sh.pv_done[i], 1); }
-        mbar_init(&sh.q_full, 4);
+        mbar_init(&sh.q_full, 1);
         mbar_init(&sh.q_empty, 1);
         sh.dead = 0;
         if (TILED) {
@@ -218,6 +219,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_wide_kernel(const _
     const int begin = share.cta_begin(blockIdx.x), end = share.cta_begin(blockIdx.x + 1);
     // A role that gives up a wait goes through the rest of its schedule without work, so that no barrier is short of a thread.
     bool alive = true;
+    const int tile_columns = C::kSets == 2 ? line.columns >> 1 : line.columns;
     // An item's steps in this CTA: tasks, one a step, or with two tiles one a tile and step; task T of the CTA has score buffer T & 1.
     auto each_item = [&](auto&& body) {
         if (begin >= end) return;
@@ -227,7 +229,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_wide_kernel(const _
         for (int pos = begin; pos < end;) {
             const int n = min(cur.steps - cur.step, end - pos);
             const Item it = item_of(c, line, a.window, batch, cur);
-            const bool pair = it.width > 128;
+            const bool pair = it.width > tile_columns;
             const int tasks = pair ? 2 * n : n;
             body(cur, it, pair, n, tasks, task, step, pos);
             task += tasks;
@@ -297,8 +299,16 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_wide_kernel(const _
             hand_over_values();
             if (items > 0) warp_wait(&sh.q_empty, (items - 1) & 1);
             ++items;
-            if (alive) {
-#pragma unroll 4
+            if (pages.q_rows) {
+                if (warp == C::kLoadWarp && lane == 0 && alive) {
+                    const int tiles = pair ? 2 : 1, row = it.seq.row + divide(it.f0, c.ratio_div);
+                    arrive_expect_at(smem_u32(&sh.q_full), tiles * tile_columns * D * 2);
+                    for (int i = 0; i < tiles; ++i)
+#pragma unroll
+                        for (int x = 0; x < D / 64; ++x)
+                            tma_load_4d_at(smem_u32(q_tiles + i * C::kQTile) + x * (128 * 128), &pages.q, 64 * x, cur.head * c.ratio, row + i * pages.q_rows, 0, smem_u32(&sh.q_full));
+                }
+            } else if (alive) {
                 for (int f = r_first; f < (pair ? 256 : 128); f += ROWS) {
                     const int ff = it.f0 + f, i = divide(ff, c.ratio_div);
                     const bool live = f < it.width;
@@ -309,13 +319,10 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_wide_kernel(const _
             }
             cp_async_commit();
             auto hand_over_queries = [&] {
-                if (a.scale2 < 0.f && alive)  // the softmax wants a positive scale
-                    for (int f = r_first; f < (pair ? 256 : 128); f += ROWS)
-                        for (int k = ch; k < CHUNKS; k += LANES) {
-                            uint4* v = reinterpret_cast<uint4*>(q_tiles + (f >> 7) * C::kQTile + place(128, f & 127, k));
-                            *v = make_uint4(v->x ^ 0x80008000u, v->y ^ 0x80008000u, v->z ^ 0x80008000u, v->w ^ 0x80008000u);
-                        }
-                arrive(&sh.q_full);
+                if (pages.q_rows) return;
+                fence_async_smem();
+                barrier(1, 128);
+                if (lt == 0) mbar_arrive(&sh.q_full);
             };
             const int32_t* table = cur.source == 0 ? c.prefix_table : c.table + (size_t)(cur.source - 1) * c.table_stride;
             const long long head_at = (long long)cur.head * c.head_stride;
@@ -479,7 +486,8 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_wide_kernel(const _
         // ── softmax: a thread a column ──
         const int set = warp >> 2, me = (warp & 3) * 32 + lane;
         const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16), o_at = lanes + C::kSum + set * D;
-        const float scale2 = fabsf(a.scale2);
+        const float scale2 = fabsf(a.scale2);  // the maximum wants a positive one
+        const bool negative = a.scale2 < 0.f;
         auto wait = [&](uint64_t* bar, uint32_t parity) {
             alive = __all_sync(0xffffffffu, alive && wait_alive(bar, parity, dead)) != 0;
             tc_fence_after();
@@ -489,6 +497,9 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_wide_kernel(const _
         auto weigh = [&](auto all, uint32_t s_at, int k0, const Range& keys, bool begun, uint32_t last) {
             uint32_t v[KEYS];
             load_scores<KEYS>(s_at, v);
+            if (negative)
+#pragma unroll
+                for (int e = 0; e < KEYS; ++e) v[e] ^= 0x80000000u;
             float top = kLowest;
             if constexpr (!decltype(all)::value) {  // NaN marks a key that the column does not see: a maximum passes it over
 #pragma unroll
@@ -550,7 +561,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_wide_kernel(const _
             }
         };
         each_item([&](const Cursor& cur, const Item& it, bool pair, int n, int tasks, uint32_t task0, uint32_t step0, int pos) {
-            const int t_first = C::kSets == 1 ? 0 : (int)((task0 & 1) ^ set), f = (pair ? t_first * 128 : 0) + me, ff = it.f0 + f;
+            const int t_first = C::kSets == 1 ? 0 : (int)((task0 & 1) ^ set), f = me < tile_columns ? (pair ? t_first * tile_columns : 0) + me : 256, ff = it.f0 + f;
             Range keys = {0, 0};
             if (f < it.width) {
                 const int i = divide(ff, c.ratio_div);
@@ -646,7 +657,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_wide_kernel(const _
             float* part = nullptr;
             float2* part_ml = nullptr;
             if (!here) {
-                const size_t at = ((size_t)(2 * blockIdx.x + (item_at < begin ? 0 : 1)) << line.columns) + f;
+                const size_t at = (size_t)(2 * blockIdx.x + (item_at < begin ? 0 : 1)) * line.columns + f;
                 part = line.slot_o + at * D;
                 part_ml = line.slot_ml + at;
             } else if (a.whole_o) {
@@ -759,14 +770,16 @@ cudaError_t go(const Launch& l, const PagedAttentionArgs& a, int line) {
     pages.tokens = c.page_size < KEYS ? c.page_size : KEYS;
     pages.boxes = KEYS / pages.tokens;
     const bool tiled = pages.tokens % 8 == 0 && KEYS % pages.tokens == 0 && c.page_size % pages.tokens == 0 &&
-                       encode_pages(&pages.k, c.k, D, c.page_size, c.n_kv, c.n_pages, c.token_stride, c.head_stride, c.page_stride, pages.tokens) &&
-                       encode_pages(&pages.v, c.v, D, c.page_size, c.n_kv, c.n_pages, c.token_stride, c.head_stride, c.page_stride, pages.tokens);
+                       encode_pages(&pages.k, c.k, D, c.page_size, c.n_kv, c.n_pages, c.token_stride, c.head_stride, c.page_stride, pages.tokens, 1) &&
+                       encode_pages(&pages.v, c.v, D, c.page_size, c.n_kv, c.n_pages, c.token_stride, c.head_stride, c.page_stride, pages.tokens, 1);
+    pages.q_rows = c.ratio <= 128 ? 128 / c.ratio : 0;
+    if (pages.q_rows && !encode_pages(&pages.q, a.q, D, c.n_q, c.rows, 1, D, a.q_stride, 0, c.ratio, pages.q_rows)) return cudaErrorInvalidValue;
     return tiled ? run<D, E, true>(l, a, line, pages) : run<D, E, false>(l, a, line, pages);
 }
 
 }  // namespace
 
-int paged_wide_columns(int head_dim) { return head_dim == 256 ? 7 : 8; }
+int paged_wide_columns(int head_dim, int ratio) { return (head_dim == 256 ? 1 : 2) * (ratio <= 128 ? 128 / ratio * ratio : 128); }
 int paged_wide_keys(int head_dim) { return head_dim == 256 ? 6 : 7; }
 bool paged_wide_takes(int head_dim, int n_seqs) {
     const size_t most = 227 * 1024 - 1024;  // less what the scan of the batch holds, up to the tiles' alignment

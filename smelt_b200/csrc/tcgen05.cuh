@@ -163,7 +163,7 @@ __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.
 // A row-major matrix of `width`-byte elements read in boxes of box_rows rows x 128 bytes, 128-byte swizzle; beyond its edges: zeros
 // (affine_line.cu).
 bool encode_rows(CUtensorMap* map, CUtensorMapDataType type, int width, const void* base, long rows, long cols, int box_rows);
-// Pages of 16-bit values [page][head][token][dim] with strides in values, read in boxes of 64 values of box_tokens tokens, 128-byte swizzle.
-bool encode_pages(CUtensorMap* map, const void* base, int dim, int tokens, int heads, int pages, int64_t token_stride, int64_t head_stride, int64_t page_stride, int box_tokens);
+// Pages of 16-bit values [page][head][token][dim] with strides in values, read in boxes of 64 values of box_tokens tokens of box_heads heads, 128-byte swizzle.
+bool encode_pages(CUtensorMap* map, const void* base, int dim, int tokens, int heads, int pages, int64_t token_stride, int64_t head_stride, int64_t page_stride, int box_tokens, int box_heads);
 
 }  // namespace smelt
