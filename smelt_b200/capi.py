@@ -275,6 +275,9 @@ def load(build_if_missing: bool = True) -> C.CDLL:
     return lib
 
 
+_PLAIN = {int, float, type(None), bytes, type(C.byref(C.c_int()))}  # what ctypes takes as it is
+
+
 def _vp(x):
     if isinstance(x, DeviceBuffer):
         return x.ptr
@@ -383,7 +386,7 @@ class Context:
 
     def call(self, name: str, *args):
         """Call ``smelt_cuda_<name>(ctx, *args)`` and raise on a non-zero status."""
-        self._check(getattr(self.lib, "smelt_cuda_" + name)(self.h, *[_vp(a) for a in args]))
+        self._check(getattr(self.lib, "smelt_cuda_" + name)(self.h, *[a if a.__class__ in _PLAIN else _vp(a) for a in args]))
 
     def call_status(self, name: str, *args) -> int:
         return getattr(self.lib, "smelt_cuda_" + name)(self.h, *[_vp(a) for a in args])

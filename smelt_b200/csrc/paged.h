@@ -62,10 +62,11 @@ cudaError_t launch_paged_append(const Launch& l, PagedType type, int head_dim, c
 // `columns` (row, query head of the group) pairs of a source; sources are the shared prefix, whose rows are those of the whole batch, and
 // the sequences.  Items follow one another source by source, block by block, key head by key head, and every worker (a CTA, or a warp of
 // it) takes as many steps in a row: as many keys, however uneven the lengths are, and no CTA has more than two items that it
-// shares with others, one at each end.  Lengths are read on the device, so that a captured call follows them.  The line is at most 2^30
+// shares with others, one at each end.  In front of an item's steps lie `extra` places that stand for what its beginning and end cost; nobody does
+// anything there.  Lengths are read on the device, so that a captured call follows them.  The line is at most 2^30
 // steps (paged_api.cu).
 struct PagedLine {
-    int columns, keys;  // keys as a power of two
+    int columns, keys, extra;  // keys as a power of two
     Divisor column_div;
     int ctas, workers;  // workers of a CTA
     int with_prefix, with_own, wide;

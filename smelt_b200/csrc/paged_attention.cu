@@ -123,12 +123,13 @@ __global__ void __launch_bounds__(kWarps<D> * 32, 1) paged_narrow_kernel(const _
     Cursor cur;
     cur.seek(c, line, a.window, batch, begin);
     Cursor ahead = cur;  // the step whose pages are looked up next
-    int at = begin;
+    bool more = false;   // there is a tile that is issued next
     int page = 0, slot = 0, head = 0;  // page and place of the lane's key of the tile that is issued next
     bool inside = false;               // ... which is one of the item's
     auto look_up = [&]() {
         inside = false;
-        if (at >= end) return;
+        more = ahead.at < end;
+        if (!more) return;
         const int key = (ahead.first + ahead.step) * kTile + lane;
         head = ahead.head;
         inside = key >= ahead.keys.lo && key < ahead.keys.hi;
@@ -138,21 +139,24 @@ __global__ void __launch_bounds__(kWarps<D> * 32, 1) paged_narrow_kernel(const _
             slot = key - p * c.page_size;
             page = table[p];
         }
-        if (++at < end) ahead.advance(c, line, a.window, batch);
+        ahead.advance(c, line, a.window, batch);
     };
     constexpr int LANES = D / 8 < 32 ? D / 8 : 32, TURN = 32 / LANES;  // lanes of a row of 16-byte pieces, rows of a turn of the warp
     const int turn_row = lane / LANES;
     const E *k_pool = static_cast<const E*>(c.k) + lane % LANES * 8, *v_pool = static_cast<const E*>(c.v) + lane % LANES * 8;
     const uint32_t ring_at = smem_u32(ring) + turn_row * PITCH + lane % LANES * 16;
     uint32_t there = 0;  // keys of the tile that are read; the others' rows are zeros
+    bool tile = false;   // there is a tile that is issued
     auto issue_unit = [&](int w, int place) {  // unit w of a tile
         if (w == 0) {
+            tile = more;
             bool take = inside && (uint32_t)page < (uint32_t)c.n_pages;
             if (inside && !take && c.err) atomicOr(c.err, KERR_BAD_PAGE);
             rows[lane] = take ? (long long)page * c.page_stride + (long long)slot * c.token_stride + (long long)head * c.head_stride : 0;
             there = __ballot_sync(0xffffffffu, take);
             look_up();
         }
+        if (!tile) return;
         __syncwarp();  // the rows are there, and the unit's last readers are through
         const E* pool = w < kGroups ? k_pool : v_pool;
         const uint32_t dst = ring_at + place * UNIT;
@@ -167,7 +171,6 @@ __global__ void __launch_bounds__(kWarps<D> * 32, 1) paged_narrow_kernel(const _
         }
     };
     look_up();
-    const int n_units = 2 * kGroups * (end - begin);
     int issued = 0, issue_place = 0, freed = NU;  // the next unit to issue, its place in the ring, and up to which unit there is room
 
     const E* q = static_cast<const E*>(a.q);
@@ -197,7 +200,7 @@ __global__ void __launch_bounds__(kWarps<D> * 32, 1) paged_narrow_kernel(const _
     auto arrived = [&]() {  // in one place of the code: it is long, and short calls wait for instructions as for anything else
 #pragma unroll 1
         for (; issued < freed; ++issued) {
-            if (issued < n_units) issue_unit(issued % (2 * kGroups), issue_place);
+            issue_unit(issued % (2 * kGroups), issue_place);
             cp_async_commit();
             if (++issue_place == NU) issue_place = 0;
         }
@@ -211,8 +214,8 @@ __global__ void __launch_bounds__(kWarps<D> * 32, 1) paged_narrow_kernel(const _
         freed += kGroups;
     };
 
-    load_queries(cur);
-    for (int pos = begin; pos < end;) {
+    if (cur.at < end) load_queries(cur);
+    while (cur.at < end) {
         // ── an item: its columns' key ranges ──
         const Seq seq = seq_of(cur.source);
         const int f0 = cur.block * line.columns, width = width_of(cur, seq);
@@ -243,7 +246,7 @@ __global__ void __launch_bounds__(kWarps<D> * 32, 1) paged_narrow_kernel(const _
             clear_hi = min(clear_hi, __shfl_xor_sync(0xffffffffu, clear_hi, off));
         }
         const Cursor item = cur;
-        const int item_at = pos - cur.step;  // the item's first step on the line
+        const int item_at = cur.at - cur.step;  // the item's first step on the line
 
         // ── its steps in this warp's stretch: keys, then values ──
         uint32_t pb[kGroups][NH][4];
@@ -333,11 +336,9 @@ __global__ void __launch_bounds__(kWarps<D> * 32, 1) paged_narrow_kernel(const _
                         pb[z][nh][2] = movmatrix_trans(TileElem<E>::pack(p[0] - fa.x, p[1] - fa.y));
                         pb[z][nh][3] = movmatrix_trans(TileElem<E>::pack(p[2] - fc.x, p[3] - fc.y));
                     }
-                last = cur.step + 1 == cur.steps || pos + 1 == end;
-                if (++pos < end) {
-                    cur.advance(c, line, a.window, batch);
-                    if (last) load_queries(cur);  // of the next item, on their way meanwhile
-                }
+                last = cur.step + 1 == cur.steps || cur.at + 1 == end;
+                cur.advance(c, line, a.window, batch);
+                if (last && cur.at < end) load_queries(cur);  // of the next item, on their way meanwhile
             } else {
 #pragma unroll
                 for (int z = 0; z < kGroups; ++z) {
@@ -543,10 +544,10 @@ __global__ void __launch_bounds__(kMergeWarps * 32) paged_merge_kernel(const __g
             int at = prefix ? 0 : line.cum[s + 1], steps;
             if (prefix) {
                 steps = steps_of({line.cum[c.n_seqs + 2], c.prefix_length}, line.keys);
-                at += block * c.n_kv * steps;
+                at += block * c.n_kv * places_of(line, steps);
             } else {
                 int before = 0;
-                for (int b = lane; b < block; b += 32) before += c.n_kv * steps_of(block_keys(c, line, seq, b, a.window), line.keys);
+                for (int b = lane; b < block; b += 32) before += c.n_kv * places_of(line, steps_of(block_keys(c, line, seq, b, a.window), line.keys));
                 if (block) {
 #pragma unroll
                     for (int k = 16; k > 0; k >>= 1) before += __shfl_xor_sync(0xffffffffu, before, k);
@@ -555,7 +556,7 @@ __global__ void __launch_bounds__(kMergeWarps * 32) paged_merge_kernel(const __g
                 steps = steps_of(block_keys(c, line, seq, block, a.window), line.keys);
             }
             if (steps == 0) continue;
-            at += head * steps;
+            at += head * places_of(line, steps) + line.extra;
             const int first = share.cta_of(at), last = share.cta_of(at + steps - 1);
             const bool whole = first == last;
             if (whole && !a.whole_o) return;  // written by the CTA that finished it

@@ -32,16 +32,17 @@ __device__ __forceinline__ Range block_keys(const PagedArgs& c, const PagedLine&
 }
 __device__ __forceinline__ int blocks_of(const PagedArgs& c, const PagedLine& line, int rows) { return divide(rows * c.ratio + line.columns - 1, line.column_div); }
 __device__ __forceinline__ int steps_of(const Range& r, int keys) { return r.hi > r.lo ? ((r.hi - 1) >> keys) - (r.lo >> keys) + 1 : 0; }
-// Steps of all blocks of a sequence, those of one key head.
-__device__ __forceinline__ int steps_of_seq(const PagedArgs& c, const PagedLine& line, const Seq& s, int blocks, uint32_t window) {
+// Places on the line of an item of so many steps, and of all blocks of a sequence and one key head.
+__device__ __forceinline__ int places_of(const PagedLine& line, int steps) { return steps ? steps + line.extra : 0; }
+__device__ __forceinline__ int places_of_seq(const PagedArgs& c, const PagedLine& line, const Seq& s, int blocks, uint32_t window) {
     int sum = 0;
-    for (int k = 0; k < blocks; ++k) sum += steps_of(block_keys(c, line, s, k, window), line.keys);
+    for (int k = 0; k < blocks; ++k) sum += places_of(line, steps_of(block_keys(c, line, s, k, window), line.keys));
     return sum;
 }
 
 // What a CTA holds of the batch in shared memory.
 struct Batch {
-    int* cum;     // [n_seqs + 2]: steps in front of source 0 (the prefix), 1 (sequence 0), ..., and all of them
+    int* cum;     // [n_seqs + 2]: places in front of source 0 (the prefix), 1 (sequence 0), ..., and all of them
     int* row;     // [n_seqs + 1]
     int* length;  // [n_seqs]
     int prefix_lo;
@@ -68,7 +69,7 @@ __device__ __forceinline__ void scan_line(const PagedArgs& c, const PagedLine& l
     int mine = 0;
     for (int s = s0; s < s1; ++s) {
         const Seq q = b.seq(s);
-        if (line.with_own) mine += c.n_kv * steps_of_seq(c, line, q, blocks_of(c, line, q.n), window);
+        if (line.with_own) mine += c.n_kv * places_of_seq(c, line, q, blocks_of(c, line, q.n), window);
         if (line.with_prefix && window && q.n) atomicMin(&lowest, prefix_keys(q, 0, c.prefix_length, window).lo);
     }
     int run = mine;
@@ -85,14 +86,14 @@ __device__ __forceinline__ void scan_line(const PagedArgs& c, const PagedLine& l
     int before = run - mine;
     if (n > 32 * per)
         for (int w = 0; w < warp; ++w) before += warp_sums[w];
-    if (line.with_prefix) before += c.n_kv * blocks_of(c, line, b.row[n]) * steps_of({b.prefix_lo, c.prefix_length}, line.keys);
+    if (line.with_prefix) before += c.n_kv * blocks_of(c, line, b.row[n]) * places_of(line, steps_of({b.prefix_lo, c.prefix_length}, line.keys));
     if (tid == 0) { b.cum[0] = 0; b.cum[1] = before; }
     if (per == 1) {
         if (s0 < s1) b.cum[s0 + 2] = before + mine;
     } else {
         for (int s = s0; s < s1; ++s) {
             const Seq q = b.seq(s);
-            if (line.with_own) before += c.n_kv * steps_of_seq(c, line, q, blocks_of(c, line, q.n), window);
+            if (line.with_own) before += c.n_kv * places_of_seq(c, line, q, blocks_of(c, line, q.n), window);
             b.cum[s + 2] = before;
         }
     }
@@ -103,7 +104,7 @@ __device__ __forceinline__ void scan_line(const PagedArgs& c, const PagedLine& l
     }
 }
 
-// Who has which steps of the line: the first `more` workers have each + 1, the others `each`; workers from `used` on have none, so that none
+// Who has which places of the line: the first `more` workers have each + 1, the others `each`; workers from `used` on have none, so that none
 // between two owners of an item is without.
 struct Share {
     int workers, used, each, more;
@@ -117,9 +118,10 @@ struct Share {
     }
 };
 
-// A place on the line: a step of an item.
+// A step of an item, at place `at` of the line.
 struct Cursor {
     int source, block, head, step, steps, first;  // source 0: the prefix, s + 1: sequence s; first: step of the item's first key
+    int at;
     Range keys;
     int n_blocks;
 
@@ -131,32 +133,37 @@ struct Cursor {
     __device__ __forceinline__ void load_source(const PagedArgs& c, const PagedLine& line, const Batch& b) {
         n_blocks = blocks_of(c, line, source == 0 ? b.row[c.n_seqs] : b.seq(source - 1).n);
     }
-    // at < cum[n_seqs + 1]
-    __device__ __forceinline__ void seek(const PagedArgs& c, const PagedLine& line, uint32_t window, const Batch& b, int at) {
-        int lo = 0, hi = c.n_seqs;  // the last source with cum <= at
+    // The first step at place `from` or behind it, from < cum[n_seqs + 1].
+    __device__ __forceinline__ void seek(const PagedArgs& c, const PagedLine& line, uint32_t window, const Batch& b, int from) {
+        int lo = 0, hi = c.n_seqs;  // the last source with cum <= from
         while (lo < hi) {
             const int mid = (lo + hi + 1) >> 1;
-            if (b.cum[mid] <= at) lo = mid;
+            if (b.cum[mid] <= from) lo = mid;
             else hi = mid - 1;
         }
         source = lo;
         load_source(c, line, b);
-        int rest = at - b.cum[source];
+        int rest = from - b.cum[source], places;
         for (block = 0;; ++block) {
             load_block(c, line, window, b);
-            const int here = c.n_kv * steps;
-            if (rest < here || block + 1 >= n_blocks) break;
-            rest -= here;
+            places = places_of(line, steps);
+            if (rest < c.n_kv * places || block + 1 >= n_blocks) break;
+            rest -= c.n_kv * places;
         }
-        head = rest / steps;
-        step = rest - head * steps;
+        head = rest / places;
+        const int in = rest - head * places;
+        step = max(in - line.extra, 0);
+        at = from + max(line.extra - in, 0);
     }
-    // To the next step; there is one.
+    // To the next step; where there is none, `at` is behind the line.
     __device__ __forceinline__ void advance(const PagedArgs& c, const PagedLine& line, uint32_t window, const Batch& b) {
+        ++at;
         if (++step < steps) return;
         step = 0;
+        at += line.extra;
         if (++head < c.n_kv) return;
         head = 0;
+        if (at >= b.cum[c.n_seqs + 1]) return;
         do {
             if (++block >= n_blocks) {
                 block = 0;
@@ -165,6 +172,12 @@ struct Cursor {
             }
             load_block(c, line, window, b);
         } while (steps == 0);
+    }
+    // To the next item's first step.
+    __device__ __forceinline__ void next_item(const PagedArgs& c, const PagedLine& line, uint32_t window, const Batch& b) {
+        at += steps - 1 - step;
+        step = steps - 1;
+        advance(c, line, window, b);
     }
     __device__ __forceinline__ bool same_item(const Cursor& o) const { return source == o.source && block == o.block && head == o.head; }
 };

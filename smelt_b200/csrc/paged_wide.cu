@@ -117,7 +117,6 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
     return v;
 }
-constexpr uint32_t kHidden = 0x7FFFF00Du;  // a NaN of our own
 // The loads behind v have arrived (v is named so that nothing is read of it earlier).
 __device__ __forceinline__ void tmem_wait_ld32(uint32_t (&v)[32]) {
     asm volatile("tcgen05.wait::ld.sync.aligned;"
@@ -226,19 +225,15 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_wide_kernel(const _
         Cursor cur;
         cur.seek(c, line, a.window, batch, begin);
         uint32_t task = 0, step = 0;
-        for (int pos = begin; pos < end;) {
-            const int n = min(cur.steps - cur.step, end - pos);
+        while (cur.at < end) {
+            const int n = min(cur.steps - cur.step, end - cur.at);
             const Item it = item_of(c, line, a.window, batch, cur);
             const bool pair = it.width > tile_columns;
             const int tasks = pair ? 2 * n : n;
-            body(cur, it, pair, n, tasks, task, step, pos);
+            body(cur, it, pair, n, tasks, task, step);
             task += tasks;
             step += n;
-            pos += n;
-            if (pos < end) {
-                cur.step = cur.steps - 1;
-                cur.advance(c, line, a.window, batch);
-            }
+            cur.next_item(c, line, a.window, batch);
         }
     };
 
@@ -293,7 +288,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_wide_kernel(const _
             v_behind = -1;
         };
         uint32_t all_steps = 0;
-        each_item([&](const Cursor& cur, const Item& it, bool pair, int n, int, uint32_t, uint32_t step0, int) {
+        each_item([&](const Cursor& cur, const Item& it, bool pair, int n, int, uint32_t, uint32_t step0) {
             // queries, behind everything that was asked for before them
             cp_async_wait<0>();
             hand_over_values();
@@ -441,7 +436,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_wide_kernel(const _
             tc_fence_after();
         };
         uint32_t items = 0, done = 0;
-        each_item([&](const Cursor&, const Item&, bool pair, int, int tasks, uint32_t task0, uint32_t step0, int) {
+        each_item([&](const Cursor&, const Item&, bool pair, int, int tasks, uint32_t task0, uint32_t step0) {
             wait(&sh.q_full, items & 1);
             ++items;
             auto scores = [&](int t) {
@@ -486,7 +481,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_wide_kernel(const _
         // ── softmax: a thread a column ──
         const int set = warp >> 2, me = (warp & 3) * 32 + lane;
         const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16), o_at = lanes + C::kSum + set * D;
-        const float scale2 = fabsf(a.scale2);  // the maximum wants a positive one
+        const float scale2 = fmaxf(fabsf(a.scale2), 1e-30f);  // the maximum wants a positive one, and so does -inf times it
         const bool negative = a.scale2 < 0.f;
         auto wait = [&](uint64_t* bar, uint32_t parity) {
             alive = __all_sync(0xffffffffu, alive && wait_alive(bar, parity, dead)) != 0;
@@ -501,10 +496,10 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_wide_kernel(const _
 #pragma unroll
                 for (int e = 0; e < KEYS; ++e) v[e] ^= 0x80000000u;
             float top = kLowest;
-            if constexpr (!decltype(all)::value) {  // NaN marks a key that the column does not see: a maximum passes it over
+            if constexpr (!decltype(all)::value) {  // keys that the column does not see
 #pragma unroll
                 for (int e = 0; e < KEYS; ++e)
-                    if (k0 + e < keys.lo || k0 + e >= keys.hi) v[e] = kHidden;
+                    if (k0 + e < keys.lo || k0 + e >= keys.hi) v[e] = 0xFF800000u;
             }
             {
                 float most[4] = {kLowest, kLowest, kLowest, kLowest};
@@ -544,11 +539,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_wide_kernel(const _
                 for (int e = 0; e < 32; e += 2) {
                     float y0, y1;
                     split(fma2(pair_of(__uint_as_float(v[x + e]), __uint_as_float(v[x + e + 1])), scales, minus), y0, y1);
-                    float p0 = exp2_approx(y0), p1 = exp2_approx(y1);
-                    if constexpr (!decltype(all)::value) {
-                        if (v[x + e] == kHidden) p0 = 0.f;
-                        if (v[x + e + 1] == kHidden) p1 = 0.f;
-                    }
+                    const float p0 = exp2_approx(y0), p1 = exp2_approx(y1);
                     sums[e >> 1 & 1] = add2(sums[e >> 1 & 1], pair_of(p0, p1));
                     p[e / 2] = Pack<E>::two(p0, p1);
                 }
@@ -560,7 +551,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_wide_kernel(const _
                 l += l0 + l1;
             }
         };
-        each_item([&](const Cursor& cur, const Item& it, bool pair, int n, int tasks, uint32_t task0, uint32_t step0, int pos) {
+        each_item([&](const Cursor& cur, const Item& it, bool pair, int n, int tasks, uint32_t task0, uint32_t step0) {
             const int t_first = C::kSets == 1 ? 0 : (int)((task0 & 1) ^ set), f = me < tile_columns ? (pair ? t_first * tile_columns : 0) + me : 256, ff = it.f0 + f;
             Range keys = {0, 0};
             if (f < it.width) {
@@ -639,7 +630,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_wide_kernel(const _
             }
             // ── the item's sums ──
             if (any) wait(&sh.pv_done[last & 1], (last >> 1) & 1);
-            const int item_at = pos - cur.step;
+            const int item_at = cur.at - cur.step;
             const bool here = item_at >= begin && item_at + cur.steps <= end;
             const bool both = C::kSets == 2 && !pair;
             float mine = 1.f;
