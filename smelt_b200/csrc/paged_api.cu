@@ -69,7 +69,10 @@ size_t attention_plan(const smelt_cuda_ctx* ctx, const smelt_paged_cache* k, con
     const int64_t most = 2048 / D;
     const bool own_wide = can && own > most, prefix_wide = can && prefix > most;
     a->lines = 0;
+    a->prefix_line = a->own_line = -1;
     auto add = [&](bool wide, bool with_own, bool with_prefix) {
+        if (with_prefix) a->prefix_line = a->lines;
+        if (with_own) a->own_line = a->lines;
         PagedLine& line = a->line[a->lines++];
         line.wide = wide;
         line.with_own = with_own;
@@ -88,6 +91,7 @@ size_t attention_plan(const smelt_cuda_ctx* ctx, const smelt_paged_cache* k, con
     };
     if (prefix == 0) {
         add(own_wide, true, false);
+        if (!own_wide) a->counters = ctx->paged_counters;  // few sums: the kernel joins them itself
     } else if (own_wide == prefix_wide) {
         add(own_wide, true, true);
     } else {
@@ -207,7 +211,7 @@ smelt_status smelt_cuda_paged_attention(smelt_cuda_ctx* ctx, const smelt_paged_c
     a.window = window < 0x7fffffffu ? window : 0;  // positions are below that
     cudaError_t e = cudaSuccess;
     for (int i = 0; i < a.lines && e == cudaSuccess; ++i) e = (a.line[i].wide ? launch_paged_wide : launch_paged_narrow)(l, (PagedType)cache->precision, cache->head_dim, a, i);
-    if (e == cudaSuccess) e = launch_paged_merge(l, (PagedType)cache->precision, cache->head_dim, a);
+    if (e == cudaSuccess && !a.counters) e = launch_paged_merge(l, (PagedType)cache->precision, cache->head_dim, a);
     return check_cuda(ctx, e, "paged attention");
 }
 

@@ -13,7 +13,7 @@
 // CTA joins what its warps have of the same item.
 // P goes into the product as two 16-bit parts: the kernel waits for memory, and rounding P once would cost up to half a step of the
 // 16-bit type.  Keys outside an item are not read (zeros), and a value row that is not finite reaches only the columns that see it.
-// paged_merge_kernel joins the items that several CTAs share, and the prefix with the sequences.
+// What several CTAs have of an item the last of them joins; with a prefix or the tensor-core kernel in the call paged_merge_kernel does.
 #include "attention.cuh"
 #include "paged_line.cuh"
 
@@ -94,6 +94,84 @@ __device__ __noinline__ void weighted_sum_masked(uint32_t values, MaskedTile<D, 
         }
 }
 
+template <int D> struct Sums { float v[D / 32]; };
+template <int D> __device__ __forceinline__ Sums<D> load_part(const float* at, int lane) {  // a lane's values lie side by side
+    Sums<D> s;
+    if constexpr (D == 64) {
+        const float2 x = __ldcg(reinterpret_cast<const float2*>(at) + lane);
+        s.v[0] = x.x; s.v[1] = x.y;
+    } else {
+#pragma unroll
+        for (int i = 0; i < D / 128; ++i) {
+            const float4 x = __ldcg(reinterpret_cast<const float4*>(at) + lane * (D / 128) + i);
+            s.v[4 * i] = x.x; s.v[4 * i + 1] = x.y; s.v[4 * i + 2] = x.z; s.v[4 * i + 3] = x.w;
+        }
+    }
+    return s;
+}
+// A column's parts of an item, in the order of the line: where their sums and their maxima and sums of weights lie.
+struct PartList {
+    int n;
+    const float *first, *others;  // part 0, part 1; the rest `stride` columns apart
+    const float2 *first_ml, *others_ml;
+    int stride;
+    template <int D> __device__ __forceinline__ const float* at(int k) const { return k == 0 ? first : others + (size_t)(k - 1) * stride * D; }
+    __device__ __forceinline__ const float2* ml(int k) const { return k == 0 ? first_ml : others_ml + (size_t)(k - 1) * stride; }
+};
+template <int D>
+__device__ __forceinline__ PartList shared_parts(const PagedLine& line, const Share& share, int at, int first, int last, int col) {
+    const size_t slot0 = (size_t)(2 * first + (at < share.cta_begin(first) ? 0 : 1)) * line.columns + col, slot1 = (size_t)(2 * (first + 1)) * line.columns + col;
+    return {last - first + 1, line.slot_o + slot0 * D, line.slot_o + slot1 * D, line.slot_ml + slot0, line.slot_ml + slot1, 2 * line.columns};
+}
+// One warp: the parts of two lists added up and written to a row of outputs.  A lane fetches a part's maximum and sum; then the parts' sums
+// are added with their factors, eight on their way at a time.
+template <int D, class E>
+__device__ __forceinline__ void join_parts(const PartList& a, const PartList& b, E* out) {
+    const int lane = threadIdx.x & 31, parts = a.n + b.n;
+    float top = kLowest, l = 0.f, o[D / 32];
+#pragma unroll
+    for (int k = 0; k < D / 32; ++k) o[k] = 0.f;
+#pragma unroll 1
+    for (int base = 0; base < parts; base += 32) {
+        const int k = base + lane;
+        float2 ml = make_float2(kLowest, 0.f);
+        if (k < parts) ml = __ldcg(k < a.n ? a.ml(k) : b.ml(k - a.n));
+        const bool counts = ml.y != 0.f;  // a part that the row sees nothing of adds nothing, whatever its sums are
+        const float m = fmaxf(top, warp_max(counts ? ml.x : kLowest)), mine = exp2_approx(top - m), factor = counts ? exp2_approx(ml.x - m) : 0.f;
+        top = m;
+        l = l * mine + warp_sum(counts ? ml.y * factor : 0.f);
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) o[i] *= mine;
+        const uint32_t used = __ballot_sync(0xffffffffu, counts);
+        const int n = min(32, parts - base);
+#pragma unroll 1
+        for (int p = 0; p < n; p += 8) {
+            Sums<D> v[8];
+#pragma unroll
+            for (int y = 0; y < 8; ++y) {
+                const int q = base + p + y;
+                if (p + y < n && (used >> (p + y) & 1u)) v[y] = load_part<D>(q < a.n ? a.at<D>(q) : b.at<D>(q - a.n), lane);
+            }
+#pragma unroll
+            for (int y = 0; y < 8; ++y) {
+                const float w = __shfl_sync(0xffffffffu, factor, (p + y) & 31);
+                if (p + y < n && (used >> (p + y) & 1u)) {
+#pragma unroll
+                    for (int i = 0; i < D / 32; ++i) o[i] += v[y].v[i] * w;
+                }
+            }
+        }
+    }
+    const float rate = l > 0.f ? 1.f / l : l;  // l = 0: nothing was seen; NaN: what was seen is not a number
+    uint32_t w[D / 64];
+#pragma unroll
+    for (int k = 0; k < D / 64; ++k) w[k] = l == 0.f ? 0u : TileElem<E>::pack(o[2 * k] * rate, o[2 * k + 1] * rate);
+    out += lane * (D / 32);
+    if constexpr (D == 64) *reinterpret_cast<uint32_t*>(out) = w[0];
+    else if constexpr (D == 128) *reinterpret_cast<uint2*>(out) = make_uint2(w[0], w[1]);
+    else *reinterpret_cast<uint4*>(out) = make_uint4(w[0], w[1], w[2], w[3]);
+}
+
 template <int D, int NH, class E>
 __global__ void __launch_bounds__(kWarps<D> * 32, 1) paged_narrow_kernel(const __grid_constant__ PagedAttentionArgs a, const int which) {
     constexpr int W = kWarps<D>, THREADS = W * 32, NU = kUnits<D, NH>, UNIT = kUnitBytes<D>, PITCH = kPitch<D>, MT = D / 16, C = NH * 8;
@@ -113,6 +191,19 @@ __global__ void __launch_bounds__(kWarps<D> * 32, 1) paged_narrow_kernel(const _
     Batch batch;
     scan_line<THREADS>(c, line, a.window, batch, reinterpret_cast<unsigned char*>(parts + W * 2));
     const Share share(batch.cum[c.n_seqs + 1], line);
+    if (a.counters)  // no join comes behind: blocks that see nothing get their zeros here
+        for (int s = blockIdx.x * W + warp; s < c.n_seqs; s += gridDim.x * W) {
+            const Seq seq = batch.seq(s);
+            for (int b = 0, n = blocks_of(c, line, seq.n); b < n; ++b) {
+                if (steps_of(block_keys(c, line, seq, b, a.window), line.keys)) continue;
+                for (int f = b * line.columns; f < min((b + 1) * line.columns, seq.n * c.ratio); ++f) {
+                    const int i = divide(f, c.ratio_div);
+                    for (int h = 0; h < c.n_kv; ++h)
+                        for (int d = 2 * lane; d < D; d += 64)
+                            *reinterpret_cast<uint32_t*>(static_cast<E*>(a.out) + (size_t)(seq.row + i) * a.out_stride + (size_t)(h * c.ratio + f - i * c.ratio) * D + d) = 0u;
+                }
+            }
+        }
     if ((int)blockIdx.x * W >= share.used) return;
     const int begin = share.begin(blockIdx.x * W + warp), end = share.begin(blockIdx.x * W + warp + 1);
     if (lane < 2) parts[warp * 2 + lane].valid = 0;
@@ -453,6 +544,7 @@ __global__ void __launch_bounds__(kWarps<D> * 32, 1) paged_narrow_kernel(const _
     const uint32_t valid = __ballot_sync(0xffffffffu, mine), ahead_of_me = valid & ((1u << lane) - 1u);
     const int at_before = __shfl_sync(0xffffffffu, at_mine, ahead_of_me ? 31 - __clz(ahead_of_me) : 0);
     int turn = 0;
+    Part edge[2] = {{0, 0, 0, 0, 0, 0}, {0, 0, 0, 0, 0, 0}};  // the items that this CTA shares with those in front and behind
     for (uint32_t first = __ballot_sync(0xffffffffu, mine && (!ahead_of_me || at_before != at_mine)); first; first &= first - 1u) {  // the first part of each item
         const int p0 = __ffs(first) - 1, p1 = first & (first - 1u) ? __ffs(first & (first - 1u)) - 1 : 32;
         const uint32_t members = valid & ~((1u << p0) - 1u) & (p1 < 32 ? (1u << p1) - 1u : 0xffffffffu);
@@ -460,6 +552,8 @@ __global__ void __launch_bounds__(kWarps<D> * 32, 1) paged_narrow_kernel(const _
         const Seq seq = part.source == 0 ? Seq{0, batch.row[c.n_seqs], 0} : batch.seq(part.source - 1);
         const int f0 = part.block * line.columns, width = min(line.columns, seq.n * c.ratio - f0);
         const bool here = part.at >= cta_begin && part.at + part.steps <= cta_end;
+        if (part.at < cta_begin) edge[0] = part;
+        else if (!here) edge[1] = part;
         for (int f = 0; f < width; ++f) {
             if ((turn++ & (W - 1)) != warp) continue;
             const float2 ml = members >> lane & 1u ? state[lane * C + f] : make_float2(kLowest, 0.f);
@@ -493,118 +587,84 @@ __global__ void __launch_bounds__(kWarps<D> * 32, 1) paged_narrow_kernel(const _
             }
         }
     }
+    if (!a.counters || !(edge[0].valid || edge[1].valid)) return;
+    // ── the last CTA of a shared item joins its parts; the item is counted at the CTA that it begins in ──
+    __shared__ int join[2];
+    __threadfence();
+    __syncthreads();
+    if (tid == 0) {
+#pragma unroll
+        for (int side = 0; side < 2; ++side) {
+            join[side] = 0;
+            if (!edge[side].valid) continue;
+            const int first = share.cta_of(edge[side].at), last = share.cta_of(edge[side].at + edge[side].steps - 1);
+            if (atomicAdd(a.counters + first, 1) == last - first) {
+                a.counters[first] = 0;
+                join[side] = 1;
+            }
+        }
+    }
+    __syncthreads();
+    __threadfence();
+#pragma unroll 1
+    for (int side = 0; side < 2; ++side) {
+        if (!join[side]) continue;
+        const Part part = side ? edge[1] : edge[0];
+        const Seq seq = batch.seq(part.source - 1);
+        const int f0 = part.block * line.columns, width = min(line.columns, seq.n * c.ratio - f0), first = share.cta_of(part.at), last = share.cta_of(part.at + part.steps - 1);
+        for (int f = warp; f < width; f += W) {
+            const int i = divide(f0 + f, c.ratio_div);
+            join_parts<D, E>(shared_parts<D>(line, share, part.at, first, last, f), {0, nullptr, nullptr, nullptr, nullptr, 0},
+                             static_cast<E*>(a.out) + (size_t)(seq.row + i) * a.out_stride + (size_t)(part.head * c.ratio + f0 + f - i * c.ratio) * D);
+        }
+    }
 }
 
 // ── the join ────────────────────────────────────────────────────────────────
-// A warp a row and query head: the parts of its item of the sequence and of its item of the prefix, in the order of the line.  A lane
-// fetches a part's maximum and sum; then the parts' sums are added with their factors, eight on their way at a time.
+// A warp a row and query head: the parts of its item of the prefix and of its item of the sequence.
 constexpr int kMergeWarps = 4;
-
-template <int D> struct Sums { float v[D / 32]; };
-template <int D> __device__ __forceinline__ Sums<D> load_part(const float* at, int lane) {  // a lane's values lie side by side
-    Sums<D> s;
-    if constexpr (D == 64) {
-        const float2 x = __ldcg(reinterpret_cast<const float2*>(at) + lane);
-        s.v[0] = x.x; s.v[1] = x.y;
-    } else {
-#pragma unroll
-        for (int i = 0; i < D / 128; ++i) {
-            const float4 x = __ldcg(reinterpret_cast<const float4*>(at) + lane * (D / 128) + i);
-            s.v[4 * i] = x.x; s.v[4 * i + 1] = x.y; s.v[4 * i + 2] = x.z; s.v[4 * i + 3] = x.w;
-        }
-    }
-    return s;
-}
 
 template <int D, class E>
 __global__ void __launch_bounds__(kMergeWarps * 32) paged_merge_kernel(const __grid_constant__ PagedAttentionArgs a) {
     const PagedArgs& c = a.c;
     const int lane = threadIdx.x & 31;
     const int id = blockIdx.x * kMergeWarps + (threadIdx.x >> 5), r = id / c.n_q, h = id - r * c.n_q, head = divide(h, c.ratio_div);
+    const PagedLine &own = a.line[a.own_line], &ahead = a.line[max(a.prefix_line, 0)];
     pdl_trigger();
     pdl_wait();
+    const int own_places = own.cum[c.n_seqs + 1], ahead_places = ahead.cum[c.n_seqs + 1], ahead_lo = ahead.cum[c.n_seqs + 2];  // (on their way while the sequence is looked for)
     if (r >= c.rows || r >= first_row(c, c.n_seqs)) return;
     int start = 0;
     const int s = warp_find_seq(c.row_start, c.n_seqs, c.rows, r, &start);
     if (s < 0) return;
+    const int own_at = own.cum[s + 1];
     const Seq seq = {start, max(first_row(c, s + 1) - start, 0), tokens_of(c, s)};
     const int i = r - start;
     if (i >= seq.n) return;
-    float top = kLowest, l = 0.f, o[D / 32];
-#pragma unroll
-    for (int k = 0; k < D / 32; ++k) o[k] = 0.f;
-#pragma unroll 1
-    for (int x = 0; x < a.lines; ++x) {
-        const PagedLine& line = a.line[x];
-        const Share share(line.cum[c.n_seqs + 1], line);
-#pragma unroll 1
-        for (int prefix = line.with_prefix ? 1 : 0; prefix >= (line.with_own ? 0 : 1); --prefix) {
-            // the item of this row and head: its first step on the line, and its steps
-            const int f = (prefix ? r : i) * c.ratio + h - head * c.ratio, block = divide(f, line.column_div), col = f - block * line.columns;
-            int at = prefix ? 0 : line.cum[s + 1], steps;
-            if (prefix) {
-                steps = steps_of({line.cum[c.n_seqs + 2], c.prefix_length}, line.keys);
-                at += block * c.n_kv * places_of(line, steps);
-            } else {
-                int before = 0;
-                for (int b = lane; b < block; b += 32) before += c.n_kv * places_of(line, steps_of(block_keys(c, line, seq, b, a.window), line.keys));
-                if (block) {
-#pragma unroll
-                    for (int k = 16; k > 0; k >>= 1) before += __shfl_xor_sync(0xffffffffu, before, k);
-                }
-                at += before;
-                steps = steps_of(block_keys(c, line, seq, block, a.window), line.keys);
-            }
-            if (steps == 0) continue;
-            at += head * places_of(line, steps) + line.extra;
-            const int first = share.cta_of(at), last = share.cta_of(at + steps - 1);
-            const bool whole = first == last;
-            if (whole && !a.whole_o) return;  // written by the CTA that finished it
-            const size_t whole_at = ((prefix ? (size_t)c.rows : 0) + r) * c.n_q + h;
-            const int parts = last - first + 1;
-            const float* part0 = whole ? a.whole_o + whole_at * D : line.slot_o + ((size_t)(2 * first + (at < share.cta_begin(first) ? 0 : 1)) * line.columns + col) * D;
-            // every part but the first begins in front of its CTA's stretch: slot 0
-            const float* part1 = line.slot_o + ((size_t)(2 * (first + 1)) * line.columns + col) * D;
-            const size_t stride = (size_t)2 * line.columns * D;
-#pragma unroll 1
-            for (int base = 0; base < parts; base += 32) {
-                const int k = base + lane;
-                float2 ml = make_float2(kLowest, 0.f);
-                if (k < parts) ml = whole ? __ldcg(a.whole_ml + whole_at) : __ldcg(line.slot_ml + (size_t)(2 * (first + k) + (k == 0 && at >= share.cta_begin(first) ? 1 : 0)) * line.columns + col);
-                const bool counts = ml.y != 0.f;  // a part that the row sees nothing of adds nothing, whatever its sums are
-                const float here = counts ? ml.x : kLowest, m = fmaxf(top, warp_max(here)), mine = exp2_approx(top - m), factor = counts ? exp2_approx(here - m) : 0.f;
-                top = m;
-                l = l * mine + warp_sum(counts ? ml.y * factor : 0.f);
-#pragma unroll
-                for (int k2 = 0; k2 < D / 32; ++k2) o[k2] *= mine;
-                const uint32_t used = __ballot_sync(0xffffffffu, counts);
-                const int n = min(32, parts - base);
-#pragma unroll 1
-                for (int p = 0; p < n; p += 8) {
-                    Sums<D> v[8];
-#pragma unroll
-                    for (int y = 0; y < 8; ++y)
-                        if (p + y < n && (used >> (p + y) & 1u)) v[y] = load_part<D>(base + p + y == 0 ? part0 : part1 + (size_t)(base + p + y - 1) * stride, lane);
-#pragma unroll
-                    for (int y = 0; y < 8; ++y) {
-                        const float w = __shfl_sync(0xffffffffu, factor, (p + y) & 31);
-                        if (p + y < n && (used >> (p + y) & 1u)) {
-#pragma unroll
-                            for (int k2 = 0; k2 < D / 32; ++k2) o[k2] += v[y].v[k2] * w;
-                        }
-                    }
-                }
-            }
-        }
+    // the parts of the item of this row and head that begins at place `at`
+    auto parts_of = [&](const PagedLine& line, int places, bool prefix, int at, int steps, int col) -> PartList {
+        if (steps == 0) return {0, nullptr, nullptr, nullptr, nullptr, 0};
+        const Share share(places, line);
+        const int first = share.cta_of(at), last = share.cta_of(at + steps - 1);
+        if (first != last) return shared_parts<D>(line, share, at, first, last, col);
+        const size_t to = ((prefix ? (size_t)c.rows : 0) + r) * c.n_q + h;
+        return {a.whole_o ? 1 : -1, a.whole_o + to * D, nullptr, a.whole_ml + to, nullptr, 0};  // -1: written by the CTA that finished it
+    };
+    PartList prefix = {0, nullptr, nullptr, nullptr, nullptr, 0};
+    if (a.prefix_line >= 0) {
+        const int f = r * c.ratio + h - head * c.ratio, block = divide(f, ahead.column_div), steps = steps_of({ahead_lo, c.prefix_length}, ahead.keys);
+        prefix = parts_of(ahead, ahead_places, true, (block * c.n_kv + head) * places_of(ahead, steps) + ahead.extra, steps, f - block * ahead.columns);
     }
-    const float rate = l > 0.f ? 1.f / l : l;  // l = 0: nothing was seen; NaN: what was seen is not a number
-    uint32_t w[D / 64];
+    const int f = i * c.ratio + h - head * c.ratio, block = divide(f, own.column_div), steps = steps_of(block_keys(c, own, seq, block, a.window), own.keys);
+    int before = 0;
+    if (block) {
+        for (int b = lane; b < block; b += 32) before += c.n_kv * places_of(own, steps_of(block_keys(c, own, seq, b, a.window), own.keys));
 #pragma unroll
-    for (int k = 0; k < D / 64; ++k) w[k] = l == 0.f ? 0u : TileElem<E>::pack(o[2 * k] * rate, o[2 * k + 1] * rate);
-    E* out = static_cast<E*>(a.out) + (size_t)r * a.out_stride + (size_t)h * D + lane * (D / 32);
-    if constexpr (D == 64) *reinterpret_cast<uint32_t*>(out) = w[0];
-    else if constexpr (D == 128) *reinterpret_cast<uint2*>(out) = make_uint2(w[0], w[1]);
-    else *reinterpret_cast<uint4*>(out) = make_uint4(w[0], w[1], w[2], w[3]);
+        for (int k = 16; k > 0; k >>= 1) before += __shfl_xor_sync(0xffffffffu, before, k);
+    }
+    const PartList mine = parts_of(own, own_places, false, own_at + before + head * places_of(own, steps) + own.extra, steps, f - block * own.columns);
+    if (mine.n < 0) return;
+    join_parts<D, E>(prefix, mine, static_cast<E*>(a.out) + (size_t)r * a.out_stride + (size_t)h * D);
 }
 
 template <class Kernel, class... Args>

@@ -139,6 +139,8 @@ smelt_status smelt_cuda_create(int device_ordinal, smelt_cuda_ctx** out_ctx) {
     ok = ok && cudaMemset(ctx->qmm_counters, 0, 4096 * sizeof(int)) == cudaSuccess;
     ok = ok && cudaMalloc(&ctx->attn_counters, 4096 * sizeof(int)) == cudaSuccess;
     ok = ok && cudaMemset(ctx->attn_counters, 0, 4096 * sizeof(int)) == cudaSuccess;
+    ok = ok && cudaMalloc(&ctx->paged_counters, ctx->sm_count * sizeof(int)) == cudaSuccess;
+    ok = ok && cudaMemset(ctx->paged_counters, 0, ctx->sm_count * sizeof(int)) == cudaSuccess;
     ctx->argmax_scratch_bytes = 64 * 1024 * sizeof(uint64_t);
     ok = ok && cudaMalloc(&ctx->argmax_scratch, ctx->argmax_scratch_bytes) == cudaSuccess;
     ok = ok && cudaEventCreate(&ctx->ev_start) == cudaSuccess && cudaEventCreate(&ctx->ev_stop) == cudaSuccess;
@@ -167,6 +169,7 @@ void smelt_cuda_destroy(smelt_cuda_ctx* ctx) {
     cudaFree(ctx->err_dev);
     cudaFree(ctx->attn_scratch);
     cudaFree(ctx->attn_counters);
+    cudaFree(ctx->paged_counters);
     cudaFree(ctx->qmm_scratch);
     if (ctx->prefill_scratch) cudaFree(ctx->prefill_scratch);
     cudaFree(ctx->qmm_counters);

@@ -151,6 +151,7 @@ struct smelt_cuda_ctx {
     size_t prefill_scratch_bytes = 0;
     int* qmm_counters = nullptr;   // ... and their arrival counters (4096), zero between launches
     int* attn_counters = nullptr;  // one zeroed int per (sequence, KV head): in-kernel merge of attention splits
+    int* paged_counters = nullptr; // one zeroed int per SM: CTAs that have written their part of a shared item (paged_attention.cu)
     uint64_t* argmax_scratch = nullptr;
     size_t argmax_scratch_bytes = 0;
 
