@@ -62,12 +62,14 @@ size_t attention_plan(const smelt_cuda_ctx* ctx, const smelt_paged_cache* k, con
         at += (bytes + 15) & ~(size_t)15;
         return p;
     };
-    // Columns of a source: up to 2048 / head_dim on the streaming kernel, more on the tensor core.  A launch takes sequences and
-    // prefix together where they go to the same kernel.
+    // Columns of a source: up to 16 on the streaming kernel (8 with heads of 256), more on the tensor core.  us with 16 | 32 columns, 16 sequences of
+    // 2000 tokens and 8 key heads of 128: streaming 43 | 67, tensor core 61 | 63; heads of 64: 34 | 49 and 41 | 44; heads of 256 and 8 | 16
+    // columns: 70 | 122 and 78 | 79.  A launch takes sequences and prefix together where they go to the same kernel, and a prefix that is no
+    // more than four tiles a warp (about as many us) goes with the sequences rather than into a launch of 15 us of its own.
     const int64_t own = (int64_t)(b->max_rows > 0 ? b->max_rows : 1) * a->c.ratio, prefix = b->prefix_length > 0 ? (int64_t)b->rows * a->c.ratio : 0;
     const bool can = paged_wide_takes(D, b->n_seqs);
-    const int64_t most = 2048 / D;
-    const bool own_wide = can && own > most, prefix_wide = can && prefix > most;
+    const int64_t most = D == 256 ? 8 : 16, prefix_tiles = (prefix + most - 1) / most * k->n_kv * ((b->prefix_length >> paged_narrow_keys()) + 2);
+    const bool own_wide = can && own > most, prefix_wide = can && prefix > most && (own_wide || prefix_tiles > (int64_t)4 * ctx->sm_count * paged_narrow_workers(D));
     a->lines = 0;
     a->prefix_line = a->own_line = -1;
     auto add = [&](bool wide, bool with_own, bool with_prefix) {

@@ -26,7 +26,7 @@ using attn::TileElem;
 
 template <int D> constexpr int kWarps = D == 256 ? 4 : 8;
 constexpr int kGroups = 2, kTile = 16 * kGroups;  // of 16 keys a tile: a chain of products, exchange and exponentials takes two as fast as one
-template <int D, int NH> constexpr int kUnits = D == 64 ? (NH == 1 ? 10 : NH == 2 ? 8 : 6) : D == 128 ? (NH == 1 ? 5 : 4) : 5;  // of a warp's ring: the K or V rows of 16 keys each
+template <int D, int NH> constexpr int kUnits = D == 64 ? (NH == 1 ? 10 : 8) : D == 128 ? (NH == 1 ? 5 : 4) : 5;  // of a warp's ring: the K or V rows of 16 keys each
 template <int D> constexpr int kPitch = D * 2 + 16;
 template <int D> constexpr int kUnitBytes = 16 * kPitch<D>;
 
@@ -694,13 +694,13 @@ cudaError_t narrow(const Launch& l, PagedType type, const PagedAttentionArgs& a,
 
 }  // namespace
 
-int paged_narrow_columns(int head_dim, int64_t columns) { return columns <= 8 || head_dim == 256 ? 8 : columns <= 16 || head_dim == 128 ? 16 : 32; }
+int paged_narrow_columns(int head_dim, int64_t columns) { return columns <= 8 || head_dim == 256 ? 8 : 16; }
 int paged_narrow_keys() { return 5; }
 int paged_narrow_workers(int head_dim) { return head_dim == 256 ? kWarps<256> : kWarps<128>; }
 
 cudaError_t launch_paged_narrow(const Launch& l, PagedType type, int head_dim, const PagedAttentionArgs& a, int line) {
     const int groups = a.line[line].columns / 8;
-    if (head_dim == 64) return groups == 1 ? narrow<64, 1>(l, type, a, line) : groups == 2 ? narrow<64, 2>(l, type, a, line) : narrow<64, 4>(l, type, a, line);
+    if (head_dim == 64) return groups == 1 ? narrow<64, 1>(l, type, a, line) : narrow<64, 2>(l, type, a, line);
     if (head_dim == 128) return groups == 1 ? narrow<128, 1>(l, type, a, line) : narrow<128, 2>(l, type, a, line);
     return narrow<256, 1>(l, type, a, line);
 }

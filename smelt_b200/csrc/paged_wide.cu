@@ -117,6 +117,8 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
     return v;
 }
+// The lowest n bits.
+__device__ __forceinline__ uint32_t below(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; }
 // The loads behind v have arrived (v is named so that nothing is read of it earlier).
 __device__ __forceinline__ void tmem_wait_ld32(uint32_t (&v)[32]) {
     asm volatile("tcgen05.wait::ld.sync.aligned;"
@@ -498,8 +500,12 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_wide_kernel(const _
             float top = kLowest;
             if constexpr (!decltype(all)::value) {  // keys that the column does not see
 #pragma unroll
-                for (int e = 0; e < KEYS; ++e)
-                    if (k0 + e < keys.lo || k0 + e >= keys.hi) v[e] = 0xFF800000u;
+                for (int x = 0; x < KEYS; x += 32) {
+                    const uint32_t seen = below(keys.hi - k0 - x) & ~below(keys.lo - k0 - x);
+#pragma unroll
+                    for (int e = 0; e < 32; ++e)
+                        if (!(seen >> e & 1u)) v[x + e] = 0xFF800000u;
+                }
             }
             {
                 float most[4] = {kLowest, kLowest, kLowest, kLowest};
