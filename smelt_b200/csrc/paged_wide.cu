@@ -253,6 +253,12 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_wide_kernel(const _
             __syncwarp();
             if (lane == 0) mbar_arrive(bar);
         };
+        // Lanes of a tile behind its columns: no box writes their rows, and scores of what lies there by chance would look like new maxima.
+        for (int i = 0; i < C::kSets; ++i)
+            for (int f = tile_columns + r_first; f < 128; f += ROWS)
+                for (int k = ch; k < CHUNKS; k += LANES) *reinterpret_cast<uint4*>(q_tiles + i * C::kQTile + place(128, f, k)) = make_uint4(0, 0, 0, 0);
+        fence_async_smem();
+        barrier(1, 128);  // the queries' barrier is passed on by one thread
         uint32_t items = 0;
         int v_behind = -1;        // stage of the values that were asked for last and not handed over yet
         bool v_check = false;     // ... that not every column sees all of
@@ -497,7 +503,6 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_wide_kernel(const _
             if (negative)
 #pragma unroll
                 for (int e = 0; e < KEYS; ++e) v[e] ^= 0x80000000u;
-            float top = kLowest;
             if constexpr (!decltype(all)::value) {  // keys that the column does not see
 #pragma unroll
                 for (int x = 0; x < KEYS; x += 32) {
@@ -507,19 +512,46 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_wide_kernel(const _
                         if (!(seen >> e & 1u)) v[x + e] = 0xFF800000u;
                 }
             }
-            {
+            auto largest = [&] {
                 float most[4] = {kLowest, kLowest, kLowest, kLowest};
 #pragma unroll
                 for (int e = 0; e < KEYS; e += 8)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) most[i] = fmaxf(most[i], fmaxf(__uint_as_float(v[e + 2 * i]), __uint_as_float(v[e + 2 * i + 1])));
-                top = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
-            }
-            top = top == kLowest ? kLowest : top * scale2;
-            const bool move = top > m + 8.f || !begun;
-            if (!begun) {
-                m = top;
-            } else if (__any_sync(0xffffffffu, move)) {
+                const float top = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
+                return top == kLowest ? kLowest : top * scale2;
+            };
+            if (!begun) m = largest();
+            // Behind an item's first task the weights are relative to the maximum so far: the new one is only looked at afterwards, and where it is
+            // past the old by 2^8 the task is done again.
+            float added, over;
+            auto exponentials = [&] {
+                const uint64_t scales = pair_of(scale2, scale2), minus = pair_of(-m, -m);
+                uint64_t sums[2] = {0ull, 0ull};
+                float most[2] = {kLowest, kLowest};
+#pragma unroll
+                for (int x = 0; x < KEYS; x += 32) {
+                    uint32_t p[16];
+#pragma unroll
+                    for (int e = 0; e < 32; e += 2) {
+                        float y0, y1;
+                        split(fma2(pair_of(__uint_as_float(v[x + e]), __uint_as_float(v[x + e + 1])), scales, minus), y0, y1);
+                        most[e >> 1 & 1] = fmaxf(most[e >> 1 & 1], fmaxf(y0, y1));
+                        const float p0 = exp2_approx(y0), p1 = exp2_approx(y1);
+                        sums[e >> 1 & 1] = add2(sums[e >> 1 & 1], pair_of(p0, p1));
+                        p[e / 2] = Pack<E>::two(p0, p1);
+                    }
+                    tmem_st16(s_at + x / 2, p);
+                }
+                float l0, l1;
+                split(add2(sums[0], sums[1]), l0, l1);
+                added = l0 + l1;
+                over = fmaxf(most[0], most[1]);
+            };
+            exponentials();
+            if (begun && __any_sync(0xffffffffu, over > 8.f)) {
+                const float top = largest();
+                const bool move = top > m + 8.f;
                 const float keep = move ? exp2_approx(m - top) : 1.f;
                 if (move) m = top;
                 l *= keep;
@@ -527,35 +559,17 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_wide_kernel(const _
                 if (alive) {
 #pragma unroll 1
                     for (int x = 0; x < D; x += 16) {
-                        uint32_t v[16];
-                        tmem_ld16(o_at + x, v);
-                        tmem_wait_ld16(v);
+                        uint32_t w[16];
+                        tmem_ld16(o_at + x, w);
+                        tmem_wait_ld16(w);
 #pragma unroll
-                        for (int e = 0; e < 16; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * keep);
-                        tmem_st16(o_at + x, v);
+                        for (int e = 0; e < 16; ++e) w[e] = __float_as_uint(__uint_as_float(w[e]) * keep);
+                        tmem_st16(o_at + x, w);
                     }
                 }
+                exponentials();
             }
-            const uint64_t scales = pair_of(scale2, scale2), minus = pair_of(-m, -m);
-            uint64_t sums[2] = {0ull, 0ull};
-#pragma unroll
-            for (int x = 0; x < KEYS; x += 32) {
-                uint32_t p[16];
-#pragma unroll
-                for (int e = 0; e < 32; e += 2) {
-                    float y0, y1;
-                    split(fma2(pair_of(__uint_as_float(v[x + e]), __uint_as_float(v[x + e + 1])), scales, minus), y0, y1);
-                    const float p0 = exp2_approx(y0), p1 = exp2_approx(y1);
-                    sums[e >> 1 & 1] = add2(sums[e >> 1 & 1], pair_of(p0, p1));
-                    p[e / 2] = Pack<E>::two(p0, p1);
-                }
-                tmem_st16(s_at + x / 2, p);
-            }
-            {
-                float l0, l1;
-                split(add2(sums[0], sums[1]), l0, l1);
-                l += l0 + l1;
-            }
+            l += added;
         };
         each_item([&](const Cursor& cur, const Item& it, bool pair, int n, int tasks, uint32_t task0, uint32_t step0) {
             const int t_first = C::kSets == 1 ? 0 : (int)((task0 & 1) ^ set), f = me < tile_columns ? (pair ? t_first * tile_columns : 0) + me : 256, ff = it.f0 + f;
@@ -626,7 +640,6 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_wide_kernel(const _
                         }
                     }
                     if (t < C::kSets) *(volatile uint32_t*)&sh.keep[b] = keep_sum;
-                    tmem_wait_st();
                     tc_fence_before();
                     any = true;
                     last = T;

@@ -176,6 +176,16 @@ def test_what_a_row_does_not_see_does_not_reach_it(ctx, kind, rows, bad):
     assert not np.isfinite(got[0]).any() and not np.isfinite(got[rows - cut:rows]).any()
 
 
+@pytest.mark.parametrize("dim,n_q", [(64, 5), (128, 5), (128, 14), (256, 7)])
+def test_queries_of_an_earlier_call_do_not_reach_the_next(ctx, dim, n_q):
+    """Groups that do not fill a tile, behind a call whose queries were as large as the type holds."""
+    g = np.random.default_rng(dim)
+    b = cases.Batch(g, [300, 64], [900, 700], 16, 2, dim)
+    k, v, _ = b.fill(g, 0.0)
+    Device(ctx, b, "bf16", 16, k, v).attend(np.full((b.total, 16, dim), 3e38), 1.0)
+    check_attention(ctx, g, "bf16", 2 * n_q, cases.Batch(g, [120, 33], [1500, 800], 16, 2, dim))
+
+
 def test_large_scores_and_small_ones(ctx):
     g = np.random.default_rng(11)
     for scale in (40.0, 1e-6, 0.0, -3.0):
