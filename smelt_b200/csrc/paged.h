@@ -8,6 +8,8 @@ enum PagedType : int { kPagedF16 = 0, kPagedBf16 = 1 };
 enum : uint32_t { KERR_BAD_PAGE = 0x10000u };  // a page id outside the pool, or a row without a token of its own
 constexpr int kPagedSeqs = 1024;               // sequences of one call: their rows and lengths are held in shared memory
 
+constexpr int kPagedCtas = 256;                // of a line's kernel at most: the join has a thread for each
+
 // n / d for 0 <= n < 2^31 as a multiplication: with 2^l >= d > 2^(l-1), n / d = (umulhi(m, n) + n) >> l for m = 2^32 (2^l - d) / d + 1.
 struct Divisor {
     uint32_t mul, shift;
@@ -65,6 +67,7 @@ cudaError_t launch_paged_append(const Launch& l, PagedType type, int head_dim, c
 // shares with others, one at each end.  In front of an item's steps lie `extra` places that stand for what its beginning and end cost; nobody does
 // anything there.  Lengths are read on the device, so that a captured call follows them.  The line is at most 2^30
 // steps (paged_api.cu).
+struct PagedShared { int parts, row, f0, width, head; };  // an item of so many CTAs (0: none): first row of its sequence, first column and how many, key head
 struct PagedLine {
     int columns, keys, extra;  // keys as a power of two
     Divisor column_div;
@@ -73,6 +76,7 @@ struct PagedLine {
     int32_t* cum;     // [n_seqs + 3] written by CTA 0: steps before each source, and the first prefix key that any row sees
     float* slot_o;    // [2 ctas][columns][D] weighted sums of items shared by several CTAs
     float2* slot_ml;  // [2 ctas][columns] their running maxima and sums
+    PagedShared* shared;  // [ctas] the item that begins in a CTA and goes on behind it, for the join (tensor-core kernel without a prefix)
 };
 struct PagedAttentionArgs {
     PagedArgs c;
@@ -96,7 +100,9 @@ int paged_wide_columns(int head_dim, int ratio);
 int paged_wide_keys(int head_dim);
 bool paged_wide_takes(int head_dim, int n_seqs);
 cudaError_t launch_paged_wide(const Launch& l, PagedType type, int head_dim, const PagedAttentionArgs& a, int line);
+// What joins the parts of items: with a prefix every row's (merge), without one the shared items' (join).
 cudaError_t launch_paged_merge(const Launch& l, PagedType type, int head_dim, const PagedAttentionArgs& a);
+cudaError_t launch_paged_join(const Launch& l, PagedType type, int head_dim, const PagedAttentionArgs& a);
 
 // Drafted tokens against the target (verify.cu).
 struct VerifyArgs {

@@ -85,11 +85,12 @@ size_t attention_plan(const smelt_cuda_ctx* ctx, const smelt_paged_cache* k, con
         line.keys = wide ? paged_wide_keys(D) : paged_narrow_keys();
         // What an item costs beside its steps: 8 us of 3 us a step on the tensor core (a masked step, the end), 1 us of 1 us a tile on the streaming kernel.
         line.extra = wide ? 3 : 1;
-        line.ctas = ctx->sm_count;
+        line.ctas = ctx->sm_count < kPagedCtas ? ctx->sm_count : kPagedCtas;
         line.workers = wide ? 1 : paged_narrow_workers(D);
         line.cum = (int32_t*)room((size_t)(b->n_seqs + 3) * sizeof(int32_t));
         line.slot_o = (float*)room((size_t)2 * line.ctas * line.columns * D * sizeof(float));
         line.slot_ml = (float2*)room((size_t)2 * line.ctas * line.columns * sizeof(float2));
+        line.shared = (PagedShared*)room((size_t)line.ctas * sizeof(PagedShared));
     };
     if (prefix == 0) {
         add(own_wide, true, false);
@@ -213,7 +214,7 @@ smelt_status smelt_cuda_paged_attention(smelt_cuda_ctx* ctx, const smelt_paged_c
     a.window = window < 0x7fffffffu ? window : 0;  // positions are below that
     cudaError_t e = cudaSuccess;
     for (int i = 0; i < a.lines && e == cudaSuccess; ++i) e = (a.line[i].wide ? launch_paged_wide : launch_paged_narrow)(l, (PagedType)cache->precision, cache->head_dim, a, i);
-    if (e == cudaSuccess && !a.counters) e = launch_paged_merge(l, (PagedType)cache->precision, cache->head_dim, a);
+    if (e == cudaSuccess && !a.counters) e = (a.whole_o ? launch_paged_merge : launch_paged_join)(l, (PagedType)cache->precision, cache->head_dim, a);
     return check_cuda(ctx, e, "paged attention");
 }
 

@@ -119,9 +119,13 @@ struct PartList {
     __device__ __forceinline__ const float2* ml(int k) const { return k == 0 ? first_ml : others_ml + (size_t)(k - 1) * stride; }
 };
 template <int D>
+__device__ __forceinline__ PartList parts_from(const PagedLine& line, int slot0, int slot1, int n, int col) {
+    const size_t at0 = (size_t)slot0 * line.columns + col, at1 = (size_t)slot1 * line.columns + col;
+    return {n, line.slot_o + at0 * D, line.slot_o + at1 * D, line.slot_ml + at0, line.slot_ml + at1, 2 * line.columns};
+}
+template <int D>
 __device__ __forceinline__ PartList shared_parts(const PagedLine& line, const Share& share, int at, int first, int last, int col) {
-    const size_t slot0 = (size_t)(2 * first + (at < share.cta_begin(first) ? 0 : 1)) * line.columns + col, slot1 = (size_t)(2 * (first + 1)) * line.columns + col;
-    return {last - first + 1, line.slot_o + slot0 * D, line.slot_o + slot1 * D, line.slot_ml + slot0, line.slot_ml + slot1, 2 * line.columns};
+    return parts_from<D>(line, 2 * first + (at < share.cta_begin(first) ? 0 : 1), 2 * (first + 1), last - first + 1, col);
 }
 // One warp: the parts of two lists added up and written to a row of outputs.  A lane fetches a part's maximum and sum; then the parts' sums
 // are added with their factors, eight on their way at a time.
@@ -621,15 +625,17 @@ __global__ void __launch_bounds__(kWarps<D> * 32, 1) paged_narrow_kernel(const _
 }
 
 // ── the join ────────────────────────────────────────────────────────────────
-// A warp a row and query head: the parts of its item of the prefix and of its item of the sequence.
+// With a prefix: a warp some query heads of a row and key head, one or all of them: the parts of each one's item of the prefix and of its
+// item of the sequence.  Looking for the sequence and its blocks costs more than the sums, so many rows have a warp do it once for a group's
+// heads.
 constexpr int kMergeWarps = 4;
 
 template <int D, class E>
-__global__ void __launch_bounds__(kMergeWarps * 32) paged_merge_kernel(const __grid_constant__ PagedAttentionArgs a) {
+__global__ void __launch_bounds__(kMergeWarps * 32) paged_merge_kernel(const __grid_constant__ PagedAttentionArgs a, const int heads) {
     const PagedArgs& c = a.c;
     const int lane = threadIdx.x & 31;
-    const int id = blockIdx.x * kMergeWarps + (threadIdx.x >> 5), r = id / c.n_q, h = id - r * c.n_q, head = divide(h, c.ratio_div);
-    const PagedLine &own = a.line[a.own_line], &ahead = a.line[max(a.prefix_line, 0)];
+    const int id = blockIdx.x * kMergeWarps + (threadIdx.x >> 5), turns = c.n_q / heads, r = id / turns, h0 = (id - r * turns) * heads, head = divide(h0, c.ratio_div);
+    const PagedLine &own = a.line[a.own_line], &ahead = a.line[a.prefix_line];
     pdl_trigger();
     pdl_wait();
     const int own_places = own.cum[c.n_seqs + 1], ahead_places = ahead.cum[c.n_seqs + 1], ahead_lo = ahead.cum[c.n_seqs + 2];  // (on their way while the sequence is looked for)
@@ -641,39 +647,78 @@ __global__ void __launch_bounds__(kMergeWarps * 32) paged_merge_kernel(const __g
     const Seq seq = {start, max(first_row(c, s + 1) - start, 0), tokens_of(c, s)};
     const int i = r - start;
     if (i >= seq.n) return;
-    // the parts of the item of this row and head that begins at place `at`
-    auto parts_of = [&](const PagedLine& line, int places, bool prefix, int at, int steps, int col) -> PartList {
+    // the parts of the item of this row and a head that begins at place `at`
+    auto parts_of = [&](const PagedLine& line, int places, bool prefix, int h, int at, int steps, int col) -> PartList {
         if (steps == 0) return {0, nullptr, nullptr, nullptr, nullptr, 0};
         const Share share(places, line);
         const int first = share.cta_of(at), last = share.cta_of(at + steps - 1);
         if (first != last) return shared_parts<D>(line, share, at, first, last, col);
         const size_t to = ((prefix ? (size_t)c.rows : 0) + r) * c.n_q + h;
-        return {a.whole_o ? 1 : -1, a.whole_o + to * D, nullptr, a.whole_ml + to, nullptr, 0};  // -1: written by the CTA that finished it
+        return {1, a.whole_o + to * D, nullptr, a.whole_ml + to, nullptr, 0};
     };
-    PartList prefix = {0, nullptr, nullptr, nullptr, nullptr, 0};
-    if (a.prefix_line >= 0) {
-        const int f = r * c.ratio + h - head * c.ratio, block = divide(f, ahead.column_div), steps = steps_of({ahead_lo, c.prefix_length}, ahead.keys);
-        prefix = parts_of(ahead, ahead_places, true, (block * c.n_kv + head) * places_of(ahead, steps) + ahead.extra, steps, f - block * ahead.columns);
-    }
-    const int f = i * c.ratio + h - head * c.ratio, block = divide(f, own.column_div), steps = steps_of(block_keys(c, own, seq, block, a.window), own.keys);
-    int before = 0;
-    if (block) {
-        for (int b = lane; b < block; b += 32) before += c.n_kv * places_of(own, steps_of(block_keys(c, own, seq, b, a.window), own.keys));
+    const int ahead_steps = steps_of({ahead_lo, c.prefix_length}, ahead.keys);
+    int known = -1, steps = 0, before = 0;  // of the block that was looked at last
+    for (int h = h0; h < h0 + heads; ++h) {
+        const int g = h - head * c.ratio, f = i * c.ratio + g, block = divide(f, own.column_div);
+        if (block != known) {
+            known = block;
+            steps = steps_of(block_keys(c, own, seq, block, a.window), own.keys);
+            before = 0;
+            if (block) {
+                for (int b = lane; b < block; b += 32) before += c.n_kv * places_of(own, steps_of(block_keys(c, own, seq, b, a.window), own.keys));
 #pragma unroll
-        for (int k = 16; k > 0; k >>= 1) before += __shfl_xor_sync(0xffffffffu, before, k);
+                for (int k = 16; k > 0; k >>= 1) before += __shfl_xor_sync(0xffffffffu, before, k);
+            }
+        }
+        const int af = r * c.ratio + g, ahead_block = divide(af, ahead.column_div);
+        const PartList prefix = parts_of(ahead, ahead_places, true, h, (ahead_block * c.n_kv + head) * places_of(ahead, ahead_steps) + ahead.extra, ahead_steps, af - ahead_block * ahead.columns);
+        const PartList mine = parts_of(own, own_places, false, h, own_at + before + head * places_of(own, steps) + own.extra, steps, f - block * own.columns);
+        join_parts<D, E>(prefix, mine, static_cast<E*>(a.out) + (size_t)r * a.out_stride + (size_t)h * D);
     }
-    const PartList mine = parts_of(own, own_places, false, own_at + before + head * places_of(own, steps) + own.extra, steps, f - block * own.columns);
-    if (mine.n < 0) return;
-    join_parts<D, E>(prefix, mine, static_cast<E*>(a.out) + (size_t)r * a.out_stride + (size_t)h * D);
+}
+
+// Without one, behind the tensor-core kernel: the columns of the items that begin in a CTA of it and go on behind, shared out evenly.
+constexpr int kJoinWarps = 8;
+constexpr int kJoinCtas = 2;  // of an SM, resident together
+
+template <int D, class E>
+__global__ void __launch_bounds__(kJoinWarps * 32, kJoinCtas) paged_join_kernel(const __grid_constant__ PagedAttentionArgs a) {
+    __shared__ PagedShared items[kPagedCtas];
+    __shared__ int owner[kPagedCtas], count[kPagedCtas / 32];
+    static_assert(kPagedCtas == kJoinWarps * 32, "a thread a CTA");
+    const PagedArgs& c = a.c;
+    const PagedLine& line = a.line[0];
+    const int tid = threadIdx.x, warp = tid >> 5;
+    pdl_trigger();
+    pdl_wait();
+    const PagedShared mine = tid < line.ctas ? line.shared[tid] : PagedShared{};
+    const uint32_t some = __ballot_sync(0xffffffffu, mine.parts != 0);
+    count[warp] = __popc(some);
+    __syncthreads();
+    int n = 0, at = __popc(some & ((1u << (tid & 31)) - 1u));
+    for (int w = 0; w < kJoinWarps; ++w) {
+        if (w < warp) at += count[w];
+        n += count[w];
+    }
+    if (mine.parts) { items[at] = mine; owner[at] = tid; }
+    __syncthreads();
+    for (int k = blockIdx.x * kJoinWarps + warp; k < n * line.columns; k += gridDim.x * kJoinWarps) {
+        const int which = divide(k, line.column_div), f = k - which * line.columns, first = owner[which];
+        const PagedShared item = items[which];
+        if (f >= item.width) continue;
+        const int i = divide(item.f0 + f, c.ratio_div);
+        join_parts<D, E>(parts_from<D>(line, 2 * first + 1, 2 * (first + 1), item.parts, f), {0, nullptr, nullptr, nullptr, nullptr, 0},
+                         static_cast<E*>(a.out) + (size_t)(item.row + i) * a.out_stride + (size_t)(item.head * c.ratio + item.f0 + f - i * c.ratio) * D);
+    }
 }
 
 template <class Kernel, class... Args>
-cudaError_t launch(const Launch& l, Kernel kernel, int grid, int threads, size_t shared, Args... args) {
+cudaError_t launch(const Launch& l, Kernel kernel, dim3 grid, int threads, size_t shared, Args... args) {
     cudaError_t e = allow_shared(kernel, shared);
     if (e == cudaSuccess) e = prefer_max_shared(kernel);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(grid);
+    cfg.gridDim = grid;
     cfg.blockDim = dim3(threads);
     cfg.dynamicSmemBytes = shared;
     cfg.stream = l.stream;
@@ -706,11 +751,21 @@ cudaError_t launch_paged_narrow(const Launch& l, PagedType type, int head_dim, c
 }
 
 cudaError_t launch_paged_merge(const Launch& l, PagedType type, int head_dim, const PagedAttentionArgs& a) {
-    const int grid = (a.c.rows * a.c.n_q + kMergeWarps - 1) / kMergeWarps;
-    auto go = [&](auto f16, auto bf16) { return type == kPagedF16 ? launch(l, f16, grid, kMergeWarps * 32, 0, a) : launch(l, bf16, grid, kMergeWarps * 32, 0, a); };
+    const int64_t all = (int64_t)a.c.rows * a.c.n_q;
+    const int heads = all > (int64_t)a.line[0].ctas * 64 ? a.c.ratio : 1;  // 64 warps an SM hold a head each
+    const int grid = (int)((all / heads + kMergeWarps - 1) / kMergeWarps);
+    auto go = [&](auto f16, auto bf16) { return type == kPagedF16 ? launch(l, f16, grid, kMergeWarps * 32, 0, a, heads) : launch(l, bf16, grid, kMergeWarps * 32, 0, a, heads); };
     if (head_dim == 64) return go(paged_merge_kernel<64, __half>, paged_merge_kernel<64, __nv_bfloat16>);
     if (head_dim == 128) return go(paged_merge_kernel<128, __half>, paged_merge_kernel<128, __nv_bfloat16>);
     return go(paged_merge_kernel<256, __half>, paged_merge_kernel<256, __nv_bfloat16>);
+}
+
+cudaError_t launch_paged_join(const Launch& l, PagedType type, int head_dim, const PagedAttentionArgs& a) {
+    const int grid = kJoinCtas * a.line[0].ctas;
+    auto go = [&](auto f16, auto bf16) { return type == kPagedF16 ? launch(l, f16, grid, kJoinWarps * 32, 0, a) : launch(l, bf16, grid, kJoinWarps * 32, 0, a); };
+    if (head_dim == 64) return go(paged_join_kernel<64, __half>, paged_join_kernel<64, __nv_bfloat16>);
+    if (head_dim == 128) return go(paged_join_kernel<128, __half>, paged_join_kernel<128, __nv_bfloat16>);
+    return go(paged_join_kernel<256, __half>, paged_join_kernel<256, __nv_bfloat16>);
 }
 
 }  // namespace smelt

@@ -247,7 +247,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_wide_kernel(const _
         constexpr int LANES = CHUNKS < 32 ? CHUNKS : 32, ROWS = 128 / LANES;  // lanes of a row, rows of a turn of the four warps
         const int ch = lt % LANES, r_first = lt / LANES;
         auto place = [](int rows, int row, int chunk) { return (uint32_t)((chunk >> 3) * rows * 128 + row * 128 + (((chunk & 7) ^ (row & 7)) << 4)); };
-        auto warp_wait = [&](uint64_t* bar, uint32_t parity) { alive = __all_sync(0xffffffffu, alive && wait_alive(bar, parity, dead)) != 0; };
+        auto warp_wait = [&](uint64_t* bar, uint32_t parity) { alive = __all_sync(0xffffffffu, alive && wait_alive_short(smem_u32(bar), parity, smem_u32(&sh.dead))) != 0; };
         auto arrive = [&](uint64_t* bar) {
             fence_async_smem();
             __syncwarp();
@@ -434,13 +434,42 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_wide_kernel(const _
                 mbar_poll_bounded(&sh.k_full[s], use & 1);
                 mbar_poll_bounded(&sh.v_full[s], use & 1);
             }
+    } else if (warp > C::kMmaWarp) {
+        // ── without a prefix no join of all rows comes behind: the item that others finish is named for the join, and blocks that see
+        // nothing, which have no item, get their zeros here ──
+        if (!a.whole_o) {
+            if (warp == C::kMmaWarp + 1) {
+                PagedShared shared = {};
+                each_item([&](const Cursor& cur, const Item& it, bool, int, int, uint32_t, uint32_t) {
+                    const int item_at = cur.at - cur.step;
+                    if (item_at >= begin && item_at + cur.steps > end) shared = {share.cta_of(item_at + cur.steps - 1) - (int)blockIdx.x + 1, it.seq.row, it.f0, it.width, cur.head};
+                });
+                if (lane == 0) line.shared[blockIdx.x] = shared;
+            }
+            for (int s = blockIdx.x * 3 + warp - C::kMmaWarp - 1; s < c.n_seqs; s += gridDim.x * 3) {
+                const Seq seq = batch.seq(s);
+                const int blocks = blocks_of(c, line, seq.n);
+                for (int b0 = 0; b0 < blocks; b0 += 32) {
+                    uint32_t none = __ballot_sync(0xffffffffu, b0 + lane < blocks && steps_of(block_keys(c, line, seq, b0 + lane, a.window), line.keys) == 0);
+                    for (; none; none &= none - 1u) {
+                        const int f0 = (b0 + __ffs(none) - 1) * line.columns, f1 = min(f0 + line.columns, seq.n * c.ratio);
+                        for (int f = f0; f < f1; ++f) {
+                            const int i = divide(f, c.ratio_div);
+                            for (int h = 0; h < c.n_kv; ++h)
+                                for (int x = 2 * lane; x < D; x += 64)
+                                    *reinterpret_cast<uint32_t*>(static_cast<E*>(a.out) + (size_t)(seq.row + i) * a.out_stride + (size_t)(h * c.ratio + f - i * c.ratio) * D + x) = 0u;
+                        }
+                    }
+                }
+            }
+        }
     } else if (warp == C::kMmaWarp) {
         // ── products ──
         constexpr uint32_t kScores = (1u << 4) | Pack<E>::kType | ((uint32_t)(KEYS >> 3) << 17) | ((128u >> 4) << 24);
         constexpr uint32_t kValues = (1u << 4) | Pack<E>::kType | (1u << 16) | ((uint32_t)(D >> 3) << 17) | ((128u >> 4) << 24);
         const uint64_t q_desc = smem_desc_sw128(smem_u32(q_tiles)), k_desc = smem_desc_sw128(smem_u32(k_tiles)), v_desc = value_desc(smem_u32(v_tiles), KEYS * 128);
         auto wait = [&](uint64_t* bar, uint32_t parity) {
-            alive = __all_sync(0xffffffffu, alive && wait_alive(bar, parity, dead)) != 0;
+            alive = __all_sync(0xffffffffu, alive && wait_alive_short(smem_u32(bar), parity, smem_u32(&sh.dead))) != 0;
             tc_fence_after();
         };
         uint32_t items = 0, done = 0;
@@ -492,7 +521,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_wide_kernel(const _
         const float scale2 = fmaxf(fabsf(a.scale2), 1e-30f);  // the maximum wants a positive one, and so does -inf times it
         const bool negative = a.scale2 < 0.f;
         auto wait = [&](uint64_t* bar, uint32_t parity) {
-            alive = __all_sync(0xffffffffu, alive && wait_alive(bar, parity, dead)) != 0;
+            alive = __all_sync(0xffffffffu, alive && wait_alive_short(smem_u32(bar), parity, smem_u32(&sh.dead))) != 0;
             tc_fence_after();
         };
         float m = kLowest, l = 0.f;  // of the column: what its weights are relative to, and their sum
