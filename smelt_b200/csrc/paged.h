@@ -115,7 +115,7 @@ struct VerifyArgs {
     void* stats;  // verify_workspace bytes
 };
 enum LogitsType : int { kLogitsF16 = 0, kLogitsBf16 = 1, kLogitsF32 = 2 };
-size_t verify_workspace(LogitsType type, int rows, int vocab, bool draft);
+size_t verify_workspace(LogitsType type, int n_seqs, int rows, int vocab, bool draft);
 cudaError_t launch_verify(const Launch& l, LogitsType type, const VerifyArgs& a);
 
 }  // namespace smelt

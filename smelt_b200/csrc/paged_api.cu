@@ -223,7 +223,7 @@ smelt_status smelt_cuda_verify_drafts_workspace(smelt_cuda_ctx* ctx, const smelt
     const smelt_status s = verify_args(ctx, args);
     if (s) return s;
     if (!out_bytes) return fail(ctx, SMELT_ERR_BAD_ARGUMENT, "verify drafts: null size");
-    *out_bytes = verify_workspace((LogitsType)args->precision, args->rows, args->vocab, args->draft != nullptr);
+    *out_bytes = verify_workspace((LogitsType)args->precision, args->n_seqs, args->rows, args->vocab, args->draft != nullptr);
     return SMELT_OK;
 }
 
@@ -239,7 +239,7 @@ smelt_status smelt_cuda_verify_drafts(smelt_cuda_ctx* ctx, const smelt_verify_ar
     if ((v->rows > 1 && v->target_stride < v->vocab) || (v->draft && (v->draft_step_stride < 0 || v->draft_seq_stride < 0))) return fail(ctx, SMELT_ERR_BAD_ARGUMENT, "verify drafts: bad strides");
     if (v->out_tokens == v->tokens) return fail(ctx, SMELT_ERR_BAD_ARGUMENT, "verify drafts: the answer needs a place of its own");
     const LogitsType type = (LogitsType)v->precision;
-    if (!v->workspace || !aligned16(v->workspace) || v->workspace_bytes < verify_workspace(type, v->rows, v->vocab, v->draft != nullptr))
+    if (!v->workspace || !aligned16(v->workspace) || v->workspace_bytes < verify_workspace(type, v->n_seqs, v->rows, v->vocab, v->draft != nullptr))
         return fail(ctx, SMELT_ERR_BAD_ARGUMENT, "verify drafts: workspace missing, misaligned or smaller than smelt_cuda_verify_drafts_workspace says");
     VerifyArgs a = {};
     a.n_seqs = v->n_seqs; a.rows = v->rows; a.vocab = v->vocab;

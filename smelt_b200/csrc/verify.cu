@@ -4,13 +4,14 @@
 // not the next token is drawn from max(p - q, 0), behind the last draft from p, as the first index whose running sum passes u times
 // the whole.
 //
-// Two kernels.  verify_stats_kernel reads every row of logits once (the bytes that bound the operator): a CTA takes a stretch of one row
+// verify_stats_kernel reads every row of logits once (the bytes that bound the operator): a CTA takes a stretch of one row
 // and leaves its maximum, the sum of exp((x - max) / T) and the lowest index of the maximum, in fp32 (a chance's
-// error of 1e-7 turns a draw that lies as near to it).  verify_draw_kernel: a cluster of eight CTAs a sequence joins
-// the parts, finds the first draft that falls and reads that one row (of the target, and of the draft) again.  There a running
-// sum over the vocabulary is compared with a number, and every index is a border: probabilities and sums are fp64, and all sums are added in
-// the order of the vocabulary.
-#include <cooperative_groups.h>
+// error of 1e-7 turns a draw that lies as near to it).  Then one row of a sequence is read again, and with a draft's probabilities one
+// of those: there a running sum over the vocabulary is compared with a number, and every index is a border, so probabilities and sums are
+// fp64, and all sums are added in the order of the vocabulary.  A piece of such a row is a CTA's: verify_sums_kernel
+// (with a draft's probabilities) finds the first draft that falls and adds up the weights of p and q, verify_pick_kernel what the next token is
+// drawn by, and its last CTA of a sequence finds the index.  (A cluster of eight CTAs a sequence, which did all of that in one
+// launch, took 45 us for one sequence and 70 for 48 of them, its fp64 pipe busy for an eighth of the time.)
 #include <cuda_bf16.h>
 
 #include "paged.h"
@@ -18,11 +19,19 @@
 namespace smelt {
 namespace {
 
-namespace cg = cooperative_groups;
-
 constexpr int kStatThreads = 256, kStatWords = 4;  // words of 16 bytes a thread has on their way at a time
-constexpr int kCluster = 8, kDrawThreads = 512, kDrawWarps = kDrawThreads / 32;
+constexpr int kDrawCtas = 592, kDrawThreads = 512, kDrawWarps = kDrawThreads / 32;
 constexpr float kNone = -INFINITY;
+
+// What the kernels behind the statistics leave one another: rows that are drawn from are cut into pieces, a CTA each.
+struct Choice;
+struct Draws {
+    int pieces;
+    Choice* choice;   // [n_seqs]
+    int* arrived;     // [n_seqs] CTAs that have written their part of `chances`
+    double* sums;     // [n_seqs][pieces][2] of the weights of p and of q
+    double* chances;  // [n_seqs][pieces][warps]
+};
 
 struct Stat { float top, sum; int index, pad; };  // of a chunk or a row: largest logit, sum of exp((x - top) / T), lowest index of the largest
 
@@ -74,11 +83,9 @@ struct Row {
         const int i0 = index(w);
         if (i0 >= 0 && i0 + N <= vocab) {
             Logit<E>::word(__ldg(reinterpret_cast<const uint4*>(row + i0)), v);
-#pragma unroll
-            for (int i = 0; i < N; ++i) v[i] = known(v[i]);
         } else {
 #pragma unroll
-            for (int i = 0; i < N; ++i) v[i] = i0 + i >= 0 && i0 + i < vocab ? known(Logit<E>::at(row + i0 + i)) : kNone;
+            for (int i = 0; i < N; ++i) v[i] = i0 + i >= 0 && i0 + i < vocab ? Logit<E>::at(row + i0 + i) : kNone;
         }
     }
 };
@@ -130,7 +137,7 @@ __device__ __forceinline__ float exp2_approx(float x) {
 }
 
 template <class E>
-__global__ void __launch_bounds__(kStatThreads) verify_stats_kernel(const VerifyArgs a, const Stretches stretches) {
+__global__ void __launch_bounds__(kStatThreads) verify_stats_kernel(const VerifyArgs a, const Stretches stretches, const Draws draws) {
     constexpr int N = Logit<E>::kPerWord;
     __shared__ Stat warps[kStatThreads / 32];
     const int tid = threadIdx.x, y = blockIdx.x / stretches.count, stretch = blockIdx.x - y * stretches.count;
@@ -138,6 +145,7 @@ __global__ void __launch_bounds__(kStatThreads) verify_stats_kernel(const Verify
     const int r = draft ? y - a.rows : y;
     pdl_trigger();
     pdl_wait();
+    for (int i = blockIdx.x * kStatThreads + tid; i < a.n_seqs; i += gridDim.x * kStatThreads) draws.arrived[i] = 0;
     int start = 0;
     const int s = warp_find_seq(a.row_start, a.n_seqs, a.rows, r, &start);
     if (s < 0) return;
@@ -233,17 +241,17 @@ __global__ void __launch_bounds__(kStatThreads) verify_stats_kernel(const Verify
     }
 }
 
-// exp((x - top) / T) in fp64 to about 1e-13; rate = 1 / T.  With y = (x - top) / T <= 0 and k the whole number next to 256 y / ln 2, it is
-// 2^(k / 256), from a table and an exponent, times exp(z), z = y - k ln 2 / 256, |z| < 0.00136, of which the series' fourth power is below 2e-13.
+// exp((x - top) / T) in fp64 to about 1e-13; rate = 1 / T.  With y = (top - x) / T >= 0 and k the whole number next to -256 y / ln 2, it is
+// 2^(k / 256), from a table and an exponent, times exp(z), z = -y - k ln 2 / 256, |z| < 0.00136, of which the series' fourth power is below 2e-13.
 constexpr int kTable = 256;
 __device__ __forceinline__ double weight(float x, float top, double rate, const double* table) {
-    if (top == INFINITY) return x == top ? 1.0 : 0.0;
     constexpr double kRound = 6755399441055744.0;  // 1.5 2^52: a sum's mantissa ends in whole numbers
-    const double y = ((double)x - (double)top) * rate, t = fma(y, 369.32994629211595, kRound), z = fma(t - kRound, -0.0027076061740622863, y);  // 256 / ln 2, ln 2 / 256
-    if ((uint32_t)__double2hiint(y) >= 0xC0859000u) return 0.0;  // below -690 (as a pattern of bits; -inf and NaN too): under 1e-299
+    const double y = ((double)top - (double)x) * rate, t = fma(y, -369.32994629211595, kRound), z = fma(kRound - t, 0.0027076061740622863, -y);  // 256 / ln 2, ln 2 / 256
     const int k = __double2loint(t);
     const double p = table[k & (kTable - 1)], e = fma(p, fma(z * z, fma(z, 1.0 / 6.0, 0.5), z), p);
-    return __hiloint2double(__double2hiint(e) + ((k >> 8) << 20), __double2loint(e));
+    const double scaled = __hiloint2double(__double2hiint(e) + ((k >> 8) << 20), __double2loint(e));
+    // above 690 (as a pattern of bits; infinity and NaN too): under 1e-299, or one of the infinities that are the largest.  No branch: eight of these run side by side.
+    return (uint32_t)__double2hiint(y) < 0x40859000u ? scaled : x == top ? 1.0 : 0.0;
 }
 __device__ __forceinline__ double not_below_zero(double v) { return __double2hiint(v) < 0 ? 0.0 : v; }
 
@@ -252,56 +260,76 @@ template <class E>
 struct Law {
     Row<E> p, q;
     float p_top, q_top;
-    double p_rate, q_rate;         // 1 / sum of the weights
+    double scale, p_rate, q_rate;  // 1 / T; 1 / sum of the weights
     int without;                   // index that has no weight (a draft without probabilities), -1: none
     bool less;                     // q is taken off
+    // What the elements of word w of p's row are drawn by (outside the row: 0).
+    __device__ __forceinline__ void chances(int w, bool drop, const double* table, double (&c)[Row<E>::N]) const {
+        constexpr int N = Row<E>::N;
+        const int i0 = p.index(w);
+        float v[N];
+        p.load(w, v);
+#pragma unroll
+        for (int e = 0; e < N; ++e) c[e] = weight(v[e], p_top, scale, table) * p_rate;
+        if (!drop) return;
+        if (less) {
+            if (q.skew == p.skew) {
+                q.load(w, v);
+            } else {
+#pragma unroll
+                for (int e = 0; e < N; ++e) v[e] = i0 + e >= 0 && i0 + e < p.vocab ? Logit<E>::at(q.row + i0 + e) : kNone;
+            }
+#pragma unroll
+            for (int e = 0; e < N; ++e) c[e] = not_below_zero(fma(-q_rate, weight(v[e], q_top, scale, table), c[e]));
+        } else {
+#pragma unroll
+            for (int e = 0; e < N; ++e)
+                if (i0 + e == without) c[e] = 0.0;
+        }
+    }
 };
 
-template <class E>
-__global__ void __launch_bounds__(kDrawThreads, 2) __cluster_dims__(kCluster, 1, 1) verify_draw_kernel(const VerifyArgs a, const Stretches stretches) {
-    constexpr int N = Logit<E>::kPerWord;
-    __shared__ int fallen;
-    __shared__ double table[kTable], warp_p[kDrawWarps], warp_q[kDrawWarps], cta_p, cta_q, warp_sums[kDrawWarps], cta_sum;
-    cg::cluster_group cluster = cg::this_cluster();
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, rank = (int)cluster.block_rank(), s = blockIdx.x / kCluster;
-    for (int i = tid; i < kTable; i += kDrawThreads) table[i] = exp2((double)i / kTable);
-    pdl_trigger();
-    pdl_wait();
-    const int start = min(max(a.row_start[s], 0), a.rows), n = min(max(a.row_start[s + 1], 0), a.rows) - start;
-    if (n <= 0) {
-        if (rank == 0 && tid == 0) a.accepted[s] = 0;
-        return;  // the whole cluster does
+// How far a sequence's drafts stand, and what the next token is drawn from.
+struct Choice {
+    int kept;
+    float p_top, q_top;
+    int token;  // kDraw, or what is known already: the largest logit's index, -1 where every token is masked
+};
+constexpr int kDraw = -2;
+
+__device__ __forceinline__ Stat row_stat(const VerifyArgs& a, const Stretches& stretches, bool draft, int r, float scale) {  // a warp's
+    Stat v = {kNone, 0.f, 0x7fffffff, 0};
+    const Stat* from = static_cast<const Stat*>(a.stats) + ((size_t)(draft ? a.rows : 0) + r) * stretches.count;
+    for (int i = threadIdx.x & 31; i < stretches.count; i += 32) {
+        const float4 w = __ldcg(reinterpret_cast<const float4*>(from) + i);
+        v = join(v, Stat{w.x, w.y, __float_as_int(w.z), 0}, scale);
     }
+    return warp_join(v, scale);
+}
+// Every thread of the CTA calls it, n > 0: a warp a draft, and then all of them the row that is drawn from.
+template <class E>
+__device__ __forceinline__ Choice choose(const VerifyArgs& a, const Stretches& stretches, int s, int start, int n, const double* table) {
+    __shared__ int fallen;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const float T = temperature_of(a, s);
     const bool greedy = !(T > 0.f);
     const float scale_f = greedy ? 0.f : 1.4426950408889634f / T;
     const double scale = greedy ? 0.0 : 1.0 / (double)T;
-    const Stat* stats = static_cast<const Stat*>(a.stats);
-    auto row_stat = [&](bool draft, int r) {  // a warp's
-        Stat v = {kNone, 0.f, 0x7fffffff, 0};
-        const Stat* from = stats + ((size_t)(draft ? a.rows : 0) + r) * stretches.count;
-        for (int i = lane; i < stretches.count; i += 32) {
-            const float4 w = __ldcg(reinterpret_cast<const float4*>(from) + i);
-            v = join(v, Stat{w.x, w.y, __float_as_int(w.z), 0}, scale_f);
-        }
-        return warp_join(v, scale_f);
-    };
     if (tid == 0) fallen = n - 1;
     __syncthreads();
-    // ── which drafts stand: a warp a draft, the same in every CTA of the cluster ──
     for (int j = warp; j < n - 1; j += kDrawWarps) {
         const int r = start + j, x = a.tokens[r + 1];
-        const Stat p = row_stat(false, r);
+        const Stat p = row_stat(a, stretches, false, r, scale_f);
         bool stands = false;
         if (x >= 0 && x < a.vocab) {
             if (greedy) {
                 stands = p.index == x;
             } else {
-                const double px = p.sum > 0.f ? weight(known(Logit<E>::at(logits_row<E>(a, false, s, r, j) + x)), p.top, scale, table) / (double)p.sum : 0.0;
+                const double px = p.sum > 0.f ? weight(Logit<E>::at(logits_row<E>(a, false, s, r, j) + x), p.top, scale, table) / (double)p.sum : 0.0;
                 double qx = 1.0;
                 if (a.draft) {
-                    const Stat q = row_stat(true, r);
-                    qx = q.sum > 0.f ? weight(known(Logit<E>::at(logits_row<E>(a, true, s, r, j) + x)), q.top, scale, table) / (double)q.sum : 0.0;
+                    const Stat q = row_stat(a, stretches, true, r, scale_f);
+                    qx = q.sum > 0.f ? weight(Logit<E>::at(logits_row<E>(a, true, s, r, j) + x), q.top, scale, table) / (double)q.sum : 0.0;
                 }
                 stands = (double)a.random[r] * qx < px;
             }
@@ -309,43 +337,59 @@ __global__ void __launch_bounds__(kDrawThreads, 2) __cluster_dims__(kCluster, 1,
         if (!stands && lane == 0) atomicMin(&fallen, j);
     }
     __syncthreads();
-    const int kept = fallen, r = start + kept;
-    const bool last = kept == n - 1;
-    const Stat p = row_stat(false, r);
-    auto answer = [&](int token) {  // a thread's
-        for (int i = 0; i < n; ++i) a.out_tokens[start + i] = i < kept ? a.tokens[start + 1 + i] : i == kept ? token : -1;
-        a.accepted[s] = kept;
-    };
-    if (greedy || p.top == kNone) {
-        if (rank == 0 && tid == 0) answer(p.top == kNone ? -1 : p.index);
-        return;  // the whole cluster does
-    }
-    const bool less = !last && a.draft != nullptr;
-    Law<E> law = {Row<E>(logits_row<E>(a, false, s, r, kept), a.vocab), Row<E>(less ? logits_row<E>(a, true, s, r, kept) : logits_row<E>(a, false, s, r, kept), a.vocab),
-                  p.top, 0.f, 0.0, 0.0, !last && !a.draft ? a.tokens[r + 1] : -1, less};
-    if (less) law.q_top = row_stat(true, r).top;
-    // the warp's words of a row, in order of (rank, warp)
-    auto words_of = [&](const Row<E>& row, int& w1) {
-        const int words = row.words(), each = (words + kCluster * kDrawWarps - 1) / (kCluster * kDrawWarps), w0 = (rank * kDrawWarps + warp) * each;
-        w1 = min(words, w0 + each);
-        return w0;
-    };
-    auto warp_total = [&](double v) {
+    Choice c;
+    c.kept = fallen;
+    const Stat p = row_stat(a, stretches, false, start + c.kept, scale_f);
+    c.p_top = p.top;
+    c.q_top = kNone;
+    c.token = p.top == kNone ? -1 : greedy ? p.index : kDraw;
+    if (c.token == kDraw && a.draft && c.kept < n - 1) c.q_top = row_stat(a, stretches, true, start + c.kept, scale_f).top;
+    return c;
+}
+
+// A row's words in the order of (piece of the row, warp of the CTA that has it).
+template <class E>
+__device__ __forceinline__ int words_of(const Row<E>& row, int pieces, int piece, int warp, int& w1) {
+    const int words = row.words(), each = (words + 32 * pieces * kDrawWarps - 1) / (32 * pieces * kDrawWarps) * 32, w0 = min(words, (piece * kDrawWarps + warp) * each);
+    w1 = min(words, w0 + each);
+    return w0;
+}
+__device__ __forceinline__ double warp_total(double v) {
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-        return v;
-    };
-    auto cta_total = [&](const double* sums) {  // of the warps, in order
-        double v = 0.0;
-#pragma unroll
-        for (int w = 0; w < kDrawWarps; ++w) v += sums[w];
-        return v;
-    };
-    // ── sums of the weights ──
-    auto sum_row = [&](const Row<E>& row, float top) {
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+__device__ __forceinline__ void fill_table(double* table) {
+    for (int i = threadIdx.x; i < kTable; i += kDrawThreads) table[i] = exp2((double)i / kTable);
+}
+__device__ __forceinline__ int rows_of(const VerifyArgs& a, int s, int& start) {
+    start = min(max(a.row_start[s], 0), a.rows);
+    return min(max(a.row_start[s + 1], 0), a.rows) - start;
+}
+
+// With a draft's probabilities: which drafts stand, and a piece's sums of the weights of p and q, where they are to be subtracted.
+template <class E>
+__global__ void __launch_bounds__(kDrawThreads, 2) verify_sums_kernel(const VerifyArgs a, const Stretches stretches, const Draws draws) {
+    constexpr int N = Logit<E>::kPerWord;
+    __shared__ double table[kTable], sums[2][kDrawWarps];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, s = blockIdx.x / draws.pieces, piece = blockIdx.x - s * draws.pieces;
+    fill_table(table);
+    pdl_trigger();
+    pdl_wait();
+    int start;
+    const int n = rows_of(a, s, start);
+    if (n <= 0) return;
+    const Choice c = choose<E>(a, stretches, s, start, n, table);
+    if (piece == 0 && tid == 0) draws.choice[s] = c;
+    if (c.token != kDraw || c.kept == n - 1) return;
+    const double scale = 1.0 / (double)temperature_of(a, s);
+#pragma unroll 1
+    for (int side = 0; side < 2; ++side) {
+        const Row<E> row(logits_row<E>(a, side, s, start + c.kept, c.kept), a.vocab);
+        const float top = side ? c.q_top : c.p_top;
         double sum = 0.0;
         int w1;
-        const int w0 = words_of(row, w1);
+        const int w0 = words_of(row, draws.pieces, piece, warp, w1);
         if (top != kNone)
 #pragma unroll 2
             for (int w = w0 + lane; w < w1; w += 32) {
@@ -354,166 +398,238 @@ __global__ void __launch_bounds__(kDrawThreads, 2) __cluster_dims__(kCluster, 1,
 #pragma unroll
                 for (int e = 0; e < N; ++e) sum += weight(v[e], top, scale, table);
             }
-        return warp_total(sum);
-    };
-    law.p_rate = 1.0;  // without a draft's chances to take off, weights need no common measure
-    if (less) {
-        const double sp = sum_row(law.p, law.p_top), sq = sum_row(law.q, law.q_top);
-        if (lane == 0) { warp_p[warp] = sp; warp_q[warp] = sq; }
-        __syncthreads();
-        if (tid == 0) {
-            cta_p = cta_total(warp_p);
-            cta_q = cta_total(warp_q);
-        }
-        cluster.sync();
-        double x = 0.0, y = 0.0;
+        sum = warp_total(sum);
+        if (lane == 0) sums[side][warp] = sum;
+    }
+    __syncthreads();
+    if (tid < 2) {
+        double v = 0.0;
 #pragma unroll
-        for (int c = 0; c < kCluster; ++c) { x += *cluster.map_shared_rank(&cta_p, c); y += *cluster.map_shared_rank(&cta_q, c); }
+        for (int w = 0; w < kDrawWarps; ++w) v += sums[tid][w];
+        draws.sums[((size_t)s * draws.pieces + piece) * 2 + tid] = v;
+    }
+}
+
+// The next token.  Every warp leaves what its words of the row are drawn by; the last CTA of a sequence finds the warp in whose words the running
+// sum passes u times the whole, and there the index.
+template <class E>
+__global__ void __launch_bounds__(kDrawThreads, 2) verify_pick_kernel(const VerifyArgs a, const Stretches stretches, const Draws draws) {
+    constexpr int N = Logit<E>::kPerWord;
+    __shared__ double table[kTable], upto_warp[kDrawWarps], part_at;
+    __shared__ int last, first, with, part;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, s = blockIdx.x / draws.pieces, piece = blockIdx.x - s * draws.pieces;
+    fill_table(table);
+    pdl_trigger();
+    pdl_wait();
+    int start;
+    const int n = rows_of(a, s, start);
+    if (n <= 0) {
+        if (piece == 0 && tid == 0) a.accepted[s] = 0;
+        return;
+    }
+    Choice c;
+    if (a.draft) {
+        const float4 w = __ldcg(reinterpret_cast<const float4*>(draws.choice + s));
+        c = {__float_as_int(w.x), w.y, w.z, __float_as_int(w.w)};
+        __syncthreads();  // the table
+    } else {
+        c = choose<E>(a, stretches, s, start, n, table);
+    }
+    const int r = start + c.kept;
+    auto answer = [&](int token) {  // a warp's
+        for (int i = lane; i < n; i += 32) a.out_tokens[start + i] = i < c.kept ? a.tokens[start + 1 + i] : i == c.kept ? token : -1;
+        if (lane == 0) a.accepted[s] = c.kept;
+    };
+    if (c.token != kDraw) {
+        if (piece == 0 && warp == 0) answer(c.token);
+        return;
+    }
+    const bool less = c.kept < n - 1 && a.draft;
+    Law<E> law = {Row<E>(logits_row<E>(a, false, s, r, c.kept), a.vocab), Row<E>(logits_row<E>(a, less, s, r, c.kept), a.vocab), c.p_top, c.q_top,
+                  1.0 / (double)temperature_of(a, s), 1.0, 0.0, c.kept < n - 1 && !a.draft ? a.tokens[r + 1] : -1, less};
+    if (less) {  // (without a draft's chances to take off, weights need no common measure)
+        double x = 0.0, y = 0.0;
+        for (int i = lane; i < draws.pieces; i += 32) {
+            const double2 v = __ldcg(reinterpret_cast<const double2*>(draws.sums) + (size_t)s * draws.pieces + i);
+            x += v.x;
+            y += v.y;
+        }
+        x = warp_total(x);
+        y = warp_total(y);
         law.p_rate = 1.0 / x;
         law.q_rate = y > 0.0 ? 1.0 / y : 0.0;
     }
-    // What the elements of word w of p's row are drawn by (outside the row: 0).
-    auto chances = [&](int w, bool drop, double (&c)[N]) {
-        const int i0 = law.p.index(w);
-        float v[N];
-        law.p.load(w, v);
-#pragma unroll
-        for (int e = 0; e < N; ++e) c[e] = weight(v[e], law.p_top, scale, table) * law.p_rate;
-        if (!drop) return;
-        if (law.less) {
-            if (law.q.skew == law.p.skew) {
-                law.q.load(w, v);
-            } else {
-#pragma unroll
-                for (int e = 0; e < N; ++e) v[e] = i0 + e >= 0 && i0 + e < a.vocab ? known(Logit<E>::at(law.q.row + i0 + e)) : kNone;
-            }
-#pragma unroll
-            for (int e = 0; e < N; ++e) c[e] = not_below_zero(fma(-law.q_rate, weight(v[e], law.q_top, scale, table), c[e]));
-        } else {
-#pragma unroll
-            for (int e = 0; e < N; ++e)
-                if (i0 + e == law.without) c[e] = 0.0;
-        }
-    };
-    int w1;
-    const int w0 = words_of(law.p, w1);
-    // ── max(p - q, 0); where that leaves nothing, p ──
-    for (int drop = law.less || law.without >= 0 ? 1 : 0; drop >= 0; --drop) {
+    double* const by_warp = draws.chances + (size_t)s * draws.pieces * kDrawWarps;
+    auto weigh = [&](int of, bool drop) {  // a piece's
         double sum = 0.0;
+        int w1;
+        const int w0 = words_of(law.p, draws.pieces, of, warp, w1);
+#pragma unroll 1
         for (int w = w0 + lane; w < w1; w += 32) {
-            double c[N];
-            chances(w, drop, c);
+            double v[N];
+            law.chances(w, drop, table, v);
 #pragma unroll
-            for (int e = 0; e < N; ++e) sum += c[e];
+            for (int e = 0; e < N; ++e) sum += v[e];
         }
         sum = warp_total(sum);
-        if (lane == 0) warp_sums[warp] = sum;
+        if (lane == 0) __stcg(by_warp + of * kDrawWarps + warp, sum);
+    };
+    bool drop = less || law.without >= 0;
+    weigh(piece, drop);
+    __threadfence();
+    __syncthreads();
+    if (tid == 0) last = atomicAdd(draws.arrived + s, 1) == draws.pieces - 1;
+    __syncthreads();
+    if (!last) return;
+    __threadfence();
+    // ── the warp whose words have the border: a thread some of them in a row ──
+    const int all = draws.pieces * kDrawWarps, each = (all + kDrawThreads - 1) / kDrawThreads, m0 = min(all, tid * each), m1 = min(all, m0 + each);
+    double mine, before, total;
+    for (;; drop = false) {
+        mine = 0.0;
+        for (int m = m0; m < m1; ++m) mine += __ldcg(by_warp + m);
+        double incl = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const double x = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += x;
+        }
+        before = __shfl_up_sync(0xffffffffu, incl, 1);
+        if (lane == 0) before = 0.0;
+        if (lane == 31) upto_warp[warp] = incl;
+        if (tid == 0) { first = kDrawThreads; with = 0; }
         __syncthreads();
-        if (tid == 0) cta_sum = cta_total(warp_sums);
-        cluster.sync();
-        double sums[kCluster], before = 0.0, total = 0.0;
-        int owner = -1, last_with = -1;
+        total = 0.0;
 #pragma unroll
-        for (int c = 0; c < kCluster; ++c) sums[c] = *cluster.map_shared_rank(&cta_sum, c);
-#pragma unroll
-        for (int c = 0; c < kCluster; ++c) total += sums[c];
-        const double chance = (double)a.random[start + n - 1] * total;
-        double run = 0.0;
-#pragma unroll
-        for (int c = 0; c < kCluster; ++c) {
-            const double x = sums[c];
-            if (c == rank) before = run;
-            run += x;
-            if (x > 0.0) last_with = c;
-            if (owner < 0 && run > chance) owner = c;
+        for (int w = 0; w < kDrawWarps; ++w) {
+            if (w == warp) before += total;
+            total += upto_warp[w];
         }
-        if (owner < 0) owner = last_with;
-        cluster.sync();  // the sums have been read: they may be written again, and their CTA may end
-        if (total > 0.0) {
-            if (owner != rank) return;
-            int mine = -1, with = -1;
-            double at = before, at_mine = before;
-#pragma unroll
-            for (int w = 0; w < kDrawWarps; ++w) {
-                if (warp_sums[w] > 0.0) with = w;
-                if (mine < 0 && at + warp_sums[w] > chance) { mine = w; at_mine = at; }
-                at += warp_sums[w];
-            }
-            if (mine < 0) {
-                mine = with;
-                at_mine = INFINITY;  // behind every border: the last index with a weight
-            }
-            if (warp != mine) return;
-            // ── the index, 32 words at a time ──
-            double base = at_mine;
-            int found = -1, best = -1;
-            for (int w = w0; w < w1 && found < 0; w += 32) {
-                double c[N], lane_sum = 0.0;
-#pragma unroll
-                for (int e = 0; e < N; ++e) c[e] = 0.0;
-                if (w + lane < w1) chances(w + lane, drop, c);
-                int lane_best = -1;
-#pragma unroll
-                for (int e = 0; e < N; ++e) {
-                    lane_sum += c[e];
-                    if (c[e] > 0.0) lane_best = law.p.index(w + lane) + e;
-                }
-                double incl = lane_sum;
-#pragma unroll
-                for (int o = 1; o < 32; o <<= 1) {
-                    const double x = __shfl_up_sync(0xffffffffu, incl, o);
-                    if (lane >= o) incl += x;
-                }
-                double run_e = base + (incl - lane_sum);
-                int hit = 0x7fffffff;
-#pragma unroll
-                for (int e = 0; e < N; ++e) {
-                    run_e += c[e];
-                    if (hit == 0x7fffffff && c[e] > 0.0 && run_e > chance && at_mine != INFINITY) hit = law.p.index(w + lane) + e;
-                }
-#pragma unroll
-                for (int o = 16; o > 0; o >>= 1) {
-                    hit = min(hit, __shfl_xor_sync(0xffffffffu, hit, o));
-                    lane_best = max(lane_best, __shfl_xor_sync(0xffffffffu, lane_best, o));
-                }
-                if (hit != 0x7fffffff) found = hit;
-                if (lane_best >= 0) best = lane_best;
-                base += __shfl_sync(0xffffffffu, incl, 31);
-            }
-            if (lane == 0) answer(found >= 0 ? found : best);
-            return;
-        }
+        if (total > 0.0 || !drop) break;
+        for (int of = 0; of < draws.pieces; ++of) weigh(of, false);  // p - q leaves nothing: p, and this CTA alone
+        __threadfence();
+        __syncthreads();
     }
-    if (rank == 0 && tid == 0) answer(-1);
+    const double chance = (double)a.random[start + n - 1] * total, none = INFINITY;
+    if (mine > 0.0) {
+        atomicMax(&with, tid);
+        if (before + mine > chance) atomicMin(&first, tid);
+    }
+    __syncthreads();
+    const bool past = first < kDrawThreads;
+    if (tid == (past ? first : with)) {
+        int part_with = m0;
+        part = -1;
+        part_at = none;  // behind every border: the last index with a weight
+        for (int m = m0; m < m1; ++m) {
+            const double v = __ldcg(by_warp + m);
+            if (v > 0.0) part_with = m;
+            if (part < 0 && past && v > 0.0 && before + v > chance) { part = m; part_at = before; }
+            before += v;
+        }
+        if (part < 0) part = part_with;
+    }
+    __syncthreads();
+    if (warp) return;
+    if (!(total > 0.0)) {
+        answer(-1);
+        return;
+    }
+    double base = part_at;
+    const bool behind = base == none;
+    // ── the index, 32 words at a time ──
+    int w1, found = -1, best = -1;
+    for (int w = words_of(law.p, draws.pieces, part / kDrawWarps, part % kDrawWarps, w1); w < w1 && found < 0; w += 32) {
+        double v[N], lane_sum = 0.0;
+#pragma unroll
+        for (int e = 0; e < N; ++e) v[e] = 0.0;
+        if (w + lane < w1) law.chances(w + lane, drop, table, v);
+        int lane_best = -1;
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            lane_sum += v[e];
+            if (v[e] > 0.0) lane_best = law.p.index(w + lane) + e;
+        }
+        double upto = lane_sum;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const double x = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += x;
+        }
+        double run = base + (upto - lane_sum);
+        int hit = 0x7fffffff;
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            run += v[e];
+            if (hit == 0x7fffffff && v[e] > 0.0 && run > chance && !behind) hit = law.p.index(w + lane) + e;
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            hit = min(hit, __shfl_xor_sync(0xffffffffu, hit, o));
+            lane_best = max(lane_best, __shfl_xor_sync(0xffffffffu, lane_best, o));
+        }
+        if (hit != 0x7fffffff) found = hit;
+        if (lane_best >= 0) best = lane_best;
+        base += __shfl_sync(0xffffffffu, upto, 31);
+    }
+    answer(found >= 0 ? found : best);
 }
 
-template <class E>
-cudaError_t go(const Launch& l, const VerifyArgs& a) {
-    const int rows = (a.draft ? 2 : 1) * a.rows;
-    const Stretches stretches = stretches_of(rows, a.vocab, Logit<E>::kPerWord);
+size_t padded(size_t bytes) { return (bytes + 15) & ~(size_t)15; }
+size_t stats_bytes(int rows, const Stretches& stretches) { return (size_t)rows * stretches.count * sizeof(Stat); }
+// Where the pieces of the rows that are drawn from leave their sums (memory null: the bytes only).
+size_t draws_of(unsigned char* memory, int n_seqs, int vocab, int per_word, Draws* d) {
+    const int words = (vocab + 2 * per_word - 2) / per_word, most = (words + kDrawThreads - 1) / kDrawThreads;
+    const int wanted = n_seqs < kDrawCtas ? kDrawCtas / (n_seqs > 0 ? n_seqs : 1) : 1, turns = (most + wanted - 1) / wanted;  // of a warp over 32 words
+    d->pieces = (most + turns - 1) / turns;
+    size_t at = 0;
+    auto room = [&](size_t bytes) {
+        unsigned char* p = memory ? memory + at : nullptr;
+        at += padded(bytes);
+        return p;
+    };
+    d->choice = (Choice*)room((size_t)n_seqs * sizeof(Choice));
+    d->arrived = (int*)room((size_t)n_seqs * sizeof(int));
+    d->sums = (double*)room((size_t)n_seqs * d->pieces * 2 * sizeof(double));
+    d->chances = (double*)room((size_t)n_seqs * d->pieces * kDrawWarps * sizeof(double));
+    return at;
+}
+
+template <class Kernel, class... Args>
+cudaError_t launch(const Launch& l, Kernel kernel, unsigned grid, int threads, Args... args) {
+    const cudaError_t e = prefer_max_shared(kernel);
+    if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)rows * (unsigned)stretches.count);
-    cfg.blockDim = dim3(kStatThreads);
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(threads);
     cfg.stream = l.stream;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = l.pdl ? 1 : 0;
-    cudaError_t e = prefer_max_shared(verify_stats_kernel<E>);
-    if (e == cudaSuccess) e = cudaLaunchKernelEx(&cfg, verify_stats_kernel<E>, a, stretches);
-    if (e == cudaSuccess) e = prefer_max_shared(verify_draw_kernel<E>);
-    if (e != cudaSuccess) return e;
-    cfg.gridDim = dim3((unsigned)a.n_seqs * kCluster);
-    cfg.blockDim = dim3(kDrawThreads);
-    return cudaLaunchKernelEx(&cfg, verify_draw_kernel<E>, a, stretches);
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
+template <class E>
+cudaError_t go(const Launch& l, const VerifyArgs& a) {
+    const int rows = (a.draft ? 2 : 1) * a.rows;
+    const Stretches stretches = stretches_of(rows, a.vocab, Logit<E>::kPerWord);
+    Draws draws;
+    draws_of(static_cast<unsigned char*>(a.stats) + stats_bytes(rows, stretches), a.n_seqs, a.vocab, Logit<E>::kPerWord, &draws);
+    const unsigned pieces = (unsigned)a.n_seqs * (unsigned)draws.pieces;
+    cudaError_t e = launch(l, verify_stats_kernel<E>, (unsigned)rows * (unsigned)stretches.count, kStatThreads, a, stretches, draws);
+    if (e == cudaSuccess && a.draft) e = launch(l, verify_sums_kernel<E>, pieces, kDrawThreads, a, stretches, draws);
+    if (e == cudaSuccess) e = launch(l, verify_pick_kernel<E>, pieces, kDrawThreads, a, stretches, draws);
+    return e;
 }
 
 }  // namespace
 
-size_t verify_workspace(LogitsType type, int rows, int vocab, bool draft) {
-    const int all = (draft ? 2 : 1) * rows;
-    return (size_t)all * stretches_of(all, vocab, type == kLogitsF32 ? 4 : 8).count * sizeof(Stat);
+size_t verify_workspace(LogitsType type, int n_seqs, int rows, int vocab, bool draft) {
+    const int all = (draft ? 2 : 1) * rows, per_word = type == kLogitsF32 ? 4 : 8;
+    Draws draws;
+    return stats_bytes(all, stretches_of(all, vocab, per_word)) + draws_of(nullptr, n_seqs, vocab, per_word, &draws);
 }
 
 cudaError_t launch_verify(const Launch& l, LogitsType type, const VerifyArgs& a) {
