@@ -7,9 +7,10 @@
 // however far the position is, and only what is left goes to 32 bits (float sincospi).  Products and sums are fp32, rounded once to the
 // 16-bit type.
 //
-// A CTA takes one row (four from 600 rows on, so that the chain row -> sequence -> length -> page and the sines are paid once for
-// more bytes): a warp a row finds its sequence, all threads share the sines and cosines through shared memory, then a thread takes 16
-// bytes of a head and the 16 bytes they turn with.
+// A CTA takes one row, or two from 900 rows on (the chain row -> sequence -> length -> page and the sines are then paid for
+// twice the bytes; us with one | two, 40 query and 8 key heads of 128: 600 rows 6.2 | 6.9, 900 8.4 | 8.3, 1200 10.3 | 8.4, 32768 103 | 96): a warp a row
+// finds its sequence, all threads share the sines and cosines through shared memory, then a thread takes 16 bytes of a head and
+// the 16 bytes they turn with.  Memory bounds it: 515 MB of 32768 rows go through in 96 us, 5.3 TB/s.
 #include <cuda_bf16.h>
 
 #include "paged.h"
@@ -17,7 +18,7 @@
 namespace smelt {
 namespace {
 
-constexpr int kThreads = 256, kMostRows = 4, kMostPairs = 128;
+constexpr int kThreads = 256, kMostRows = 2, kMostPairs = 128;
 
 template <class E> struct Pair16;
 template <> struct Pair16<__half> {
@@ -32,13 +33,16 @@ template <> struct Pair16<__nv_bfloat16> {
     }
 };
 
+// Every eight pairs a gap of 16 bytes: the lanes of a load, 64 bytes apart, would meet in four banks.
+__host__ __device__ constexpr int slot(int pair) { return pair + (pair >> 3) * 2; }
+
 __device__ __forceinline__ float first_of(float a, float b, float2 t) { return __fsub_rn(__fmul_rn(a, t.x), __fmul_rn(b, t.y)); }
 __device__ __forceinline__ float second_of(float a, float b, float2 t) { return __fadd_rn(__fmul_rn(b, t.x), __fmul_rn(a, t.y)); }
 
 // WIDE: rows of 16 bytes that turn together with rows of 16 bytes (rope_dim a multiple of 8, in halves of 16)
 template <int D, class E, bool HALVES, bool WIDE>
 __global__ void __launch_bounds__(kThreads) paged_append_kernel(const PagedAppendArgs a, const int rows_a_cta) {
-    __shared__ float2 turn[kMostRows][kMostPairs];  // {cos, sin} factor
+    __shared__ __align__(16) float2 turn[kMostRows][slot(kMostPairs)];  // {cos, sin} factor of pair p at slot(p)
     __shared__ long long place[kMostRows];  // of the row's token in the pools (head 0), in elements; -1: nowhere, -2: not a row of the batch
     __shared__ int token[kMostRows];  // position, in tokens
     const PagedArgs& c = a.c;
@@ -74,7 +78,7 @@ __global__ void __launch_bounds__(kThreads) paged_append_kernel(const PagedAppen
         const double turns = (double)token[r] * (a.freq[p] * 0.15915494309189533577);
         float sn, cs;
         sincospif((float)(2.0 * (turns - rint(turns))), &sn, &cs);
-        turn[r][p] = make_float2(cs * a.factor, sn * a.factor);
+        turn[r][slot(p)] = make_float2(cs * a.factor, sn * a.factor);
     }
     __syncthreads();
     const int n_q = a.q ? c.n_q : 0, heads = n_q + c.n_kv;
@@ -112,7 +116,8 @@ __global__ void __launch_bounds__(kThreads) paged_append_kernel(const PagedAppen
                     uint32_t u[4], w[4];
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        const float2 p = Pair16<E>::unpack(xs[e]), q = Pair16<E>::unpack(ys[e]), t0 = t[d + 2 * e], t1 = t[d + 2 * e + 1];
+                        const float4 two = *reinterpret_cast<const float4*>(t + slot(d) + 2 * e);
+                        const float2 p = Pair16<E>::unpack(xs[e]), q = Pair16<E>::unpack(ys[e]), t0 = make_float2(two.x, two.y), t1 = make_float2(two.z, two.w);
                         u[e] = Pair16<E>::pack(first_of(p.x, q.x, t0), first_of(p.y, q.y, t1));
                         w[e] = Pair16<E>::pack(second_of(p.x, q.x, t0), second_of(p.y, q.y, t1));
                     }
@@ -124,9 +129,11 @@ __global__ void __launch_bounds__(kThreads) paged_append_kernel(const PagedAppen
                     const uint32_t xs[4] = {x.x, x.y, x.z, x.w};
                     uint32_t u[4];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const float2 p = Pair16<E>::unpack(xs[e]), t0 = t[4 * j + e];
+                    for (int e = 0; e < 4; e += 2) {
+                        const float4 two = *reinterpret_cast<const float4*>(t + slot(4 * j) + e);
+                        const float2 p = Pair16<E>::unpack(xs[e]), q = Pair16<E>::unpack(xs[e + 1]), t0 = make_float2(two.x, two.y), t1 = make_float2(two.z, two.w);
                         u[e] = Pair16<E>::pack(first_of(p.x, p.y, t0), second_of(p.x, p.y, t0));
+                        u[e + 1] = Pair16<E>::pack(first_of(q.x, q.y, t1), second_of(q.x, q.y, t1));
                     }
                     *reinterpret_cast<uint4*>(dst + d) = make_uint4(u[0], u[1], u[2], u[3]);
                 }
@@ -139,7 +146,7 @@ __global__ void __launch_bounds__(kThreads) paged_append_kernel(const PagedAppen
                     dst[d1] = y;
                 } else {
                     const float fx = (float)x, fy = (float)y;
-                    const uint32_t v = Pair16<E>::pack(first_of(fx, fy, t[j]), second_of(fx, fy, t[j]));
+                    const uint32_t v = Pair16<E>::pack(first_of(fx, fy, t[slot(j)]), second_of(fx, fy, t[slot(j)]));
                     reinterpret_cast<uint16_t*>(dst)[d0] = (uint16_t)v;
                     reinterpret_cast<uint16_t*>(dst)[d1] = (uint16_t)(v >> 16);
                 }
@@ -150,7 +157,7 @@ __global__ void __launch_bounds__(kThreads) paged_append_kernel(const PagedAppen
 
 template <int D, class E>
 cudaError_t go(const Launch& l, const PagedAppendArgs& a) {
-    const int rows_a_cta = a.c.rows >= 600 ? kMostRows : 1;
+    const int rows_a_cta = a.c.rows >= 900 ? kMostRows : 1;
     const bool halves = a.layout == 1, wide = halves ? a.rope_dim % 16 == 0 : a.rope_dim % 8 == 0;
     auto kernel = halves ? (wide ? paged_append_kernel<D, E, true, true> : paged_append_kernel<D, E, true, false>)
                          : (wide ? paged_append_kernel<D, E, false, true> : paged_append_kernel<D, E, false, false>);

@@ -90,11 +90,12 @@ struct Row {
     }
 };
 
-// Stretches of a row: as many as give every SM eight CTAs, of 1024 words at least and 8192 at most.
+// Stretches of a row: as many as give every SM four CTAs (us of the whole with four | eight, 152k tokens: 8 sequences 37 | 39, 16 46 | 50,
+// 48 81 | 81), of 1024 words at least and 8192 at most.
 struct Stretches { int count, words; };
 Stretches stretches_of(int rows, int vocab, int per_word) {
     const int words = (vocab + 2 * per_word - 2) / per_word, least = (words + 8191) / 8192, most = (words + 1023) / 1024;
-    const int wanted = 1184 / (rows > 0 ? rows : 1), count = wanted < least ? least : wanted > most ? most : wanted;
+    const int wanted = 592 / (rows > 0 ? rows : 1), count = wanted < least ? least : wanted > most ? most : wanted;
     return {count, (words + count - 1) / count};
 }
 
