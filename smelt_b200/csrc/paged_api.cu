@@ -59,7 +59,7 @@ size_t attention_plan(const smelt_cuda_ctx* ctx, const smelt_paged_cache* k, con
     size_t at = 0;
     auto room = [&](size_t bytes) {
         void* p = workspace ? static_cast<char*>(workspace) + at : nullptr;
-        at += (bytes + 15) & ~(size_t)15;
+        at += (bytes + 31) & ~(size_t)31;
         return p;
     };
     // Columns of a source: up to 16 on the streaming kernel (8 with heads of 256), more on the tensor core.  us with 16 | 32 columns, 16 sequences of
@@ -83,8 +83,9 @@ size_t attention_plan(const smelt_cuda_ctx* ctx, const smelt_paged_cache* k, con
         line.columns = wide ? paged_wide_columns(D, a->c.ratio) : paged_narrow_columns(D, columns);
         line.column_div = Divisor::of((uint32_t)line.columns);
         line.keys = wide ? paged_wide_keys(D) : paged_narrow_keys();
-        // What an item costs beside its steps: 8 us of 3 us a step on the tensor core (a masked step, the end), 1 us of 1 us a tile on the streaming kernel.
-        line.extra = wide ? 3 : 1;
+        // What an item costs beside its steps: 11 us of 2.2 us a step on the tensor core (the first scores, a masked step, the end; three | five | eight
+        // places: 2000 rows in four prompts 180 | 172 | 173 us, 64 sequences of 16 rows 59 | 60 | 67), 1 us of 1 us a tile on the streaming kernel.
+        line.extra = wide ? 5 : 1;
         line.ctas = ctx->sm_count < kPagedCtas ? ctx->sm_count : kPagedCtas;
         line.workers = wide ? 1 : paged_narrow_workers(D);
         line.cum = (int32_t*)room((size_t)(b->n_seqs + 3) * sizeof(int32_t));

@@ -30,6 +30,7 @@ struct Cfg {
     static constexpr int kSets = D == 256 ? 1 : 2;   // of four softmax warps, each with an accumulator of its own
     static constexpr int kKeys = D == 256 ? 64 : 128;
     static constexpr int kStages = D == 64 ? 3 : 2;
+    static constexpr int kJoint = kSets == 2 ? 32 * 128 * 4 : 0;
     static constexpr int kQTile = 128 * D * 2, kTile = kKeys * D * 2;
     static constexpr int kLoadWarp = kSets * 4, kMmaWarp = kLoadWarp + 4, kThreads = (kMmaWarp + 4) * 32;
     // registers of a thread: the softmax holds a column's scores; 512 threads (384) are launched with 128 (168)
@@ -48,7 +49,7 @@ struct Shared {  // behind the tiles
 };
 template <int D>
 constexpr size_t wide_shared(int n_seqs) {
-    return (size_t)Cfg<D>::kSets * Cfg<D>::kQTile + 2 * Cfg<D>::kStages * Cfg<D>::kTile + Cfg<D>::kSets * 128 * 16 * 4 + ((sizeof(Shared) + 15) & ~(size_t)15) + batch_bytes(n_seqs);
+    return (size_t)Cfg<D>::kSets * Cfg<D>::kQTile + 2 * Cfg<D>::kStages * Cfg<D>::kTile + Cfg<D>::kJoint + ((sizeof(Shared) + 15) & ~(size_t)15) + batch_bytes(n_seqs);
 }
 
 template <class E> struct Pack;
@@ -169,6 +170,16 @@ __device__ __forceinline__ Item item_of(const PagedArgs& c, const PagedLine& lin
     return it;
 }
 
+// 32 bytes; whole: on a boundary of as many
+__device__ __forceinline__ void store32(void* p, const uint32_t (&v)[8], bool whole) {
+    if (whole) {
+        asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
+    } else {
+        reinterpret_cast<uint4*>(p)[0] = make_uint4(v[0], v[1], v[2], v[3]);
+        reinterpret_cast<uint4*>(p)[1] = make_uint4(v[4], v[5], v[6], v[7]);
+    }
+}
+
 template <int REGS> __device__ __forceinline__ void registers_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS)); }
 template <int REGS> __device__ __forceinline__ void registers_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS)); }
 
@@ -186,8 +197,8 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_wide_kernel(const _
     constexpr int KEYS = C::kKeys, S = C::kStages, CHUNKS = D / 8;  // 16-byte chunks of a row
     extern __shared__ __align__(1024) unsigned char raw[];
     unsigned char *q_tiles = raw, *k_tiles = q_tiles + C::kSets * C::kQTile, *v_tiles = k_tiles + S * C::kTile;
-    float* joint = reinterpret_cast<float*>(v_tiles + S * C::kTile);  // what the ends of items go through: [sets][128][16]
-    Shared& sh = *reinterpret_cast<Shared*>(reinterpret_cast<unsigned char*>(joint) + C::kSets * 128 * 16 * 4);
+    float* joint = reinterpret_cast<float*>(v_tiles + S * C::kTile);  // what the set of the other steps has, at the end of an item: [32][128]
+    Shared& sh = *reinterpret_cast<Shared*>(reinterpret_cast<unsigned char*>(joint) + C::kJoint);
     const PagedArgs& c = a.c;
     const PagedLine& line = a.line[which];
     const int tid = threadIdx.x, warp = uniform(tid >> 5), lane = tid & 31;
@@ -705,65 +716,42 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_wide_kernel(const _
             const bool write = writer && f < it.width && alive;
             if (write && part) *part_ml = make_float2(m, l);
             const float rate = part ? 1.f : l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;
-            // 16 values of a column at a time, through shared memory: a store of the warp takes whole sectors of a few columns
-            float* exchange = joint;                                                 // [128][16] of the set that is added to the other
-            float* stage = joint + ((both ? 1 : set) * 4 + (warp & 3)) * (32 * 16);  // [32][16] of the warp
-            auto turned = [](int row, int piece) { return row * 16 + ((piece ^ (row >> 1 & 3)) << 2); };
-            const uint32_t stores = __ballot_sync(0xffffffffu, write);
-            char* dest = reinterpret_cast<char*>(part);  // the column's values in memory
-            if (!part) dest = reinterpret_cast<char*>(static_cast<E*>(a.out) + row * a.out_stride + head * D);
+            // 32 values of a column at a time.  A lane has a column to itself, and writes whole sectors of 32 bytes where the rows begin at one
+            E* to = part ? nullptr : static_cast<E*>(a.out) + row * a.out_stride + head * D;
+            const bool sectors = (reinterpret_cast<uintptr_t>(part ? (const void*)part : to) & 31) == 0;
 #pragma unroll 1
-            for (int x = 0; x < D; x += 16) {
-                uint32_t v[16];
+            for (int x = 0; x < D; x += 32) {
+                uint32_t v[32];
                 if (any && alive) {
-                    tmem_ld16(o_at + x, v);
-                    tmem_wait_ld16(v);
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * mine);
+                    tmem_ld32(o_at + x, v);
+                    tmem_wait_ld32(v);
                 } else {
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) v[e] = 0u;
+                    for (int e = 0; e < 32; ++e) v[e] = 0u;
                 }
-                if (both) {
-                    if (!writer)
+                if (both) {  // one set's to the other's: [32][128] in shared memory
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) *reinterpret_cast<uint4*>(exchange + turned(me, e)) = make_uint4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
+                    for (int e = 0; e < 32; ++e) {
+                        v[e] = __float_as_uint(__uint_as_float(v[e]) * mine);
+                        if (!writer) joint[e * 128 + me] = __uint_as_float(v[e]);
+                    }
                     barrier(2, 256);
                     if (writer)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const float4 w = *reinterpret_cast<const float4*>(exchange + turned(me, e));
-                            v[4 * e] = __float_as_uint(__uint_as_float(v[4 * e]) + w.x); v[4 * e + 1] = __float_as_uint(__uint_as_float(v[4 * e + 1]) + w.y);
-                            v[4 * e + 2] = __float_as_uint(__uint_as_float(v[4 * e + 2]) + w.z); v[4 * e + 3] = __float_as_uint(__uint_as_float(v[4 * e + 3]) + w.w);
-                        }
+                        for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) + joint[e * 128 + me]);
                     barrier(2, 256);
                 }
-                if (!stores) continue;
-                if (part) {  // 64 bytes a column
+                if (!write) continue;
+                if (part) {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) *reinterpret_cast<uint4*>(stage + turned(lane, e)) = make_uint4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
-                    __syncwarp();
+                    for (int e = 0; e < 32; e += 8) store32(part + x + e, *reinterpret_cast<const uint32_t(*)[8]>(v + e), sectors);
+                } else {
+                    uint32_t w[16];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int r = 8 * i + (lane >> 2);
-                        char* to = reinterpret_cast<char*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(dest), r));
-                        if (stores >> r & 1u) *reinterpret_cast<uint4*>(to + x * 4 + (lane & 3) * 16) = *reinterpret_cast<const uint4*>(stage + turned(r, lane & 3));
-                    }
-                } else {  // 32 bytes a column
-                    uint32_t w[8];
+                    for (int e = 0; e < 32; e += 2) w[e / 2] = l == 0.f ? 0u : Pack<E>::two(__uint_as_float(v[e]) * rate, __uint_as_float(v[e + 1]) * rate);
 #pragma unroll
-                    for (int e = 0; e < 16; e += 2) w[e / 2] = l == 0.f ? 0u : Pack<E>::two(__uint_as_float(v[e]) * rate, __uint_as_float(v[e + 1]) * rate);
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) *reinterpret_cast<uint4*>(stage + turned(lane, e)) = make_uint4(w[4 * e], w[4 * e + 1], w[4 * e + 2], w[4 * e + 3]);
-                    __syncwarp();
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const int r = 16 * i + (lane >> 1);
-                        char* to = reinterpret_cast<char*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(dest), r));
-                        if (stores >> r & 1u) *reinterpret_cast<uint4*>(to + x * 2 + (lane & 1) * 16) = *reinterpret_cast<const uint4*>(stage + turned(r, lane & 1));
-                    }
+                    for (int e = 0; e < 16; e += 8) store32(to + x + 2 * e, *reinterpret_cast<const uint32_t(*)[8]>(w + e), sectors);
                 }
-                __syncwarp();
             }
             tc_fence_before();
         });
