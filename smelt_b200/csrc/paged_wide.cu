@@ -145,13 +145,10 @@ __device__ __forceinline__ void barrier(int id, int threads) { asm volatile("bar
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool take) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(take ? 16 : 0) : "memory");
 }
-template <class E> __device__ __forceinline__ bool word_not_finite(const uint4& w) {
-    constexpr uint32_t m = Pack<E>::kInf;
-    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-    bool odd = false;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) odd = odd || (u[i] & m) == m || ((u[i] >> 16) & m) == m;
-    return odd;
+// Not 0 where one of the eight values is not finite: an exponent of all ones, and one more, carries into the sign's place.
+template <class E> __device__ __forceinline__ uint32_t not_finite(const uint4& w) {
+    constexpr uint32_t m = Pack<E>::kInf * 0x10001u, one = (0x8000u - Pack<E>::kInf) * 0x10001u;
+    return (((w.x & m) + one) | ((w.y & m) + one) | ((w.z & m) + one) | ((w.w & m) + one)) & 0x80008000u;
 }
 
 // What every role knows of an item.
@@ -290,9 +287,15 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_wide_kernel(const _
             }
             if (v_check) {
                 barrier(1, 128);  // the stage's words of odd keys are zero
-                for (int r = r_first; r < KEYS; r += ROWS)
-                    for (int k = ch; k < CHUNKS; k += LANES)
-                        if (word_not_finite<E>(*reinterpret_cast<const uint4*>(tile + place(KEYS, r, k)))) atomicOr(&sh.odd[v_behind][r >> 5], 1u << (r & 31));
+#pragma unroll 1
+                for (int r0 = r_first; r0 < KEYS; r0 += 4 * ROWS) {
+                    uint32_t odd[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) odd[i] = not_finite<E>(*reinterpret_cast<const uint4*>(tile + place(KEYS, r0 + i * ROWS, ch)));
+                    if (__any_sync(0xffffffffu, odd[0] | odd[1] | odd[2] | odd[3]))
+                        for (int i = 0; i < 4; ++i)
+                            if (odd[i]) atomicOr(&sh.odd[v_behind][(r0 + i * ROWS) >> 5], 1u << ((r0 + i * ROWS) & 31));
+                }
                 barrier(1, 128);
                 for (int r = r_first; r < KEYS; r += ROWS)
                     if (sh.odd[v_behind][r >> 5] >> (r & 31) & 1u) zero_row(tile, r);
@@ -308,9 +311,12 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_wide_kernel(const _
         };
         uint32_t all_steps = 0;
         each_item([&](const Cursor& cur, const Item& it, bool pair, int n, int, uint32_t, uint32_t step0) {
-            // queries, behind everything that was asked for before them
-            cp_async_wait<0>();
-            hand_over_values();
+            // queries.  Where pages come as boxes the values before them are handed over behind this item's first keys: looking
+            // through them would hold those up.
+            if (!TILED) {
+                cp_async_wait<0>();
+                hand_over_values();
+            }
             if (items > 0) warp_wait(&sh.q_empty, (items - 1) & 1);
             ++items;
             if (pages.q_rows) {
@@ -376,7 +382,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_wide_kernel(const _
                         barrier(1, 128);
                     }
                     copy(&pages.k, k_tiles, &sh.k_full[s]);
-                    if (i > 0) hand_over_values();
+                    hand_over_values();
                     if (use > 0) warp_wait(&sh.v_empty[s], (use - 1) & 1);
                     if (lt < 4) sh.odd[s][lt] = 0;
                     v_check = k0 < it.clear.lo || min(k0 + KEYS, cur.keys.hi) > it.clear.hi;
