@@ -233,7 +233,11 @@ smelt_status smelt_cuda_verify_drafts(smelt_cuda_ctx* ctx, const smelt_verify_ar
     smelt_status s = enter(ctx, &l);
     if (!s) s = verify_args(ctx, v);
     if (s) return s;
-    if (v->n_seqs == 0 || v->rows == 0) return SMELT_OK;
+    if (v->n_seqs == 0) return SMELT_OK;
+    if (v->rows == 0) {  // nobody has a draft
+        if (!v->accepted) return fail(ctx, SMELT_ERR_BAD_ARGUMENT, "verify drafts: null pointer");
+        return check_cuda(ctx, cudaMemsetAsync(v->accepted, 0, (size_t)v->n_seqs * sizeof(int32_t), l.stream), "verify drafts");
+    }
     if (!v->row_start || !v->target || !v->tokens || !v->random || !v->out_tokens || !v->accepted) return fail(ctx, SMELT_ERR_BAD_ARGUMENT, "verify drafts: null pointer");
     const uintptr_t width = v->precision == SMELT_LOGITS_F32 ? 4 : 2;
     if ((uintptr_t)v->target % width || (uintptr_t)v->draft % width) return fail(ctx, SMELT_ERR_BAD_ARGUMENT, "verify drafts: misaligned logits");

@@ -152,7 +152,7 @@ __global__ void __launch_bounds__(kStatThreads) verify_stats_kernel(const Verify
     if (s < 0) return;
     const int n = min(max(a.row_start[s + 1], 0), a.rows) - start, j = r - start;
     if (j >= n - (draft ? 1 : 0)) return;
-    const float T = temperature_of(a, s), scale = T > 0.f ? 1.4426950408889634f / T : 0.f;
+    const float T = temperature_of(a, s), scale = T > 0.f ? 1.4426950408889634f / T : 0.f;  // 0 with T = inf, too: all tokens alike
     const Row<E> row(logits_row<E>(a, draft, s, r, j), a.vocab);
     const int first = stretch * stretches.words, end = min(row.words(), first + stretches.words);
     const int whole0 = max(first, row.skew ? 1 : 0), whole1 = min(end, (row.skew + a.vocab) / N);  // words that lie inside the row
@@ -165,7 +165,7 @@ __global__ void __launch_bounds__(kStatThreads) verify_stats_kernel(const Verify
 #pragma unroll
             for (int e = 0; e < N; ++e) top = fmaxf(top, v[i][e]);
         if (top == kNone) return;
-        if (scale == 0.f) {  // only the largest counts
+        if (!(T > 0.f)) {  // only the largest counts
             if (top > mine.top) {
                 mine.top = top;
                 mine.index = 0x7fffffff;
@@ -184,7 +184,7 @@ __global__ void __launch_bounds__(kStatThreads) verify_stats_kernel(const Verify
             return;
         }
         if (top > mine.top) {
-            mine.sum *= exp2_approx((mine.top - top) * scale);
+            if (mine.top != kNone) mine.sum *= exp2_approx((mine.top - top) * scale);
             mine.top = top;
         }
         const float minus = -mine.top * scale;
@@ -200,7 +200,7 @@ __global__ void __launch_bounds__(kStatThreads) verify_stats_kernel(const Verify
 #pragma unroll
             for (int i = 0; i < K; ++i)
 #pragma unroll
-                for (int e = 0; e < N; ++e) sum[0] += v[i][e] == mine.top ? 1.f : known(v[i][e]) == kNone ? 0.f : exp2_approx((v[i][e] - mine.top) * scale);
+                for (int e = 0; e < N; ++e) sum[0] += v[i][e] == mine.top ? 1.f : known(v[i][e]) == kNone || mine.top == INFINITY ? 0.f : exp2_approx((v[i][e] - mine.top) * scale);
         }
         mine.sum += sum[0];
     };
@@ -297,6 +297,7 @@ struct Choice {
     int token;  // kDraw, or what is known already: the largest logit's index, -1 where every token is masked
 };
 constexpr int kDraw = -2;
+constexpr double kNothing = 1e-12;  // a whole of max(p - q, 0) that is only what equal chances differ by in fp64
 
 __device__ __forceinline__ Stat row_stat(const VerifyArgs& a, const Stretches& stretches, bool draft, int r, float scale) {  // a warp's
     Stat v = {kNone, 0.f, 0x7fffffff, 0};
@@ -506,7 +507,7 @@ __global__ void __launch_bounds__(kDrawThreads, 2) verify_pick_kernel(const Veri
             if (w == warp) before += total;
             total += upto_warp[w];
         }
-        if (total > 0.0 || !drop) break;
+        if (total > (drop && less ? kNothing : 0.0) || !drop) break;
         for (int of = 0; of < draws.pieces; ++of) weigh(of, false);  // p - q leaves nothing: p, and this CTA alone
         __threadfence();
         __syncthreads();

@@ -192,6 +192,58 @@ def test_large_scores_and_small_ones(ctx):
         check_attention(ctx, g, "bf16", 4, cases.Batch(g, [1, 3], [500, 77], 16, 2, 64, prefix=40), scale=scale)
 
 
+@pytest.mark.parametrize("kind,n_q,n_kv,dim", [("f16", 8, 2, 64), ("bf16", 8, 2, 128), ("f16", 8, 2, 256)])
+def test_maxima_that_move_under_many_columns(ctx, kind, n_q, n_kv, dim):
+    """Scores so far apart that a later step's are many powers of two above the first's."""
+    g = np.random.default_rng(dim)
+    for spread in (40.0, -20.0, 0.0):
+        check_attention(ctx, g, kind, n_q, cases.Batch(g, [90, 1], [1500, 77], 16, n_kv, dim), spread=spread)
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("prefix,window", [(0, 0), (0, 30), (70, 0)])
+def test_blocks_of_rows_without_tokens(ctx, dim, prefix, window):
+    g = np.random.default_rng(dim + window)
+    got = check_attention(ctx, g, "f16", 8, cases.Batch(g, [300, 2, 200], [40, 1, 0], 16, 2, dim, prefix=prefix, behind=3), window)
+    assert (got[:260] == 0).all() and (got[300] == 0).all() and (got[302:502] == 0).all()
+
+
+@pytest.mark.parametrize("n_q,n_kv,dim,rows", [(160, 1, 64, [1, 3]), (260, 2, 128, [2, 1]), (129, 1, 256, [1, 2])])
+@pytest.mark.parametrize("prefix", [0, 200])
+def test_more_heads_a_group_than_a_tile_has_columns(ctx, n_q, n_kv, dim, rows, prefix):
+    g = np.random.default_rng(n_q + prefix)
+    check_attention(ctx, g, "bf16", n_q, cases.Batch(g, rows, [700, 90], 16, n_kv, dim, prefix=prefix))
+
+
+@pytest.mark.parametrize("prefix", [0, 90])
+@pytest.mark.parametrize("shift", [0, 16])
+def test_strided_rows_under_many_columns(ctx, prefix, shift):
+    """Rows, outputs and workspace that begin at odd multiples of 16 bytes."""
+    g = np.random.default_rng(prefix)
+    b = cases.Batch(g, [100, 4, 60], [1700, 99, 60], 16, 2, 64, prefix=prefix)
+    k, v, tokens = b.fill(g, np.nan)
+    q, wide = cases.rounded(g.standard_normal((b.total, 8, 64)), "f16"), 8 * 64 + 8
+    d = Device(ctx, b, "f16", 8, k, v)
+    put = np.full((b.total, wide), 7.0)
+    put[:, :512] = q.reshape(b.total, -1)
+    data = ctx.to_device(np.concatenate([np.zeros(shift // 2, np.float16), cases.to_bits(put, "f16").ravel()]))
+    size = C.c_size_t()
+    ctx.call("paged_attention_workspace", C.byref(d.cache), C.byref(d.batch), C.byref(size))
+    work = ctx.alloc(size.value + shift)
+    ctx.call("paged_attention", C.byref(d.cache), C.byref(d.batch), data.at(shift), wide, data.at(shift), wide, 0.2, 0, work.at(shift), size.value)
+    got = data.download(np.float16, (b.total * wide + shift // 2,))[shift // 2:].reshape(b.total, wide).astype(np.float64)
+    assert (got[:, 512:] == 7.0).all()
+    want, large, reach = cases.attend(b, [cases.rounded(t, "f16") for t in tokens], q, np.float32(0.2))
+    assert (np.abs(got[:, :512].reshape(q.shape) - want) <= cases.attend_bound(want, large, reach, "f16", 64)).all()
+
+
+@pytest.mark.parametrize("n_q,dim", [(32, 64), (32, 128), (16, 256)])
+def test_many_sequences_under_many_columns(ctx, n_q, dim):
+    g = np.random.default_rng(dim)
+    rows = g.integers(0, 3, 1024).tolist()
+    check_attention(ctx, g, "bf16", n_q, cases.Batch(g, rows, (np.array(rows) + g.integers(0, 20, 1024)).tolist(), 16, 1, dim))
+
+
 # ── rotation and append ─────────────────────────────────────────────────────
 def check_append(ctx, g, kind, n_q, b, rope_dim, layout, positions=None, factor=1.0, pad=0, queries=True, in_place=False, theta=1e4):
     kv, dim, rows = b.kv, b.dim, b.total
@@ -412,6 +464,46 @@ def test_verify_masked_rows_bad_ids_and_equal_models(ctx):
     out, kept = check_verify(ctx, "f16", start, target, draft, tokens, temperature, random)
     assert kept[0] == 0 and out[start[0]] == -1 and kept[1] == 0 and kept[2] <= 1 and kept[3] == 2 and kept[4] == 1
     check_verify(ctx, "f16", start, target, None, tokens, temperature, random)
+
+
+@pytest.mark.parametrize("kind,pad,shift", [("f16", 0, 0), ("f16", 3, 1), ("f32", 1, 2)])
+def test_verify_bad_ids_under_equal_models_draw_from_the_target(ctx, kind, pad, shift):
+    """p - q leaves nothing but rounding, in rows that begin at different addresses too."""
+    g = np.random.default_rng(25)
+    start, target, draft, tokens, temperature, random = verify_case(g, kind, [2, 3, 2], 40001)
+    for s in range(3):
+        draft[0, s] = target[start[s]]
+        tokens[start[s] + 1] = -1
+    out, kept = check_verify(ctx, kind, start, target, draft, tokens, temperature, random, pad=pad, shift=shift)
+    assert kept.tolist() == [0, 0, 0] and (out[start[:-1]] >= 0).all()
+
+
+@pytest.mark.parametrize("drafted", [True, False])
+def test_verify_many_sequences(ctx, drafted):
+    g = np.random.default_rng(26)
+    start, target, draft, tokens, temperature, random = verify_case(g, "bf16", g.integers(0, 4, 120).tolist(), 9001)
+    check_verify(ctx, "bf16", start, target, draft if drafted else None, tokens, temperature, random)
+
+
+def test_verify_without_end_of_temperature_every_token_is_alike(ctx):
+    g = np.random.default_rng(27)
+    V = 4096
+    target = g.standard_normal((5, V)).astype(np.float32)
+    target[:, 1000:2000] = -np.inf
+    random = np.array([0.25, 0.5, 0.999, 1e-4, 0.75], np.float32)
+    out, kept = run_verify(ctx, "f32", [0, 1, 2, 5], target, None, [0, 0, 0, 5, 7], [np.inf] * 3, random)
+    left = np.r_[0:1000, 2000:V]
+    assert kept.tolist() == [0, 0, 0]  # u = 0.999 and 1 / 3096
+    assert out[0] == left[int(0.25 * left.size)] and out[1] == left[int(0.5 * left.size)]
+    assert out[2] == np.delete(left, 5)[int(0.75 * (left.size - 1))] and out[3:].tolist() == [-1, -1]
+    random[2], random[3] = 1e-4, 3e-4
+    out, kept = run_verify(ctx, "f32", [0, 1, 2, 5], target, None, [0, 0, 0, 5, 7], [np.inf] * 3, random)
+    assert kept.tolist() == [0, 0, 2] and out[2:4].tolist() == [5, 7] and out[4] == left[int(0.75 * left.size)]
+
+
+def test_verify_of_no_rows(ctx):
+    out, kept = run_verify(ctx, "f16", [0, 0, 0], np.zeros((0, 50), np.float16), None, [], [1.0, 1.0], [])
+    assert kept.tolist() == [0, 0] and out.size == 0
 
 
 def test_verify_greedy_ties_take_the_lowest_index(ctx):
