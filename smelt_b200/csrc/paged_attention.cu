@@ -13,7 +13,11 @@
 // CTA joins what its warps have of the same item.
 // P goes into the product as two 16-bit parts: the kernel waits for memory, and rounding P once would cost up to half a step of the
 // 16-bit type.  Keys outside an item are not read (zeros), and a value row that is not finite reaches only the columns that see it.
-// What several CTAs have of an item the last of them joins; with a prefix or the tensor-core kernel in the call paged_merge_kernel does.
+// What several CTAs have of an item the last of them joins; with a prefix paged_merge_kernel does, behind the tensor-core kernel paged_join_kernel.
+//
+// Memory bounds it from some tens of MB on: 819 MB of two long sequences in 150 us (5.4 TB/s), 416 MB of a ragged batch in 82 (5.1 TB/s; a
+// warp has 22 KB on its way, and 255 registers leave the SM eight warps).  Below that a call is a chain of waits, 10 to 15 us: the batch's
+// lengths, page ids, first keys, the joins of warps and of CTAs.
 #include "attention.cuh"
 #include "paged_line.cuh"
 

@@ -11,6 +11,11 @@
 // a few times an item at most, and behind the first step nobody looks for a maximum (1500 rows over 20000 tokens: 594 us with it, 542 without).
 // P is rounded once to the 16-bit type, the type of the values it is multiplied with; sums are fp32.
 //
+// What bounds it: the way from a set's scores through its exponentials to its product and the next scores, 4000 clocks for two tiles and 128 keys, of
+// which the tensor core works 2048 and the exponentials take as many beside it; the loads are hidden.  bf16, 40 query and 8 key heads of
+// 128, pages of 32: 1500 rows over 20000 tokens in 525 us (1.13 PFLOP/s, 67 % of a library product's rate), 4 x 1500 rows over their own 1500
+// tokens in 122, where an item of six steps costs as much again for its beginning and end (lookups and first loads, the masked step, the sums).
+//
 // Value rows that are not finite and that not every column of the step sees are taken out of the product (as zeros) and added
 // for the columns that see them alone, so that nothing reaches a row that it does not see.
 #include <cuda_bf16.h>
