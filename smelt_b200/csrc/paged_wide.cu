@@ -72,12 +72,6 @@ template <> struct Pack<__nv_bfloat16> {
     static __device__ __forceinline__ float one(uint16_t v) { return __uint_as_float((uint32_t)v << 16); }
 };
 
-__device__ __forceinline__ float exp2_approx(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
 // K-major operand: smem_desc_sw128 (tcgen05.cuh).  The values of a step are [key][64 values of a head] blocks of 128-byte rows: as the
 // product's second operand that is the other major order, eight keys to an atom of 1024 bytes, the next 64 values one block further.
 __device__ __forceinline__ uint64_t value_desc(uint32_t smem_addr, uint32_t block_bytes) {
@@ -105,23 +99,6 @@ __device__ __forceinline__ void tmem_ld32(uint32_t t, uint32_t (&v)[32]) {
                    "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
                  : "r"(t)
                  : "memory");
-}
-// Two fp32 values side by side, and both operations on them in one instruction.
-__device__ __forceinline__ uint64_t pair_of(float x, float y) {
-    uint64_t v;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(x), "f"(y));
-    return v;
-}
-__device__ __forceinline__ void split(uint64_t v, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v)); }
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-    uint64_t v;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(a), "l"(b), "l"(c));
-    return v;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-    uint64_t v;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
-    return v;
 }
 // The lowest n bits.
 __device__ __forceinline__ uint32_t below(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; }

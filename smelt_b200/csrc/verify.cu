@@ -12,6 +12,10 @@
 // (with a draft's probabilities) finds the first draft that falls and adds up the weights of p and q, verify_pick_kernel what the next token is
 // drawn by, and its last CTA of a sequence finds the index.  (A cluster of eight CTAs a sequence, which did all of that in one
 // launch, took 45 us for one sequence and 70 for 48 of them, its fp64 pipe busy for an eighth of the time.)
+//
+// us with 152k tokens and a draft's probabilities: 1 sequence of up to six rows 23, 16 45, 48 76, 192 of three 177.  Memory bounds none of it: the statistics of 48
+// sequences (94 MB) take 34 of the 76 (10 operations an element, and four microseconds of a CTA's beginning and end), the fp64 weights, two to an
+// element and twice over, the rest.
 #include <cuda_bf16.h>
 
 #include "paged.h"
@@ -20,7 +24,9 @@ namespace smelt {
 namespace {
 
 constexpr int kStatThreads = 256, kStatWords = 4;  // words of 16 bytes a thread has on their way at a time
-constexpr int kDrawCtas = 592, kDrawThreads = 512, kDrawWarps = kDrawThreads / 32;
+// CTAs of a launch of the draw, and their threads: 80 registers let eight fp64 chains of a thread run side by side (us of the whole, 48 | 192 sequences:
+// 256 threads and three CTAs an SM 76 | 177, 512 and two, of 64 registers, 78 | 186, 512 and one, of 108, 83 | 182).
+constexpr int kDrawCtas = 1184, kDrawThreads = 256, kDrawWarps = kDrawThreads / 32;
 constexpr float kNone = -INFINITY;
 
 // What the kernels behind the statistics leave one another: rows that are drawn from are cut into pieces, a CTA each.
@@ -91,10 +97,10 @@ struct Row {
 };
 
 // Stretches of a row: as many as give every SM four CTAs (us of the whole with four | eight, 152k tokens: 8 sequences 37 | 39, 16 46 | 50,
-// 48 81 | 81), of 1024 words at least and 8192 at most.
+// 48 81 | 81), of 1024 words at least and 16384 at most.
 struct Stretches { int count, words; };
 Stretches stretches_of(int rows, int vocab, int per_word) {
-    const int words = (vocab + 2 * per_word - 2) / per_word, least = (words + 8191) / 8192, most = (words + 1023) / 1024;
+    const int words = (vocab + 2 * per_word - 2) / per_word, least = (words + 16383) / 16384, most = (words + 1023) / 1024;
     const int wanted = 592 / (rows > 0 ? rows : 1), count = wanted < least ? least : wanted > most ? most : wanted;
     return {count, (words + count - 1) / count};
 }
@@ -131,12 +137,6 @@ __device__ __forceinline__ const E* logits_row(const VerifyArgs& a, bool draft, 
     return draft ? static_cast<const E*>(a.draft) + (int64_t)j * a.draft_step_stride + (int64_t)s * a.draft_seq_stride : static_cast<const E*>(a.target) + (int64_t)r * a.target_stride;
 }
 
-__device__ __forceinline__ float exp2_approx(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
 template <class E>
 __global__ void __launch_bounds__(kStatThreads) verify_stats_kernel(const VerifyArgs a, const Stretches stretches, const Draws draws) {
     constexpr int N = Logit<E>::kPerWord;
@@ -146,6 +146,29 @@ __global__ void __launch_bounds__(kStatThreads) verify_stats_kernel(const Verify
     const int r = draft ? y - a.rows : y;
     pdl_trigger();
     pdl_wait();
+    int first = 0, end = 0, whole0 = 0, whole1 = 0;  // words of the stretch, and those of them that lie inside the row
+    const uint4* words = nullptr;
+    uint4 next[kStatWords];
+    auto ask = [&](int w0) {
+#pragma unroll
+        for (int i = 0; i < kStatWords; ++i) {
+            next[i] = make_uint4(Logit<E>::kMasked, Logit<E>::kMasked, Logit<E>::kMasked, Logit<E>::kMasked);
+            if (w0 + i * kStatThreads < whole1) next[i] = __ldg(words + w0 + i * kStatThreads);
+        }
+    };
+    auto open = [&](const E* p) {
+        const Row<E> row(p, a.vocab);
+        first = stretch * stretches.words;
+        end = min(row.words(), first + stretches.words);
+        whole0 = max(first, row.skew ? 1 : 0);
+        whole1 = min(end, (row.skew + a.vocab) / N);
+        words = reinterpret_cast<const uint4*>(row.row - row.skew);
+        ask(whole0 + tid);
+        return row;
+    };
+    // (a row of the target is on its way before it is known whose it is)
+    Row<E> row(static_cast<const E*>(a.target), a.vocab);
+    if (!draft) row = open(logits_row<E>(a, false, 0, r, 0));
     for (int i = blockIdx.x * kStatThreads + tid; i < a.n_seqs; i += gridDim.x * kStatThreads) draws.arrived[i] = 0;
     int start = 0;
     const int s = warp_find_seq(a.row_start, a.n_seqs, a.rows, r, &start);
@@ -153,9 +176,7 @@ __global__ void __launch_bounds__(kStatThreads) verify_stats_kernel(const Verify
     const int n = min(max(a.row_start[s + 1], 0), a.rows) - start, j = r - start;
     if (j >= n - (draft ? 1 : 0)) return;
     const float T = temperature_of(a, s), scale = T > 0.f ? 1.4426950408889634f / T : 0.f;  // 0 with T = inf, too: all tokens alike
-    const Row<E> row(logits_row<E>(a, draft, s, r, j), a.vocab);
-    const int first = stretch * stretches.words, end = min(row.words(), first + stretches.words);
-    const int whole0 = max(first, row.skew ? 1 : 0), whole1 = min(end, (row.skew + a.vocab) / N);  // words that lie inside the row
+    if (draft) row = open(logits_row<E>(a, true, s, r, j));
     Stat mine = {kNone, 0.f, 0x7fffffff, 0};
     auto add = [&](auto& v, auto&& index) {  // v[i][e]: the logit at index(i) + e
         constexpr int K = sizeof(v) / sizeof(v[0]);
@@ -188,11 +209,18 @@ __global__ void __launch_bounds__(kStatThreads) verify_stats_kernel(const Verify
             mine.top = top;
         }
         const float minus = -mine.top * scale;
-        float sum[2] = {0.f, 0.f};
+        const uint64_t scales = pair_of(scale, scale), minuses = pair_of(minus, minus);
+        uint64_t sums = 0ull;
 #pragma unroll
         for (int i = 0; i < K; ++i)
 #pragma unroll
-            for (int e = 0; e < N; ++e) sum[e & 1] += exp2_approx(fmaf(v[i][e], scale, minus));
+            for (int e = 0; e < N; e += 2) {
+                float y0, y1;
+                split(fma2(pair_of(v[i][e], v[i][e + 1]), scales, minuses), y0, y1);
+                sums = add2(sums, pair_of(exp2_approx(y0), exp2_approx(y1)));
+            }
+        float sum[2];
+        split(sums, sum[0], sum[1]);
         sum[0] += sum[1];
         sum[0] = fmaf(-0.69314718f * fmaf(mine.top, scale, minus), sum[0], sum[0]);  // what `minus` was rounded by, which every term has
         if (sum[0] != sum[0]) {  // NaN counts as masked; infinities that are the largest share what there is
@@ -214,16 +242,6 @@ __global__ void __launch_bounds__(kStatThreads) verify_stats_kernel(const Verify
         row.load(end - 1, v[0]);
         add(v, [&](int) { return row.index(end - 1); });
     }
-    const uint4* words = reinterpret_cast<const uint4*>(row.row - row.skew);
-    uint4 next[kStatWords];
-    auto ask = [&](int w0) {
-#pragma unroll
-        for (int i = 0; i < kStatWords; ++i) {
-            next[i] = make_uint4(Logit<E>::kMasked, Logit<E>::kMasked, Logit<E>::kMasked, Logit<E>::kMasked);
-            if (w0 + i * kStatThreads < whole1) next[i] = __ldg(words + w0 + i * kStatThreads);
-        }
-    };
-    ask(whole0 + tid);
 #pragma unroll 1
     for (int w0 = whole0 + tid; w0 < whole1; w0 += kStatThreads * kStatWords) {
         float v[kStatWords][N];
@@ -371,7 +389,7 @@ __device__ __forceinline__ int rows_of(const VerifyArgs& a, int s, int& start) {
 
 // With a draft's probabilities: which drafts stand, and a piece's sums of the weights of p and q, where they are to be subtracted.
 template <class E>
-__global__ void __launch_bounds__(kDrawThreads, 2) verify_sums_kernel(const VerifyArgs a, const Stretches stretches, const Draws draws) {
+__global__ void __launch_bounds__(kDrawThreads, 3) verify_sums_kernel(const VerifyArgs a, const Stretches stretches, const Draws draws) {
     constexpr int N = Logit<E>::kPerWord;
     __shared__ double table[kTable], sums[2][kDrawWarps];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, s = blockIdx.x / draws.pieces, piece = blockIdx.x - s * draws.pieces;
@@ -415,7 +433,7 @@ __global__ void __launch_bounds__(kDrawThreads, 2) verify_sums_kernel(const Veri
 // The next token.  Every warp leaves what its words of the row are drawn by; the last CTA of a sequence finds the warp in whose words the running
 // sum passes u times the whole, and there the index.
 template <class E>
-__global__ void __launch_bounds__(kDrawThreads, 2) verify_pick_kernel(const VerifyArgs a, const Stretches stretches, const Draws draws) {
+__global__ void __launch_bounds__(kDrawThreads, 3) verify_pick_kernel(const VerifyArgs a, const Stretches stretches, const Draws draws) {
     constexpr int N = Logit<E>::kPerWord;
     __shared__ double table[kTable], upto_warp[kDrawWarps], part_at;
     __shared__ int last, first, with, part;
