@@ -677,7 +677,7 @@ __global__ void __launch_bounds__(kMergeWarps * 32) paged_merge_kernel(const __g
 
 // Without one, behind the tensor-core kernel: the columns of the items that begin in a CTA of it and go on behind, shared out evenly.
 constexpr int kJoinWarps = 8;
-constexpr int kJoinCtas = 2;  // of an SM, resident together
+constexpr int kJoinCtas = 2;  // of an SM, with as many registers as the sums ask for (four, of 64: 1 us less of 120 at large calls, 4 more of 27 at small ones)
 
 template <int D, class E>
 __global__ void __launch_bounds__(kJoinWarps * 32, kJoinCtas) paged_join_kernel(const __grid_constant__ PagedAttentionArgs a) {
@@ -750,7 +750,9 @@ cudaError_t launch_paged_narrow(const Launch& l, PagedType type, int head_dim, c
 
 cudaError_t launch_paged_merge(const Launch& l, PagedType type, int head_dim, const PagedAttentionArgs& a) {
     const int64_t all = (int64_t)a.c.rows * a.c.n_q;
-    const int heads = all > (int64_t)a.line[0].ctas * 64 ? a.c.ratio : 1;  // 64 warps an SM hold a head each
+    // A head a warp while 64 warps an SM hold them all, else a group (us of the call with a head | a group, 40 query and 8 key heads behind a prefix of
+    // 2000: 100 rows 29 | 37, 200 39 | 43, 300 51 | 49, 1500 207 | 196).
+    const int heads = all > (int64_t)a.line[0].ctas * 64 ? a.c.ratio : 1;
     const int grid = (int)((all / heads + kMergeWarps - 1) / kMergeWarps);
     auto go = [&](auto f16, auto bf16) { return type == kPagedF16 ? launch(l, f16, grid, kMergeWarps * 32, 0, a, heads) : launch(l, bf16, grid, kMergeWarps * 32, 0, a, heads); };
     if (head_dim == 64) return go(paged_merge_kernel<64, __half>, paged_merge_kernel<64, __nv_bfloat16>);

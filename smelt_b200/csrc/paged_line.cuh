@@ -179,7 +179,6 @@ struct Cursor {
         step = steps - 1;
         advance(c, line, window, b);
     }
-    __device__ __forceinline__ bool same_item(const Cursor& o) const { return source == o.source && block == o.block && head == o.head; }
 };
 
 // The sequence of a packed row, from row starts in shared memory.
