@@ -245,6 +245,7 @@ __global__ void __launch_bounds__(kWarps<D> * 32, 1) paged_narrow_kernel(const _
             tile = more;
             bool take = inside && (uint32_t)page < (uint32_t)c.n_pages;
             if (inside && !take && c.err) atomicOr(c.err, KERR_BAD_PAGE);
+            __syncwarp();  // the last tile's rows have been read by every lane: its last unit may have been issued just before
             rows[lane] = take ? (long long)page * c.page_stride + (long long)slot * c.token_stride + (long long)head * c.head_stride : 0;
             there = __ballot_sync(0xffffffffu, take);
             look_up();
