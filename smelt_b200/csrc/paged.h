@@ -71,6 +71,9 @@ struct PagedArgs {
     uint32_t* err;
 };
 
+// A sequence's tokens on its own pages, cut at both ends to what the table can hold.
+__device__ __forceinline__ int tokens_of(const PagedArgs& c, int s) { return min(max(c.length[s], 0), c.table_tokens); }
+
 struct PagedAppendArgs {
     PagedArgs c;
     int rope_dim, layout;  // layout: 0 adjacent pairs, 1 halves

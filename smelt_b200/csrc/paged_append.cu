@@ -60,7 +60,7 @@ __global__ void __launch_bounds__(kThreads) paged_append_kernel(const PagedAppen
         if (r < total && s >= 0) {
             const int n = min(max(c.row_start[s + 1], 0), c.rows) - start, i = r - start;
             if (i < n) {
-                const int own = min(c.length[s], c.table_tokens) - n + i;
+                const int own = tokens_of(c, s) - n + i;  // [-n, table_tokens)
                 to = -1;
                 if (own >= 0) {
                     const int p = divide(own, c.page_div), page = c.table[(size_t)s * c.table_stride + p];

@@ -13,7 +13,6 @@ struct Range { int lo, hi; };  // keys [lo, hi)
 struct Seq { int row, n, length; };
 
 __device__ __forceinline__ int first_row(const PagedArgs& c, int s) { return min(max(c.row_start[s], 0), c.rows); }
-__device__ __forceinline__ int tokens_of(const PagedArgs& c, int s) { return min(max(c.length[s], 0), c.table_tokens); }
 // Keys of its own pages that row i of a sequence sees.  (Tokens and rows are below 2^30; a window beyond that is none.)
 __device__ __forceinline__ Range own_keys(const Seq& s, int i, uint32_t window) {
     const int hi = max(s.length - s.n + i + 1, 0);

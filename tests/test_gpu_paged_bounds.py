@@ -34,3 +34,26 @@ def test_the_same_call_gives_the_same_bits(ctx, kind, n_q, n_kv, dim, page):
     assert (np.abs(first - want) <= cases.attend_bound(want, size, reach, kind, dim)).all()
     for _ in range(10):
         assert np.array_equal(d.attend(q, 0.1), first)
+
+
+@pytest.mark.parametrize("length", [-2 ** 31, -2 ** 31 + 1, -1, 0, 2 ** 31 - 1])
+@pytest.mark.parametrize("rows", [1, 3])
+def test_append_cuts_lengths_at_both_ends(ctx, length, rows):
+    """Without tokens nothing is written; tokens past the table are its last ones."""
+    g = np.random.default_rng(6)
+    b = cases.Batch(g, [rows, 2], [8, 6], 4, 1, 64)
+    b.table = np.ascontiguousarray(b.table[:, :2])  # eight tokens a sequence
+    k, v, _ = b.fill(g, 5.0)
+    d = Device(ctx, b, "f16", 1, k, v)
+    before = d.pools()[1]
+    d.kept[1].upload(np.array([length, 6], np.int32))
+    new = ctx.to_device(cases.to_bits(g.standard_normal((rows + 2, 64)), "f16"))
+    ctx.call("paged_append", C.byref(d.cache), C.byref(d.batch), None, None, 0, new.ptr, 64, new.ptr, 64, None, 0)
+    want, put = before.copy(), cases.from_bits(new.download(np.float16, (rows + 2, 64)), "f16")
+    for s, at in ((0, 8 - rows if length > 0 else None), (1, 4)):
+        for i in range(b.rows[s]):
+            if at is not None:
+                p, slot = b.place(s, at + i)
+                want[p, 0, slot] = put[b.start[s] + i]
+    assert np.array_equal(d.pools()[1], want)
+    assert ctx.device_error_flags() == (0 if length > 0 else 0x10000)
