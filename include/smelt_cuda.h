@@ -889,10 +889,13 @@ SMELT_CUDA_API smelt_status smelt_cuda_paged_attention(smelt_cuda_ctx* ctx, cons
  * random[row_start[s + 1] - 1] times the whole.  Without draft logits (null) a draft counts as certain: q(x) = 1.
  * T = temperature[s] (null: 1); 0 or less takes the lowest index of the largest logit and accepts drafts that are it.
  * Logits of -inf or NaN have no chance; a drafted id outside the vocabulary falls.
+ * row_start is read on the device: where it may give a sequence more drafts than `draft` has steps, draft_steps says how many there
+ * are, and the drafts behind them are not judged: the token behind the last judged one that stands is drawn from p of its row.
  * Leaves out_tokens[row_start[s] + i] = the accepted drafts, the drawn token (-1 where no token has a chance), then -1, and accepted[s]. */
 enum { SMELT_LOGITS_F16 = 0, SMELT_LOGITS_BF16 = 1, SMELT_LOGITS_F32 = 2 };
 typedef struct {
-    int32_t precision;           /* of both logits: SMELT_LOGITS_* */
+    int16_t precision;           /* of both logits: SMELT_LOGITS_* */
+    uint16_t draft_steps;        /* steps that `draft` holds; 0: as many as the longest sequence has drafts, whatever row_start says */
     int32_t n_seqs, rows, vocab;
     int64_t target_stride, draft_step_stride, draft_seq_stride; /* values: from row to row; from step to step, from sequence to sequence */
     const void *row_start, *target, *draft, *tokens;            /* device; int32 [n_seqs + 1], [rows, vocab], null or [steps, n_seqs, vocab], int32 [rows] */

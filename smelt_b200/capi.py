@@ -183,7 +183,7 @@ class RopeScaling(C.Structure):
 
 class VerifyArgs(C.Structure):
     """``smelt_verify_args``."""
-    _fields_ = ([(n, C.c_int32) for n in ("precision", "n_seqs", "rows", "vocab")] + [(n, C.c_int64) for n in ("target_stride", "draft_step_stride", "draft_seq_stride")]
+    _fields_ = ([("precision", C.c_int16), ("draft_steps", C.c_uint16)] + [(n, C.c_int32) for n in ("n_seqs", "rows", "vocab")] + [(n, C.c_int64) for n in ("target_stride", "draft_step_stride", "draft_seq_stride")]
                 + [(n, C.c_void_p) for n in ("row_start", "target", "draft", "tokens", "temperature", "random", "out_tokens", "accepted", "workspace")] + [("workspace_bytes", C.c_size_t)])
 
 

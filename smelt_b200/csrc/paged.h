@@ -133,6 +133,7 @@ cudaError_t launch_paged_join(const Launch& l, PagedType type, int head_dim, con
 // Drafted tokens against the target (verify.cu).
 struct VerifyArgs {
     int n_seqs, rows, vocab;
+    int steps;  // that the draft holds: a sequence's drafts behind them are not judged
     const void *target, *draft;  // draft may be null
     int64_t target_stride, draft_step_stride, draft_seq_stride;  // elements
     const int32_t *row_start, *tokens;

@@ -249,6 +249,7 @@ smelt_status smelt_cuda_verify_drafts(smelt_cuda_ctx* ctx, const smelt_verify_ar
         return fail(ctx, SMELT_ERR_BAD_ARGUMENT, "verify drafts: workspace missing, misaligned or smaller than smelt_cuda_verify_drafts_workspace says");
     VerifyArgs a = {};
     a.n_seqs = v->n_seqs; a.rows = v->rows; a.vocab = v->vocab;
+    a.steps = v->draft && v->draft_steps ? v->draft_steps : v->rows;
     a.target = v->target; a.draft = v->draft;
     a.target_stride = v->target_stride; a.draft_step_stride = v->draft_step_stride; a.draft_seq_stride = v->draft_seq_stride;
     a.row_start = (const int32_t*)v->row_start; a.tokens = (const int32_t*)v->tokens;

@@ -174,7 +174,7 @@ __global__ void __launch_bounds__(kStatThreads) verify_stats_kernel(const Verify
     const int s = warp_find_seq(a.row_start, a.n_seqs, a.rows, r, &start);
     if (s < 0) return;
     const int n = min(max(a.row_start[s + 1], 0), a.rows) - start, j = r - start;
-    if (j >= n - (draft ? 1 : 0)) return;
+    if (j >= (draft ? min(n - 1, a.steps) : n)) return;
     const float T = temperature_of(a, s), scale = T > 0.f ? 1.4426950408889634f / T : 0.f;  // 0 with T = inf, too: all tokens alike
     if (draft) row = open(logits_row<E>(a, true, s, r, j));
     Stat mine = {kNone, 0.f, 0x7fffffff, 0};
@@ -326,18 +326,18 @@ __device__ __forceinline__ Stat row_stat(const VerifyArgs& a, const Stretches& s
     }
     return warp_join(v, scale);
 }
-// Every thread of the CTA calls it, n > 0: a warp a draft, and then all of them the row that is drawn from.
+// Every thread of the CTA calls it: a warp a draft, `judged` of them, and then all of them the row that is drawn from.
 template <class E>
-__device__ __forceinline__ Choice choose(const VerifyArgs& a, const Stretches& stretches, int s, int start, int n, const double* table) {
+__device__ __forceinline__ Choice choose(const VerifyArgs& a, const Stretches& stretches, int s, int start, int judged, const double* table) {
     __shared__ int fallen;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const float T = temperature_of(a, s);
     const bool greedy = !(T > 0.f);
     const float scale_f = greedy ? 0.f : 1.4426950408889634f / T;
     const double scale = greedy ? 0.0 : 1.0 / (double)T;
-    if (tid == 0) fallen = n - 1;
+    if (tid == 0) fallen = judged;
     __syncthreads();
-    for (int j = warp; j < n - 1; j += kDrawWarps) {
+    for (int j = warp; j < judged; j += kDrawWarps) {
         const int r = start + j, x = a.tokens[r + 1];
         const Stat p = row_stat(a, stretches, false, r, scale_f);
         bool stands = false;
@@ -363,7 +363,7 @@ __device__ __forceinline__ Choice choose(const VerifyArgs& a, const Stretches& s
     c.p_top = p.top;
     c.q_top = kNone;
     c.token = p.top == kNone ? -1 : greedy ? p.index : kDraw;
-    if (c.token == kDraw && a.draft && c.kept < n - 1) c.q_top = row_stat(a, stretches, true, start + c.kept, scale_f).top;
+    if (c.token == kDraw && a.draft && c.kept < judged) c.q_top = row_stat(a, stretches, true, start + c.kept, scale_f).top;
     return c;
 }
 
@@ -386,6 +386,7 @@ __device__ __forceinline__ int rows_of(const VerifyArgs& a, int s, int& start) {
     start = min(max(a.row_start[s], 0), a.rows);
     return min(max(a.row_start[s + 1], 0), a.rows) - start;
 }
+__device__ __forceinline__ int judged_of(const VerifyArgs& a, int n) { return min(n - 1, a.steps); }  // drafts of a sequence of n rows
 
 // With a draft's probabilities: which drafts stand, and a piece's sums of the weights of p and q, where they are to be subtracted.
 template <class E>
@@ -399,9 +400,10 @@ __global__ void __launch_bounds__(kDrawThreads, 3) verify_sums_kernel(const Veri
     int start;
     const int n = rows_of(a, s, start);
     if (n <= 0) return;
-    const Choice c = choose<E>(a, stretches, s, start, n, table);
+    const int judged = judged_of(a, n);
+    const Choice c = choose<E>(a, stretches, s, start, judged, table);
     if (piece == 0 && tid == 0) draws.choice[s] = c;
-    if (c.token != kDraw || c.kept == n - 1) return;
+    if (c.token != kDraw || c.kept == judged) return;
     const double scale = 1.0 / (double)temperature_of(a, s);
 #pragma unroll 1
     for (int side = 0; side < 2; ++side) {
@@ -447,13 +449,14 @@ __global__ void __launch_bounds__(kDrawThreads, 3) verify_pick_kernel(const Veri
         if (piece == 0 && tid == 0) a.accepted[s] = 0;
         return;
     }
+    const int judged = judged_of(a, n);
     Choice c;
     if (a.draft) {
         const float4 w = __ldcg(reinterpret_cast<const float4*>(draws.choice + s));
         c = {__float_as_int(w.x), w.y, w.z, __float_as_int(w.w)};
         __syncthreads();  // the table
     } else {
-        c = choose<E>(a, stretches, s, start, n, table);
+        c = choose<E>(a, stretches, s, start, judged, table);
     }
     const int r = start + c.kept;
     auto answer = [&](int token) {  // a warp's
@@ -464,9 +467,9 @@ __global__ void __launch_bounds__(kDrawThreads, 3) verify_pick_kernel(const Veri
         if (piece == 0 && warp == 0) answer(c.token);
         return;
     }
-    const bool less = c.kept < n - 1 && a.draft;
+    const bool less = c.kept < judged && a.draft;
     Law<E> law = {Row<E>(logits_row<E>(a, false, s, r, c.kept), a.vocab), Row<E>(logits_row<E>(a, less, s, r, c.kept), a.vocab), c.p_top, c.q_top,
-                  1.0 / (double)temperature_of(a, s), 1.0, 0.0, c.kept < n - 1 && !a.draft ? a.tokens[r + 1] : -1, less};
+                  1.0 / (double)temperature_of(a, s), 1.0, 0.0, c.kept < judged && !a.draft ? a.tokens[r + 1] : -1, less};
     if (less) {  // (without a draft's chances to take off, weights need no common measure)
         double x = 0.0, y = 0.0;
         for (int i = lane; i < draws.pieces; i += 32) {

@@ -57,3 +57,40 @@ def test_append_cuts_lengths_at_both_ends(ctx, length, rows):
                 want[p, 0, slot] = put[b.start[s] + i]
     assert np.array_equal(d.pools()[1], want)
     assert ctx.device_error_flags() == (0 if length > 0 else 0x10000)
+
+
+@pytest.mark.parametrize("kind", ["f16", "f32"])
+@pytest.mark.parametrize("steps", [1, 3, 6])
+@pytest.mark.parametrize("t", [0.8, 0.0])
+def test_drafts_behind_the_steps_of_a_draft_are_not_judged(ctx, kind, steps, t):
+    """Row starts that give a sequence more drafts than the draft model left logits for: those of the array are judged, and the token behind
+    them is drawn from the target.  (What lies behind the array here would let every draft stand.)"""
+    g = np.random.default_rng(steps)
+    rows, V = [7, 1, 2, 5, 0, 7, 7], 3001
+    start, target, draft, tokens, temperature, random = verify_case(g, kind, rows, V, near=0.2, peak=9.0)
+    temperature[:] = t
+    for s in (0, 5):  # drafts that stand, as far as anybody looks
+        for j in range(rows[s] - 1):
+            draft[j, s] = target[start[s] + j]
+            tokens[start[s] + 1 + j] = int(np.argmax(cases.from_bits(target[start[s] + j], kind)))
+    word, total = target.dtype.itemsize, int(start[-1])
+    dt, dd = ctx.to_device(target), ctx.to_device(draft)
+    kept = [ctx.to_device(np.asarray(a, w)) for a, w in ((start, np.int32), (tokens, np.int32), (temperature, np.float32), (random, np.float32))]
+    out, accepted = ctx.to_device(np.full(total, -99, np.int32)), ctx.to_device(np.full(len(rows), -99, np.int32))
+    a = capi.VerifyArgs(precision=LOGITS[kind], draft_steps=steps, n_seqs=len(rows), rows=total, vocab=V, target_stride=V, row_start=kept[0].ptr, target=dt.ptr, draft=dd.ptr,
+                        draft_step_stride=len(rows) * V, draft_seq_stride=V, tokens=kept[1].ptr, temperature=kept[2].ptr, random=kept[3].ptr, out_tokens=out.ptr, accepted=accepted.ptr)
+    size = C.c_size_t()
+    ctx.call("verify_drafts_workspace", C.byref(a), C.byref(size))
+    work = ctx.alloc(size.value).fill(0xFF)
+    a.workspace, a.workspace_bytes = work.ptr, size.value
+    ctx.call("verify_drafts", C.byref(a))
+    said, stood = out.download(np.int32, total), accepted.download(np.int32, len(rows))
+    for s, n in enumerate(rows):
+        cut = min(n, steps + 1)
+        at = np.arange(start[s], start[s] + cut)
+        u = random[at].copy()
+        if cut:
+            u[-1] = random[start[s] + n - 1]
+        want, full = cases.verify([0, cut], cases.from_bits(target, kind)[at], cases.from_bits(draft, kind)[:, s:s + 1], np.asarray(tokens)[at], [t], u)
+        assert stood[s] == full[0] and np.array_equal(said[start[s]:start[s] + n], np.concatenate([want, np.full(n - cut, -1)])), (s, said, want)
+    assert stood[0] == min(6, steps) and stood[5] == min(6, steps)
