@@ -831,7 +831,8 @@ SMELT_CUDA_API smelt_status smelt_cuda_prefill(smelt_cuda_ctx* ctx, const smelt_
  * may share a prefix of prefix_length tokens on the pages prefix_table lists: it comes first, and token t of a sequence is at
  * position prefix_length + t.  A sequence may have no rows or no tokens.  Lengths, starts and tables are read on the device, so that a
  * captured call follows them; they are cut to what the arrays can hold.  A page id outside the pool is not followed: nothing is written, its tokens
- * read as zeros, and bit 16 of the device error word is set (smelt_cuda_device_error then returns SMELT_ERR_OUT_OF_RANGE). */
+ * read as zeros, and bit 16 of the device error word is set (smelt_cuda_device_error then returns SMELT_ERR_OUT_OF_RANGE).  Row starts do
+ * not go down; where they do the attention leaves its outputs as they are and sets the same bit. */
 enum { SMELT_PAGED_F16 = 0, SMELT_PAGED_BF16 = 1 };
 typedef struct {
     int32_t precision;           /* of the pools, the queries and the outputs: SMELT_PAGED_* */

@@ -5,7 +5,7 @@
 namespace smelt {
 
 enum PagedType : int { kPagedF16 = 0, kPagedBf16 = 1 };
-enum : uint32_t { KERR_BAD_PAGE = 0x10000u };  // a page id outside the pool, or a row without a token of its own
+enum : uint32_t { KERR_BAD_PAGE = 0x10000u };  // a page id outside the pool, a row without a token of its own, or row starts that go down
 constexpr int kPagedSeqs = 1024;               // sequences of one call: their rows and lengths are held in shared memory
 
 constexpr int kPagedCtas = 256;                // of a line's kernel at most: the join has a thread for each
@@ -99,7 +99,7 @@ struct PagedLine {
     Divisor column_div;
     int ctas, workers;  // workers of a CTA
     int with_prefix, with_own, wide;
-    int32_t* cum;     // [n_seqs + 3] written by CTA 0: steps before each source, and the first prefix key that any row sees
+    int32_t* cum;     // [n_seqs + 3] written by CTA 0: steps before each source, and the first prefix key that any row sees (kDisordered: see paged_line.cuh)
     float* slot_o;    // [2 ctas][columns][D] weighted sums of items shared by several CTAs
     float2* slot_ml;  // [2 ctas][columns] their running maxima and sums
     PagedShared* shared;  // [ctas] the item that begins in a CTA and goes on behind it, for the join (tensor-core kernel without a prefix)

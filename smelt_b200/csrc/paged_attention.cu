@@ -638,7 +638,7 @@ __global__ void __launch_bounds__(kMergeWarps * 32) paged_merge_kernel(const __g
     pdl_trigger();
     pdl_wait();
     const int own_places = own.cum[c.n_seqs + 1], ahead_places = ahead.cum[c.n_seqs + 1], ahead_lo = ahead.cum[c.n_seqs + 2];  // (on their way while the sequence is looked for)
-    if (r >= c.rows || r >= first_row(c, c.n_seqs)) return;
+    if (ahead_lo == kDisordered || r >= c.rows || r >= first_row(c, c.n_seqs)) return;
     int start = 0;
     const int s = warp_find_seq(c.row_start, c.n_seqs, c.rows, r, &start);
     if (s < 0) return;

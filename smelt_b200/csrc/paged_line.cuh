@@ -6,6 +6,7 @@ namespace smelt {
 namespace paged {
 
 constexpr float kLowest = -3.402823466e38f;
+constexpr int kDisordered = -1;  // in the place of the first prefix key that any row sees: row starts that go down, nothing is computed
 
 struct Range { int lo, hi; };  // keys [lo, hi)
 
@@ -59,11 +60,23 @@ __device__ __forceinline__ void scan_line(const PagedArgs& c, const PagedLine& l
     b.row = b.cum + n + 2;
     b.length = b.row + n + 1;
     if (tid == 0) lowest = c.prefix_length;
+    bool down = false;
     for (int s = tid; s <= n; s += THREADS) {
         b.row[s] = first_row(c, s);
-        if (s < n) b.length[s] = tokens_of(c, s);
+        if (s < n) {
+            b.length[s] = tokens_of(c, s);
+            down |= first_row(c, s + 1) < b.row[s];
+        }
     }
-    __syncthreads();
+    // Starts that go down would give rows to several sequences, and their places could be more than are counted in 32 bits: nobody has rows then.
+    if (__syncthreads_or(down)) {
+        for (int s = tid; s <= n; s += THREADS) b.row[s] = 0;
+        if (tid == 0) {
+            lowest = kDisordered;
+            if (blockIdx.x == 0 && c.err) atomicOr(c.err, KERR_BAD_PAGE);
+        }
+        __syncthreads();
+    }
     const int per = (n + THREADS - 1) / THREADS, s0 = min(n, tid * per), s1 = min(n, s0 + per);
     int mine = 0;
     for (int s = s0; s < s1; ++s) {
@@ -81,7 +94,7 @@ __device__ __forceinline__ void scan_line(const PagedArgs& c, const PagedLine& l
     }
     if (lane == 31) warp_sums[warp] = run;
     __syncthreads();
-    b.prefix_lo = window ? lowest : 0;
+    b.prefix_lo = window || lowest < 0 ? lowest : 0;
     int before = run - mine;
     if (n > 32 * per)
         for (int w = 0; w < warp; ++w) before += warp_sums[w];

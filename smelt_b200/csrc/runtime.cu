@@ -210,7 +210,7 @@ smelt_status smelt_cuda_device_error(smelt_cuda_ctx* ctx, uint32_t* out_flags) {
     if (s) return s;
     if (*out_flags) {
         clear_after_timeout(ctx);
-        if (*out_flags == KERR_BAD_PAGE) return fail(ctx, SMELT_ERR_OUT_OF_RANGE, "a page id outside the pool, or a row without a token on its sequence's pages");
+        if (*out_flags == KERR_BAD_PAGE) return fail(ctx, SMELT_ERR_OUT_OF_RANGE, "a page id outside the pool, a row without a token on its sequence's pages, or row starts that go down");
         return fail(ctx, SMELT_ERR_DEVICE_TIMEOUT, "a kernel's bounded wait gave up (flags " + std::to_string(*out_flags) + ")");
     }
     return SMELT_OK;

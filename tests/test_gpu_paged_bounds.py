@@ -94,3 +94,23 @@ def test_drafts_behind_the_steps_of_a_draft_are_not_judged(ctx, kind, steps, t):
         want, full = cases.verify([0, cut], cases.from_bits(target, kind)[at], cases.from_bits(draft, kind)[:, s:s + 1], np.asarray(tokens)[at], [t], u)
         assert stood[s] == full[0] and np.array_equal(said[start[s]:start[s] + n], np.concatenate([want, np.full(n - cut, -1)])), (s, said, want)
     assert stood[0] == min(6, steps) and stood[5] == min(6, steps)
+
+
+@pytest.mark.parametrize("n_q,dim,rows", [(4, 64, 4), (32, 128, 40), (16, 256, 30)])  # streaming and tensor-core kernel
+@pytest.mark.parametrize("prefix,window", [(0, 0), (100, 0), (100, 60)])
+def test_row_starts_that_go_down_compute_nothing(ctx, n_q, dim, rows, prefix, window):
+    g = np.random.default_rng(dim + prefix)
+    b = cases.Batch(g, [rows] * 5, [rows + 50] * 5, 16, 2, dim, prefix=prefix)
+    k, v, tokens = b.fill(g, 0.0)
+    q = cases.rounded(g.standard_normal((b.total, n_q, dim)), "f16")
+    d = Device(ctx, b, "f16", n_q, k, v)
+    good = d.attend(q, 0.1, window)
+    for starts in ([0, 5 * rows, 0, 5 * rows, 0, 5 * rows], [0, rows, 2 * rows, 2 * rows - 1, 4 * rows, 5 * rows], [1, 0, 2, 3, 4, 5], [0, rows, 3 * rows, 4 * rows, 5 * rows, -(2 ** 31)]):
+        d.kept[0].upload(np.array(starts, np.int32))
+        assert (d.attend(q, 0.1, window) == 7.0).all()
+        assert ctx.device_error_flags() == 0x10000
+    d.kept[0].upload(np.minimum(b.start.astype(np.int64) * 2 ** 20, 2 ** 31 - 1).astype(np.int32))  # cut to the rows there are: all are the first sequence's, whose last tokens they are
+    d.attend(q, 0.1, window)
+    assert ctx.device_error_flags() == 0
+    d.kept[0].upload(b.start)
+    assert np.array_equal(d.attend(q, 0.1, window), good)
