@@ -876,7 +876,8 @@ SMELT_CUDA_API smelt_status smelt_cuda_paged_append(smelt_cuda_ctx* ctx, const s
  * its own, with a window (0: none) the last `window` of them.  A row that sees nothing
  * (a sequence with more rows than tokens) gets zeros.  out may be q.  The prefix is read once for all
  * sequences.  At most 1024 sequences.  The workspace (smelt_cuda_paged_attention_workspace bytes, 16-byte aligned) holds partial sums
- * during the call; its contents need no preparation; calls that may run at the same time need one each. */
+ * during the call; its contents need no preparation; calls that may run at the same time (of several contexts, or graphs that the caller
+ * captured from smelt_cuda_stream) need one each. */
 SMELT_CUDA_API smelt_status smelt_cuda_paged_attention_workspace(smelt_cuda_ctx* ctx, const smelt_paged_cache* cache,
                                                                  const smelt_paged_batch* batch, size_t* out_bytes);
 SMELT_CUDA_API smelt_status smelt_cuda_paged_attention(smelt_cuda_ctx* ctx, const smelt_paged_cache* cache, const smelt_paged_batch* batch,

@@ -108,7 +108,7 @@ struct PagedAttentionArgs {
     PagedArgs c;
     PagedLine line[2];  // one or two launches' work
     int lines, prefix_line, own_line;  // which of them has the prefix (-1: none), and which the sequences
-    int* counters;      // [ctas], zero between launches: the last CTA of a shared item joins its parts; null: a launch of the join does
+    int* counters;      // [ctas], zero at a launch's beginning and end: the last CTA of a shared item joins its parts; null: a launch of the join does
     float *whole_o;     // [2][rows n_q][D] items that one CTA finishes, beside a prefix: 0 of the sequences, 1 of the prefix
     float2* whole_ml;
     const void* q;

@@ -96,7 +96,7 @@ size_t attention_plan(const smelt_cuda_ctx* ctx, const smelt_paged_cache* k, con
     };
     if (prefix == 0) {
         add(own_wide, true, false);
-        if (!own_wide) a->counters = ctx->paged_counters;  // few sums: the kernel joins them itself
+        if (!own_wide) a->counters = (int*)room((size_t)a->line[0].ctas * sizeof(int));  // few sums: the kernel joins them itself
     } else if (own_wide == prefix_wide) {
         add(own_wide, true, true);
     } else {
@@ -215,6 +215,18 @@ smelt_status smelt_cuda_paged_attention(smelt_cuda_ctx* ctx, const smelt_paged_c
     a.scale2 = scale * 1.4426950408889634f;
     a.window = window < 0x7fffffffu ? window : 0;  // positions are below that
     cudaError_t e = cudaSuccess;
+    if (a.counters) {
+        // Calls on the context's stream follow one another, and so do replays of its own capture: they share its counters, which every call
+        // leaves at zero.  A graph that the caller captures from the stream may run beside them: it counts in its workspace.
+        cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+        if (!ctx->capturing) e = cudaStreamIsCapturing(l.stream, &capture);
+        if (e == cudaSuccess && capture == cudaStreamCaptureStatusActive) {
+            e = cudaMemsetAsync(a.counters, 0, (size_t)a.line[0].ctas * sizeof(int), l.stream);
+            l.pdl = false;  // the kernel follows the memset
+        } else {
+            a.counters = ctx->paged_counters;
+        }
+    }
     for (int i = 0; i < a.lines && e == cudaSuccess; ++i) e = (a.line[i].wide ? launch_paged_wide : launch_paged_narrow)(l, (PagedType)cache->precision, cache->head_dim, a, i);
     if (e == cudaSuccess && !a.counters) e = (a.whole_o ? launch_paged_merge : launch_paged_join)(l, (PagedType)cache->precision, cache->head_dim, a);
     return check_cuda(ctx, e, "paged attention");

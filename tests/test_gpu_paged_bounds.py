@@ -114,3 +114,44 @@ def test_row_starts_that_go_down_compute_nothing(ctx, n_q, dim, rows, prefix, wi
     assert ctx.device_error_flags() == 0
     d.kept[0].upload(b.start)
     assert np.array_equal(d.attend(q, 0.1, window), good)
+
+
+def test_graphs_that_the_caller_captures_run_side_by_side(ctx):
+    """Two calls captured from the context's stream, each with a workspace of its own, replayed on two streams, and eager calls beside them."""
+    torch = pytest.importorskip("torch")
+    g = np.random.default_rng(51)
+    calls = []
+    for lengths, n_q in (([600], 8), ([900, 40, 3], 4), ([500, 2], 8)):
+        b = cases.Batch(g, [1] * len(lengths), lengths, 16, 2, 128)
+        k, v, _ = b.fill(g, 0.0)
+        q = cases.rounded(g.standard_normal((b.total, n_q, 128)), "f16")
+        d = Device(ctx, b, "f16", n_q, k, v)
+        want = d.attend(q, 0.1)
+        dq, out = ctx.to_device(np.float16(q)), ctx.to_device(np.full(q.shape, 7, np.float16))
+        work, size = d.workspace()
+        args = (C.byref(d.cache), C.byref(d.batch), dq.ptr, n_q * 128, out.ptr, n_q * 128, 0.1, 0, work.ptr, size)
+        calls.append((args, out, want, (d, dq, work)))
+    torch.cuda.set_device(0)
+    torch.zeros(1, device="cuda")
+    own = torch.cuda.ExternalStream(ctx.lib.smelt_cuda_stream(ctx.h))
+    graphs, sides = [], [torch.cuda.Stream(), torch.cuda.Stream()]
+    for args, _, _, _ in calls[:2]:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.stream(own):
+            graph.capture_begin(capture_error_mode="thread_local")
+            ctx.call("paged_attention", *args)
+            graph.capture_end()
+        graphs.append(graph)
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for _, out, want, _ in calls:
+            out.upload(np.full(want.shape, 7, np.float16))
+        for _ in range(10):
+            for graph, side in zip(graphs, sides):
+                with torch.cuda.stream(side):
+                    graph.replay()
+            ctx.call("paged_attention", *calls[2][0])
+        torch.cuda.synchronize()
+        for _, out, want, _ in calls:
+            assert np.array_equal(out.download(np.float16, want.shape).astype(np.float64), want)
+    del graphs
