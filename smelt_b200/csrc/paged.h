@@ -26,7 +26,7 @@ __device__ __forceinline__ float exp2_approx(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-// Two fp32 values side by side, and both operations on them in one instruction.
+// Two fp32 values side by side, and an operation on both of them in one instruction.
 __device__ __forceinline__ uint64_t pair_of(float x, float y) {
     uint64_t v;
     asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(x), "f"(y));
@@ -36,6 +36,11 @@ __device__ __forceinline__ void split(uint64_t v, float& x, float& y) { asm("mov
 __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
     uint64_t v;
     asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(a), "l"(b), "l"(c));
+    return v;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t v;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
     return v;
 }
 __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {

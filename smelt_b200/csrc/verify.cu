@@ -208,21 +208,20 @@ __global__ void __launch_bounds__(kStatThreads) verify_stats_kernel(const Verify
             if (mine.top != kNone) mine.sum *= exp2_approx((mine.top - top) * scale);
             mine.top = top;
         }
-        const float minus = -mine.top * scale;
-        const uint64_t scales = pair_of(scale, scale), minuses = pair_of(minus, minus);
+        // (the difference first: the logits' products with 1 / T would be rounded by as much as the whole argument at a small T)
+        const uint64_t scales = pair_of(scale, scale), minus = pair_of(-mine.top, -mine.top);
         uint64_t sums = 0ull;
 #pragma unroll
         for (int i = 0; i < K; ++i)
 #pragma unroll
             for (int e = 0; e < N; e += 2) {
                 float y0, y1;
-                split(fma2(pair_of(v[i][e], v[i][e + 1]), scales, minuses), y0, y1);
+                split(mul2(add2(pair_of(v[i][e], v[i][e + 1]), minus), scales), y0, y1);
                 sums = add2(sums, pair_of(exp2_approx(y0), exp2_approx(y1)));
             }
         float sum[2];
         split(sums, sum[0], sum[1]);
         sum[0] += sum[1];
-        sum[0] = fmaf(-0.69314718f * fmaf(mine.top, scale, minus), sum[0], sum[0]);  // what `minus` was rounded by, which every term has
         if (sum[0] != sum[0]) {  // NaN counts as masked; infinities that are the largest share what there is
             sum[0] = 0.f;
 #pragma unroll

@@ -155,3 +155,46 @@ def test_graphs_that_the_caller_captures_run_side_by_side(ctx):
         for _, out, want, _ in calls:
             assert np.array_equal(out.download(np.float16, want.shape).astype(np.float64), want)
     del graphs
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("t", [1e-2, 1e-3, 1e-4, 1e-5, 1e-6, 1e-8, 1e-30, 1e-40])
+@pytest.mark.parametrize("drafted", [True, False])
+def test_small_temperatures(ctx, kind, t, drafted):
+    """Almost greedy: a draft that is the only likely token of both models stands, whatever u below 1, and so does the draw."""
+    g = np.random.default_rng(61)
+    rows, V = [4] * 40, 4099
+    start, target, draft, tokens, temperature, random = verify_case(g, "f32", rows, V)
+    target, draft = np.minimum(target, 6.0), np.minimum(draft, 6.0)
+    for r in range(int(start[-1])):  # one token far above the rest, at any height
+        target[r, tokens[r + 1] if r + 1 < len(tokens) else 0] = g.uniform(8, 30)
+    for s, n in enumerate(rows):
+        for j in range(n - 1):
+            draft[j, s, tokens[start[s] + j + 1]] = g.uniform(8, 30)
+        tokens[start[s]] = 0
+    target[3::4] = np.minimum(target[3::4], 6.0)
+    for r in range(3, int(start[-1]), 4):
+        target[r, g.integers(0, V)] = g.uniform(8, 30)
+    random[:] = np.float32(1) - np.float32(2.0 ** -24)
+    random[3::4] = g.random(40)  # the draw's
+    target, draft = cases.to_bits(target, kind), cases.to_bits(draft, kind)
+    temperature[:] = t
+    out, kept = check_verify(ctx, kind, start, target, draft if drafted else None, tokens, temperature, random)
+    assert (kept == 3).all() and np.array_equal(out.reshape(40, 4)[:, :3], np.asarray(tokens).reshape(40, 4)[:, 1:])
+
+
+@pytest.mark.parametrize("t", [1e-3, 1e-6])
+def test_small_temperatures_share_what_is_close(ctx, t):
+    """Two tokens a fraction of T apart at the height where T is far below a logit's last place in the product with 1 / T."""
+    g = np.random.default_rng(62)
+    V, n = 1000, 64
+    target = np.full((2 * n, V), -50.0, np.float32)
+    step = np.float32(2.0 ** -20) if t < 1e-4 else np.float32(2.0 ** -11)
+    target[:, 10], target[:, 700] = np.float32(13.0), np.float32(13.0) + step  # exact in fp32
+    chance = 1 / (1 + np.exp(-float(step) / float(np.float32(t))))  # of token 700
+    random = np.repeat(np.linspace(0.01, 0.99, n), 2).astype(np.float32)
+    assert np.abs(random - chance).min() > 1e-5  # none within the error of fp32 sums
+    tokens = np.tile([0, 700], n)
+    start = np.arange(0, 2 * n + 1, 2)
+    out, kept = check_verify(ctx, "f32", start, target, None, tokens, np.full(n, t, np.float32), random)
+    assert np.array_equal(kept, (random[0::2] < chance).astype(np.int32))
