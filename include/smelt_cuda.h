@@ -874,7 +874,8 @@ SMELT_CUDA_API smelt_status smelt_cuda_paged_append(smelt_cuda_ctx* ctx, const s
                                                     int64_t k_stride, const void* v_dev, int64_t v_stride, void* q_out_dev, int64_t q_out_stride);
 /* Attention of the batch's rows over the prefix and the sequences' own pages: row i of n of a sequence sees the positions up to
  * its own, with a window (0: none) the last `window` of them.  A row that sees nothing
- * (a sequence with more rows than tokens) gets zeros.  out may be q.  The prefix is read once for all
+ * (a sequence with more rows than tokens) gets zeros.  Keys and values that are not finite reach the rows that see them alone: an infinite
+ * value makes their sums infinite (NaN: with one of the other sign, or with NaN).  out may be q.  The prefix is read once for all
  * sequences.  At most 1024 sequences.  The workspace (smelt_cuda_paged_attention_workspace bytes, 16-byte aligned) holds partial sums
  * during the call; its contents need no preparation; calls that may run at the same time (of several contexts, or graphs that the caller
  * captured from smelt_cuda_stream) need one each. */

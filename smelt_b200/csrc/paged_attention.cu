@@ -12,7 +12,8 @@
 // items, and while one warp writes down an item or waits for the next one's queries the others keep the memory busy.  At the end the
 // CTA joins what its warps have of the same item.
 // P goes into the product as two 16-bit parts: the kernel waits for memory, and rounding P once would cost up to half a step of the
-// 16-bit type.  Keys outside an item are not read (zeros), and a value row that is not finite reaches only the columns that see it.
+// 16-bit type.  Keys outside an item are not read (zeros), and a value row that is not finite reaches only the columns that see it; where an
+// item's sums come out not finite, what infinite values make of them is put in afterwards (a part of P that is 0 times one is NaN).
 // What several CTAs have of an item the last of them joins; with a prefix paged_merge_kernel does, behind the tensor-core kernel paged_join_kernel.
 //
 // Memory bounds it from some tens of MB on: 819 MB of two long sequences in 150 us (5.4 TB/s), 416 MB of a ragged batch in 82 (5.1 TB/s; a
@@ -90,6 +91,35 @@ __device__ __noinline__ void weighted_sum_masked(uint32_t values, MaskedTile<D, 
                 if ((col >> 1) == t) { m.o[nh][i][col & 1] += add[col & 1]; m.o[nh][i][2 + (col & 1)] += add[2 + (col & 1)]; }
             }
         }
+}
+
+// Writes what an item's sums are where a value that a column sees is not finite, over what the warp has just written of the item: parts (part: [columns][D + 1]),
+// sums beside a prefix or outputs.  In a function of its own and through memory, so that the sums' registers are not kept for it.
+template <int D, int NH, class E>
+__device__ __noinline__ void put_infinities(const PagedAttentionArgs& a, float* part, int source, int head, int row, int f0, int width, int from, int to, Range k0, Range k1, Range k2, Range k3) {
+    const PagedArgs& c = a.c;
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int32_t* table = source == 0 ? c.prefix_table : c.table + (size_t)(source - 1) * c.table_stride;
+    Infinite<2 * NH> found;
+    found.seen[0] = k0;
+    found.seen[1] = k1;
+    if constexpr (NH == 2) { found.seen[2] = k2; found.seen[3] = k3; }
+    __syncwarp();
+    for (int x = 0; x < D; x += 32) {
+        look_for_infinities<E>(c, table, static_cast<const E*>(c.v) + (long long)head * c.head_stride + x, from, to, found);
+        for (int col = 0; col < 2 * NH; ++col) {
+            const int f = (col >> 1) * 8 + 2 * t + (col & 1), i = divide(f0 + f, c.ratio_div);
+            if (f >= width) continue;
+            const size_t out_head = head * c.ratio + f0 + f - i * c.ratio;
+            for (int e = g; e < 32; e += 8) {
+                if (!((found.pos[col] | found.neg[col]) >> e & 1u)) continue;
+                const float v = found.sum(col, e, 0.f);
+                if (part) part[f * (D + 1) + x + e] = v;
+                else if (a.whole_o) a.whole_o[(((source == 0 ? (size_t)c.rows : 0) + row + i) * c.n_q + out_head) * D + x + e] = v;
+                else static_cast<E*>(a.out)[(size_t)(row + i) * a.out_stride + out_head * D + x + e] = round_to<E>(v);
+            }
+        }
+    }
 }
 
 template <int D> struct Sums { float v[D / 32]; };
@@ -485,6 +515,14 @@ __global__ void __launch_bounds__(kWarps<D> * 32, 1) paged_narrow_kernel(const _
         }
 
         // ── the item's sums ──
+        float odd[4] = {0.f, 0.f, 0.f, 0.f};  // NaN where a sum is not finite
+#pragma unroll
+        for (int nh = 0; nh < NH; ++nh)
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) odd[e] = fmaf(o[nh][i][e], 0.f, odd[e]);
+        const bool infinite = __any_sync(0xffffffffu, odd[0] + odd[1] + odd[2] + odd[3] != 0.f);
 #pragma unroll
         for (int nh = 0; nh < NH; ++nh)
 #pragma unroll
@@ -534,6 +572,11 @@ __global__ void __launch_bounds__(kWarps<D> * 32, 1) paged_narrow_kernel(const _
                     if (f < width) *reinterpret_cast<uint32_t*>(to + 8 * k) = w;
                 }
             }
+        }
+        if (infinite) {  // (worked out again, so that nothing more is kept over the item's steps)
+            const Range of = item.source == 0 ? Range{batch.prefix_lo, c.prefix_length} : block_keys(c, line, seq_of(item.source), item.block, a.window);
+            put_infinities<D, NH, E>(a, before ? fronts + warp * C * (D + 1) : behind ? reinterpret_cast<float*>(ring) : nullptr, item.source, item.head, seq.row, f0, width,
+                                     max((of.lo / kTile + max(begin - item_at, 0)) * kTile, of.lo), min(k0 + kTile, of.hi), keys[0][0], keys[0][1], keys[NH - 1][0], keys[NH - 1][1]);
         }
     }
     cp_async_wait<0>();

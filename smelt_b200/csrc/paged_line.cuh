@@ -1,5 +1,7 @@
 // Device side of the line of work of the paged attention kernels (PagedLine in paged.h).
 #pragma once
+#include <type_traits>
+
 #include "paged.h"
 
 namespace smelt {
@@ -202,6 +204,54 @@ __device__ __forceinline__ int seq_of_row(const Batch& b, int n_seqs, int row) {
         else hi = mid - 1;
     }
     return lo;
+}
+
+// Infinite values.  A weight times an infinite value is infinite, but weights reach the products in 16 bits, in parts or rounded, and a part that is
+// zero makes NaN of it.  Where an item's sums are not finite its values are looked through again (a whole warp calls it): the 32 values from
+// `values` on (in the pool's first token of the key head) of the keys [from, to), a key a lane.  pos and neg: bit e where value e of a key that the lane's column
+// i sees is +infinity or -infinity, both where it is NaN.
+template <int COLS> struct Infinite {
+    Range seen[COLS];
+    uint32_t pos[COLS], neg[COLS];
+    // What the sum over the keys is: as it is, where all values are finite.
+    __device__ __forceinline__ float sum(int col, int e, float finite) const {
+        const bool p = pos[col] >> e & 1u, n = neg[col] >> e & 1u;
+        return p ? (n ? __uint_as_float(0x7FC00000u) : INFINITY) : n ? -INFINITY : finite;
+    }
+};
+template <class E, int COLS>
+__device__ __forceinline__ void look_for_infinities(const PagedArgs& c, const int32_t* table, const E* values, int from, int to, Infinite<COLS>& found) {
+    constexpr uint32_t kInf = std::is_same<E, __half>::value ? 0x7C00u : 0x7F80u;
+    const int lane = threadIdx.x & 31;
+    for (int i = 0; i < COLS; ++i) found.pos[i] = found.neg[i] = 0;
+    for (int base = from; base < to; base += 32) {
+        const int key = base + lane;
+        uint32_t p = 0, n = 0;
+        if (key < to) {
+            const int at = divide(key, c.page_div), page = table[at];
+            if ((uint32_t)page < (uint32_t)c.n_pages) {
+                const uint4* row = reinterpret_cast<const uint4*>(values + (long long)page * c.page_stride + (long long)(key - at * c.page_size) * c.token_stride);
+                for (int i = 0; i < 4; ++i) {
+                    const uint4 w = row[i];
+                    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const uint32_t v = u[e >> 1] >> (16 * (e & 1)) & 0xffffu;
+                        if ((v & kInf) != kInf) continue;
+                        const bool nan = v & (0x7fffu & ~kInf);
+                        if (nan || !(v & 0x8000u)) p |= 1u << (8 * i + e);
+                        if (nan || (v & 0x8000u)) n |= 1u << (8 * i + e);
+                    }
+                }
+            }
+        }
+        for (uint32_t some = __ballot_sync(0xffffffffu, p | n); some; some &= some - 1u) {
+            const int from_lane = __ffs(some) - 1, k = base + from_lane;
+            const uint32_t pk = __shfl_sync(0xffffffffu, p, from_lane), nk = __shfl_sync(0xffffffffu, n, from_lane);
+            for (int i = 0; i < COLS; ++i)
+                if (k >= found.seen[i].lo && k < found.seen[i].hi) { found.pos[i] |= pk; found.neg[i] |= nk; }
+        }
+    }
 }
 
 }  // namespace paged

@@ -17,7 +17,8 @@
 // tokens in 122, where an item of six steps costs as much again for its beginning and end (lookups and first loads, the masked step, the sums).
 //
 // Value rows that are not finite and that not every column of the step sees are taken out of the product (as zeros) and added
-// for the columns that see them alone, so that nothing reaches a row that it does not see.
+// for the columns that see them alone, so that nothing reaches a row that it does not see.  An fp16 weight may round to 0, and 0 times infinity is
+// NaN: where fp16 sums come out not finite, what infinite values make of them is put in afterwards.
 #include <cuda_bf16.h>
 
 #include <type_traits>
@@ -728,6 +729,20 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_wide_kernel(const _
 #pragma unroll
                         for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) + joint[e * 128 + me]);
                     barrier(2, 256);
+                }
+                if constexpr (std::is_same<E, __half>::value) {  // (a bf16 weight is zero only where the fp32 one is)
+                    float odd[4] = {0.f, 0.f, 0.f, 0.f};  // NaN where a sum is not finite
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) odd[e & 3] = fmaf(__uint_as_float(v[e]), 0.f, odd[e & 3]);
+                    if (__any_sync(0xffffffffu, write && odd[0] + odd[1] + odd[2] + odd[3] != 0.f)) {
+                        Infinite<1> found;
+                        found.seen[0] = keys;
+                        look_for_infinities<E>(c, cur.source == 0 ? c.prefix_table : c.table + (size_t)(cur.source - 1) * c.table_stride,
+                                               static_cast<const E*>(c.v) + (long long)cur.head * c.head_stride + x, max((cur.first + cur.step) * KEYS, cur.keys.lo),
+                                               min((cur.first + cur.step + n) * KEYS, cur.keys.hi), found);
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(found.sum(0, e, __uint_as_float(v[e])));
+                    }
                 }
                 if (!write) continue;
                 if (part) {

@@ -198,3 +198,47 @@ def test_small_temperatures_share_what_is_close(ctx, t):
     start = np.arange(0, 2 * n + 1, 2)
     out, kept = check_verify(ctx, "f32", start, target, None, tokens, np.full(n, t, np.float32), random)
     assert np.array_equal(kept, (random[0::2] < chance).astype(np.int32))
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("n_q,n_kv,dim,rows", [(2, 2, 64, 1), (10, 1, 64, 1), (8, 2, 128, 2), (4, 1, 128, 4), (4, 1, 256, 2), (8, 2, 64, 40), (16, 2, 128, 33), (40, 1, 256, 5)])
+@pytest.mark.parametrize("prefix,window", [(0, 0), (300, 0), (300, 500)])
+def test_infinite_values_that_a_row_sees(ctx, kind, n_q, n_kv, dim, rows, prefix, window):
+    """A weight times an infinite value is infinite, however small the weight is and however many CTAs have a part of the item; infinities of both
+    signs, or what is not a number, give NaN; every other value of the row stays what it is."""
+    g = np.random.default_rng(dim + rows + prefix)
+    b = cases.Batch(g, [rows, rows, 1], [rows + 700, rows + 3, 150], 16, n_kv, dim, prefix=prefix)
+    k, v, tokens = b.fill(g, np.nan)
+    tokens = [cases.rounded(t, kind) for t in tokens]
+    odd = [np.zeros(t[1].shape) for t in tokens]  # what is not finite of every sequence's values
+
+    def put(s, t, head, d, x):
+        p, slot = (b.prefix_table[t // 16], t % 16) if t < prefix else b.place(s, t - prefix)
+        v[p, head, slot, d] = x
+        for o in odd if t < prefix else odd[s:s + 1]:
+            o[t, head, d] = x
+
+    far = prefix + b.lengths[0]
+    for n, (t, x) in enumerate([(far - rows, np.inf), (far - 1, -np.inf), (far - rows - 1, np.nan), (prefix + 5, np.inf), (prefix + 400, -np.inf), (prefix + 128, np.inf), (prefix + 131, np.inf)]):
+        put(0, t, n % n_kv, 3 * n + 1, x)
+    for t, x in ((prefix + 300, np.inf), (prefix + 301, -np.inf)):
+        put(0, t, 0, dim - 1, x)
+    put(1, prefix + 1, 0, 7, -np.inf)  # in front of every row of the second sequence
+    if prefix:
+        put(0, 17, 0, 40, np.inf), put(0, 299, 0, 41, np.nan), put(0, 250, n_kv - 1, dim - 2, -np.inf)
+    q = cases.rounded(g.standard_normal((b.total, n_q, dim)), kind)
+    scale = np.float32(4 / np.sqrt(dim))  # weights from 1 down to 2^-40 and below
+    with np.errstate(invalid="ignore"):
+        got = Device(ctx, b, kind, n_q, k, v).attend(q, scale, window)
+        clean = [np.stack([t[0], np.where(o == 0, t[1], 0)]) for t, o in zip(tokens, odd)]
+        want, size, reach = cases.attend(b, clean, q, scale, window)
+        bound = cases.attend_bound(want, size, reach, kind, dim)
+        for s, n in enumerate(b.rows):
+            for i in range(n):
+                at = prefix + b.lengths[s] - n + i
+                seen = odd[s][max(0, at + 1 - window) if window else 0:at + 1].repeat(n_q // n_kv, 1)
+                bad = np.where(seen == 0, 0, seen).sum(0)  # finite: 0
+                r = b.start[s] + i
+                assert np.array_equal(np.isnan(got[r]), np.isnan(bad)) and np.array_equal(got[r][np.isinf(bad)], bad[np.isinf(bad)]), (s, i)
+                fine = bad == 0
+                assert (np.abs(got[r] - want[r]) <= bound[r])[fine].all()
