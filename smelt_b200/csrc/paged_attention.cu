@@ -50,6 +50,9 @@ __device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], uint32_t at) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
 }
 constexpr uint32_t kHidden = 0x7FFFF00Du;  // a NaN of our own
+// The largest weight is two to this power: an fp16 weight loses bits below 2^-14, and what many small ones add up to would be lost with them (a key
+// that takes nearly all of the weight in front of thousands).  bf16 goes as far down as fp32.
+template <class E> constexpr float kAbove = std::is_same<E, __half>::value ? 14.f : 0.f;
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory"); }
 __device__ __forceinline__ void cp_async16_or_zero(uint32_t dst, const void* src, bool take) {
@@ -428,7 +431,10 @@ __global__ void __launch_bounds__(kWarps<D> * 32, 1) paged_narrow_kernel(const _
 #pragma unroll
                 for (int nh = 0; nh < NH; ++nh)
 #pragma unroll
-                    for (int x = 0; x < 2; ++x) moved = moved || top[nh][x] > m_run[nh][x];
+                    for (int x = 0; x < 2; ++x) {
+                        top[nh][x] -= kAbove<E>;
+                        moved = moved || top[nh][x] > m_run[nh][x];
+                    }
                 if (__any_sync(0xffffffffu, moved)) {  // a new maximum: rare behind the first tiles
 #pragma unroll
                     for (int nh = 0; nh < NH; ++nh)

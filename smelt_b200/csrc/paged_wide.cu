@@ -7,7 +7,7 @@
 // a column, so the softmax needs no exchange.  P overwrites S in tensor memory and is the product's operand from there.  While one
 // set is at its exponentials (128 x 128 of them take the SM's 16 a clock 1024 clocks) the tensor core works for the other (1024 clocks a
 // tile and step).  A block of 128 columns or fewer gives both sets the same tile and every other step, and their sums are joined at the
-// end.  The maximum that P is relative to is the first step's, and moves only when a step's weights add up to more than 2^10: O is rescaled
+// end.  The maximum that P is relative to is the first step's, and moves only when a step's weights add up to more than 2^10 times the first step's largest: O is rescaled
 // a few times an item at most, and behind the first step nobody looks for a maximum (1500 rows over 20000 tokens: 594 us with it, 542 without).
 // P is rounded once to the 16-bit type, the type of the values it is multiplied with; sums are fp32.
 //
@@ -550,10 +550,16 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_wide_kernel(const _
                 const float top = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
                 return top == kLowest ? kLowest : top * scale2;
             };
-            if (!begun) m = largest();
+            // An item's largest weights are 2^kAbove: fp16 loses bits below 2^-14, and with them what many small weights add up to.
+            constexpr float kAbove = std::is_same<E, __half>::value ? 6.f : 0.f;
+            if (!begun) {
+                const float top = largest();
+                m = top == kLowest ? kLowest : top - kAbove;
+            }
             // Behind an item's first task the weights are relative to the maximum so far: the new one is looked for only where their sum is past
-            // 2^10, and the task is done again.  Until then no weight is above 2^10, which either 16-bit type holds as well as 1.
-            constexpr float kMost = 1024.f;
+            // 1024 of the largest ones (what fp16 holds), and the task is done again.  Until then no weight is above that sum, which either
+            // 16-bit type holds as well as 1, and a flat task's 128 of the largest ones stay below it.
+            constexpr float kMost = std::is_same<E, __half>::value ? 65504.f : 1024.f;
             float added;
             auto exponentials = [&] {
                 const uint64_t scales = pair_of(scale2, scale2), minus = pair_of(-m, -m);
@@ -577,8 +583,8 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_wide_kernel(const _
             };
             exponentials();
             if (begun && __any_sync(0xffffffffu, added > kMost)) {
-                const float top = largest();
-                const bool move = added > kMost;  // at least one weight is above 8, so top is above m
+                const float top = largest() - kAbove;
+                const bool move = added > kMost;  // at least one weight is above 7 of the largest ones so far, so top is above m
                 const float keep = move ? exp2_approx(m - top) : 1.f;
                 if (move) m = top;
                 l *= keep;

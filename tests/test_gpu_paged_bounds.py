@@ -242,3 +242,36 @@ def test_infinite_values_that_a_row_sees(ctx, kind, n_q, n_kv, dim, rows, prefix
                 assert np.array_equal(np.isnan(got[r]), np.isnan(bad)) and np.array_equal(got[r][np.isinf(bad)], bad[np.isinf(bad)]), (s, i)
                 fine = bad == 0
                 assert (np.abs(got[r] - want[r]) <= bound[r])[fine].all()
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("n_q,n_kv,dim,rows,below", [(4, 2, 64, 1, 10.0), (4, 2, 64, 1, 17.0), (12, 1, 128, 1, 14.0), (4, 1, 256, 2, 17.0), (8, 2, 64, 6, 10.0), (8, 2, 128, 6, 13.0), (16, 2, 256, 3, 13.0)])
+@pytest.mark.parametrize("prefix", [0, 200])
+def test_many_small_weights_behind_a_large_one(ctx, kind, n_q, n_kv, dim, rows, below, prefix):
+    """The first key takes nearly all of the weight and has no value: what is left of the output is what thousands of weights of e^-below add up to."""
+    g = np.random.default_rng(dim + rows)
+    b = cases.Batch(g, [rows, 1], [rows + 1500, 30], 16, n_kv, dim, prefix=prefix)
+    k, v, tokens = b.fill(g, 0.0)
+    q = np.full((b.total, n_q, dim), 1.0)
+    for pool in [k, v]:
+        pool[:] = 0
+    tokens = [t * 0 for t in tokens]
+
+    def put(s, t, key, value):
+        p, slot = (b.prefix_table[t // 16], t % 16) if t < prefix else b.place(s, t - prefix)
+        k[p, :, slot], v[p, :, slot] = key, value
+        for u in tokens if t < prefix else [tokens[s]]:
+            u[0, t], u[1, t] = key, value
+
+    for s in range(2):
+        for t in range(prefix if s else 0, prefix + b.lengths[s]):
+            put(s, t, 0.0, float(1 + t % 3))
+        if s == 0 or not prefix:
+            put(s, 0, 1.0, 0.0)
+    check = Device(ctx, b, kind, n_q, k, v)
+    scale = np.float32(below / dim)
+    got = check.attend(q, scale)
+    want, size, reach = cases.attend(b, tokens, q, scale)
+    # a score is exact but for its product with the scale and log2(e), 2^-23 of `below` each; all else as everywhere
+    off = np.abs(got - want) - cases.attend_bound(want, size, reach, kind, dim)
+    assert off.max() <= 0, (off.max(), got[0, 0, 0], want[0, 0, 0])
