@@ -843,7 +843,8 @@ typedef struct {
 } smelt_paged_cache;
 typedef struct {
     int32_t n_seqs, rows;        /* rows: what the row arrays hold */
-    int32_t max_rows;            /* the most rows of one sequence, as far as the host knows: decides how the work is cut, not what is computed */
+    int32_t max_rows;            /* the most rows of one sequence, as far as the host knows; 0: one.  Decides how the work is cut and which kernel takes
+                                  * it, so that outputs differ in their last bits, whatever the sequences have (see smelt_cuda_paged_attention) */
     int32_t table_stride;        /* pages a row of the table holds */
     int32_t prefix_length;
     const void *row_start, *length, *table, *prefix_table; /* device, int32: [n_seqs + 1], [n_seqs], [n_seqs, table_stride], [prefix pages] */
@@ -873,12 +874,15 @@ SMELT_CUDA_API smelt_status smelt_cuda_paged_append(smelt_cuda_ctx* ctx, const s
                                                     const smelt_rope_desc* rope, const void* q_dev, int64_t q_stride, const void* k_dev,
                                                     int64_t k_stride, const void* v_dev, int64_t v_stride, void* q_out_dev, int64_t q_out_stride);
 /* Attention of the batch's rows over the prefix and the sequences' own pages: row i of n of a sequence sees the positions up to
- * its own, with a window (0: none) the last `window` of them.  A row that sees nothing
- * (a sequence with more rows than tokens) gets zeros.  Keys and values that are not finite reach the rows that see them alone: an infinite
- * value makes their sums infinite (NaN: with one of the other sign, or with NaN).  out may be q.  The prefix is read once for all
- * sequences.  At most 1024 sequences.  The workspace (smelt_cuda_paged_attention_workspace bytes, 16-byte aligned) holds partial sums
- * during the call; its contents need no preparation; calls that may run at the same time (of several contexts, or graphs that the caller
- * captured from smelt_cuda_stream) need one each. */
+ * its own, with a window (0: none) the last `window` of them.  A row that sees nothing (a sequence with more rows than tokens) gets
+ * zeros.  Keys and values that are not finite reach the rows that see them alone: an infinite value makes their sums infinite (NaN: with
+ * one of the other sign, or with NaN).  out may be q.  The prefix is read once for all sequences.  At most 1024 sequences.
+ * Scores, maxima and sums are fp32.  Weights are multiplied with the values in two 16-bit parts while max_rows n_q / n_kv is at most 16
+ * (8 with heads of 256); beyond that, and over a long prefix (how long goes by rows and the GPU's size), they are rounded once to
+ * the type of the pools, and outputs are up to 1.35 times as far from the exact ones.
+ * The workspace (smelt_cuda_paged_attention_workspace bytes, 16-byte aligned) holds partial sums during the call; its contents need no
+ * preparation; calls that may run at the same time (of several contexts, or graphs that the caller captured from smelt_cuda_stream)
+ * need one each. */
 SMELT_CUDA_API smelt_status smelt_cuda_paged_attention_workspace(smelt_cuda_ctx* ctx, const smelt_paged_cache* cache,
                                                                  const smelt_paged_batch* batch, size_t* out_bytes);
 SMELT_CUDA_API smelt_status smelt_cuda_paged_attention(smelt_cuda_ctx* ctx, const smelt_paged_cache* cache, const smelt_paged_batch* batch,
@@ -892,6 +896,8 @@ SMELT_CUDA_API smelt_status smelt_cuda_paged_attention(smelt_cuda_ctx* ctx, cons
  * random[row_start[s + 1] - 1] times the whole.  Without draft logits (null) a draft counts as certain: q(x) = 1.
  * T = temperature[s] (null: 1); 0 or less takes the lowest index of the largest logit and accepts drafts that are it.
  * Logits of -inf or NaN have no chance; a drafted id outside the vocabulary falls.
+ * Whether a draft stands is judged with fp32 sums: u q(x) within about 1e-6 of p(x), relative, may fall either way.  What is drawn goes by
+ * fp64 weights and sums; a whole of max(p - q, 0) below 1e-12 is what equal chances differ by, and counts as nothing.
  * row_start is read on the device: where it may give a sequence more drafts than `draft` has steps, draft_steps says how many there
  * are, and the drafts behind them are not judged: the token behind the last judged one that stands is drawn from p of its row.
  * Leaves out_tokens[row_start[s] + i] = the accepted drafts, the drawn token (-1 where no token has a chance), then -1, and accepted[s]. */
