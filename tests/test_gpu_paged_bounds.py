@@ -5,6 +5,7 @@ import numpy as np
 import pytest
 
 import paged_cases as cases
+import paged_pairs as pairs
 from smelt_b200 import capi
 from test_gpu_paged import CODE, LOGITS, WORD, Device, check_append, check_attention, check_verify, run_verify, verify_case  # noqa: F401
 
@@ -275,3 +276,60 @@ def test_many_small_weights_behind_a_large_one(ctx, kind, n_q, n_kv, dim, rows, 
     # a score is exact but for its product with the scale and log2(e), 2^-23 of `below` each; all else as everywhere
     off = np.abs(got - want) - cases.attend_bound(want, size, reach, kind, dim)
     assert off.max() <= 0, (off.max(), got[0, 0, 0], want[0, 0, 0])
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("n_q,n_kv,dim,rows", [(4, 2, 64, 2), (16, 1, 64, 1), (4, 1, 128, 2), (8, 2, 128, 4), (8, 1, 256, 1)])
+@pytest.mark.parametrize("prefix", [0, 12])
+def test_streamed_weights_have_two_parts(ctx, kind, n_q, n_kv, dim, rows, prefix):
+    """One rounding of the weights would be several times what the bound allows (tests/test_paged_pairs.py)."""
+    g = np.random.default_rng(dim + prefix)
+    b = cases.Batch(g, [1, rows, 1], [16, 24, 8], 16, n_kv, dim, prefix=prefix)
+    k, v, tokens = pairs.fill(g, b, kind)
+    q, scale = pairs.queries(g, b.total, n_q, dim), np.float32(0.75 / np.sqrt(dim))
+    got = Device(ctx, b, kind, n_q, k, v).attend(q, scale)
+    want, size, _ = cases.attend(b, tokens, q, scale)
+    off = np.abs(got - want) / pairs.bound(want, size, prefix + 24, pairs.largest_score(b, tokens, q, scale), kind)
+    assert off.max() <= 1, off.max()
+
+
+# ── plans that only large calls take ────────────────────────────────────────
+def merged_bytes(ctx, columns, n_seqs, rows, n_q, dim):
+    """The workspace of a call with a prefix whose lines have blocks of so many columns."""
+    pad, sm = lambda n: -(-n // 32) * 32, ctx.lib.smelt_cuda_sm_count(ctx.h)  # noqa: E731
+    lines = sum(pad(4 * (n_seqs + 3)) + pad(8 * sm * c * dim) + pad(16 * sm * c) + pad(20 * sm) for c in columns)
+    return lines + pad(8 * rows * n_q * dim) + pad(16 * rows * n_q)
+
+
+@pytest.mark.parametrize("kind,n_q,n_kv,dim,rows,prefix", [("bf16", 16, 4, 64, 70, 2300), ("f16", 4, 1, 128, 70, 8600), ("bf16", 10, 2, 128, 60, 4300), ("f16", 8, 2, 256, 70, 1200)])
+@pytest.mark.parametrize("window", [0, 700])
+def test_a_long_prefix_beside_streamed_sequences(ctx, kind, n_q, n_kv, dim, rows, prefix, window):
+    """The prefix on the tensor core, the sequences on the streaming kernel, and every row's parts of both joined."""
+    g = np.random.default_rng(prefix + window)
+    lengths = g.integers(1, 60, rows)
+    lengths[0], lengths[3] = 300, 1
+    b = cases.Batch(g, [1] * rows, lengths.tolist(), 16, n_kv, dim, prefix=prefix, behind=2)
+    ratio = n_q // n_kv
+    k, v, _ = b.fill(g, 0.0)
+    _, size = Device(ctx, b, kind, n_q, k, v).workspace()
+    assert size == merged_bytes(ctx, ((1 if dim == 256 else 2) * (128 // ratio * ratio), 8), rows, b.total, n_q, dim)
+    check_attention(ctx, g, kind, n_q, b, window)
+
+
+@pytest.mark.parametrize("n_q,n_kv,dim,prefix,window", [(16, 4, 64, 40, 0), (32, 1, 64, 200, 0), (20, 4, 128, 40, 30), (16, 4, 256, 33, 0)])
+def test_the_parts_of_a_groups_heads_joined_by_a_warp(ctx, n_q, n_kv, dim, prefix, window):
+    """Rows and heads past 64 warps an SM, behind a prefix: in blocks of one and of many rows, and a sequence that ends inside a block."""
+    g = np.random.default_rng(n_q + dim)
+    rows = 64 * ctx.lib.smelt_cuda_sm_count(ctx.h) // n_q + 9
+    b = cases.Batch(g, [rows - 100, 1, 0, 99], [rows - 100, 70, 4, 60], 16, n_kv, dim, prefix=prefix, behind=1)
+    check_attention(ctx, g, "bf16", n_q, b, window)
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("rope_dim,layout", [(64, 0), (64, 1), (6, 1), (40, 0)])
+@pytest.mark.parametrize("last", [0, 1])
+def test_append_of_two_rows_a_cta(ctx, kind, rope_dim, layout, last):
+    """900 rows and more: even and odd numbers of them, CTAs whose rows are of two sequences, rows behind the last sequence."""
+    g = np.random.default_rng(rope_dim)
+    b = cases.Batch(g, [401, 0, 503 + last], [500, 3, 503 + last], 32, 1, 64, prefix=10, behind=1)
+    check_append(ctx, g, kind, 3, b, rope_dim, layout, in_place=bool(last))
