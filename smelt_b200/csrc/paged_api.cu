@@ -17,6 +17,8 @@ smelt_status enter(smelt_cuda_ctx* ctx, Launch* l) {
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+// Arrays of `size`-byte values, null among them, where their type wants them: what is not would end the context on the device.
+template <class... P> bool aligned(size_t size, const P*... p) { return ((reinterpret_cast<uintptr_t>(p) % size == 0) && ...); }
 // Rows of `width` 16-bit values, `stride` apart, that 16-byte loads can take.
 bool rows_ok(const void* p, int64_t stride, int64_t width, int64_t rows) {
     return p && aligned16(p) && stride % 8 == 0 && (rows <= 1 || stride >= width) && stride >= 0 && stride < ((int64_t)1 << 38);
@@ -39,6 +41,7 @@ smelt_status cache_args(smelt_cuda_ctx* ctx, const smelt_paged_cache* k, const s
     if ((int64_t)b->rows * k->n_q > 0x3fffffff || (int64_t)b->prefix_length > 0x3fffffff) return fail(ctx, SMELT_ERR_OUT_OF_RANGE, "paged batch: too many rows or tokens");
     if (b->n_seqs > 0 && b->rows > 0 && (!b->row_start || !b->length || (b->table_stride > 0 && !b->table) || (b->prefix_length > 0 && !b->prefix_table)))
         return fail(ctx, SMELT_ERR_BAD_ARGUMENT, "paged batch: null pointer");
+    if (!aligned(4, b->row_start, b->length, b->table, b->prefix_table)) return fail(ctx, SMELT_ERR_BAD_ARGUMENT, "paged batch: misaligned pointer");
     *c = {};
     c->k = k->k; c->v = k->v;
     c->page_stride = k->page_stride; c->head_stride = k->head_stride; c->token_stride = k->token_stride;
@@ -158,7 +161,7 @@ smelt_status smelt_cuda_paged_append(smelt_cuda_ctx* ctx, const smelt_paged_cach
     if (s) return s;
     if (rope) {
         if (rope->rope_dim < 0 || rope->rope_dim % 2 || rope->rope_dim > cache->head_dim || (rope->layout != SMELT_ROPE_ADJACENT && rope->layout != SMELT_ROPE_HALVES) ||
-            (rope->rope_dim > 0 && !rope->freq))
+            (rope->rope_dim > 0 && !rope->freq) || !aligned(8, rope->freq) || !aligned(4, rope->position))
             return fail(ctx, SMELT_ERR_BAD_ARGUMENT, "paged append: bad rotation");
         a.rope_dim = rope->rope_dim; a.layout = rope->layout; a.factor = rope->factor; a.freq = (const double*)rope->freq; a.position = (const int32_t*)rope->position;
     }
@@ -247,6 +250,7 @@ smelt_status smelt_cuda_verify_drafts(smelt_cuda_ctx* ctx, const smelt_verify_ar
     if (!s) s = verify_args(ctx, v);
     if (s) return s;
     if (v->n_seqs == 0) return SMELT_OK;
+    if (!aligned(4, v->row_start, v->tokens, v->temperature, v->random, v->out_tokens, v->accepted)) return fail(ctx, SMELT_ERR_BAD_ARGUMENT, "verify drafts: misaligned pointer");
     if (v->rows == 0) {  // nobody has a draft
         if (!v->accepted) return fail(ctx, SMELT_ERR_BAD_ARGUMENT, "verify drafts: null pointer");
         return check_cuda(ctx, cudaMemsetAsync(v->accepted, 0, (size_t)v->n_seqs * sizeof(int32_t), l.stream), "verify drafts");

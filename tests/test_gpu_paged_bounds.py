@@ -333,3 +333,102 @@ def test_append_of_two_rows_a_cta(ctx, kind, rope_dim, layout, last):
     g = np.random.default_rng(rope_dim)
     b = cases.Batch(g, [401, 0, 503 + last], [500, 3, 503 + last], 32, 1, 64, prefix=10, behind=1)
     check_append(ctx, g, kind, 3, b, rope_dim, layout, in_place=bool(last))
+
+
+def test_misaligned_arrays_are_refused(ctx):
+    g = np.random.default_rng(71)
+    b = cases.Batch(g, [2, 1], [20, 10], 16, 2, 64, prefix=16)
+    k, v, _ = b.fill(g, 0.0)
+    d = Device(ctx, b, "f16", 4, k, v)
+    q, out = ctx.alloc(3 * 256 * 2), ctx.alloc(3 * 256 * 2)
+    work, size = d.workspace()
+    freq, position = ctx.to_device(np.ones(34)), ctx.to_device(np.zeros(4, np.int32))
+    for field in (None, "row_start", "length", "table", "prefix_table"):
+        t = capi.PagedBatch.from_buffer_copy(d.batch)
+        if field:
+            setattr(t, field, getattr(t, field) + 2)
+        status = capi.BAD_ARGUMENT if field else capi.OK
+        assert ctx.call_status("paged_attention", C.byref(d.cache), C.byref(t), q.ptr, 256, out.ptr, 256, 0.1, 0, work.ptr, size) == status, field
+        assert ctx.call_status("paged_append", C.byref(d.cache), C.byref(t), None, None, 0, q.ptr, 128, q.ptr, 128, None, 0) == status, field
+    for f, p, status in ((freq.ptr, position.ptr, capi.OK), (freq.at(4), position.ptr, capi.BAD_ARGUMENT), (freq.ptr, position.at(2), capi.BAD_ARGUMENT)):
+        rope = capi.RopeDesc(64, 1, 1.0, f, p)
+        assert ctx.call_status("paged_append", C.byref(d.cache), C.byref(d.batch), C.byref(rope), None, 0, q.ptr, 128, q.ptr, 128, None, 0) == status
+    buf = ctx.alloc(1 << 16).fill(0)
+    buf.upload(np.array([0, 2], np.int32))
+    good = dict(n_seqs=1, rows=2, vocab=100, target_stride=100, row_start=buf.ptr, target=buf.at(1024), tokens=buf.at(4096), temperature=buf.at(4608), random=buf.at(5120), out_tokens=buf.at(6144),
+                accepted=buf.at(7168), workspace=buf.at(8192), workspace_bytes=8192)
+    assert ctx.call_status("verify_drafts", C.byref(capi.VerifyArgs(**good))) == capi.OK
+    for field in ("row_start", "tokens", "temperature", "random", "out_tokens", "accepted"):
+        assert ctx.call_status("verify_drafts", C.byref(capi.VerifyArgs(**{**good, field: good[field] + 1}))) == capi.BAD_ARGUMENT, field
+
+
+@pytest.mark.parametrize("n_q,n_kv,dim", [(16, 1, 64), (4, 2, 128), (16, 1, 128), (8, 1, 256)])
+@pytest.mark.parametrize("prefix", [0, 30])
+def test_as_many_sequences_as_a_call_takes(ctx, n_q, n_kv, dim, prefix):
+    """The streaming kernel's rings beside the starts and lengths of 1024 sequences."""
+    g = np.random.default_rng(dim + prefix)
+    lengths = g.integers(0, 12, 1024)
+    lengths[[0, 511, 1023]] = 70, 200, 41
+    check_attention(ctx, g, "bf16", n_q, cases.Batch(g, [1] * 1024, lengths.tolist(), 8, n_kv, dim, prefix=prefix))
+
+
+PLANS = [("streaming", 8, 2, 64, 0, 2), ("tensor core", 32, 2, 64, 0, 8), ("one line with a prefix", 8, 2, 64, 100, 2), ("tensor core with a prefix", 32, 2, 128, 300, 8), ("two lines", 16, 4, 64, 2600, 1)]
+
+
+@pytest.mark.parametrize("name,n_q,n_kv,dim,prefix,most", PLANS, ids=[p[0] for p in PLANS])
+def test_a_captured_call_follows_lengths_and_tables(ctx, name, n_q, n_kv, dim, prefix, most):
+    """Every plan, captured once: starts, lengths and pages of each replay as an eager call has them, bit for bit."""
+    g = np.random.default_rng(dim + prefix)
+    seqs = 70
+    b = cases.Batch(g, [most] * seqs, [most + 90] * seqs, 16, n_kv, dim, prefix=prefix)
+    k, v, _ = b.fill(g, 0.0)
+    d = Device(ctx, b, "f16", n_q, k, v)
+    q = ctx.to_device(np.float16(g.standard_normal((b.total, n_q, dim))))
+    outs = [ctx.alloc(b.total * n_q * dim * 2) for _ in range(2)]
+    (work, size), (other, _) = d.workspace(), d.workspace()
+
+    def call(out, memory):
+        ctx.call("paged_attention", C.byref(d.cache), C.byref(d.batch), q.ptr, n_q * dim, out.ptr, n_q * dim, 0.1, 0, memory.ptr, size)
+
+    ctx.call("capture_begin")
+    call(outs[0], work)
+    call(outs[0], work)  # and one behind the other, over the same workspace
+    ctx.call("capture_end")
+    ms = C.c_float()
+    for turn in range(5):
+        rows = g.integers(0, most + 1, seqs)
+        d.kept[0].upload(np.concatenate([[0], np.cumsum(rows)]).astype(np.int32))
+        d.kept[1].upload(np.array([rows + g.integers(0, 90, seqs), rows, np.zeros(seqs)][turn % 3], np.int32))
+        d.kept[2].upload(g.permutation(b.table.reshape(-1)).reshape(b.table.shape) if turn == 4 else b.table)
+        for out in outs:
+            out.upload(np.full(b.total * n_q * dim, 7, np.float16))
+        ctx.call("capture_replay", turn % 2, 1 + turn % 2, C.byref(ms))
+        call(outs[1], other)
+        first, second = (out.download(np.uint16, b.total * n_q * dim) for out in outs)
+        assert np.array_equal(first, second)
+        assert (first.reshape(b.total, -1)[rows.sum():] == np.float16(7).view(np.uint16)).all()
+        assert ctx.device_error_flags() in ((0, 0x10000) if turn == 4 else (0,))
+
+
+def test_two_contexts_side_by_side(ctx):
+    """Calls of two contexts, on their two streams, with a workspace each."""
+    other = capi.Context(0)
+    try:
+        sides = []
+        for c, (n_q, n_kv, dim, prefix, rows) in zip((ctx, other) * 2, ((8, 2, 128, 0, 1), (8, 2, 128, 0, 1), (32, 2, 64, 0, 9), (16, 2, 64, 200, 3))):
+            g = np.random.default_rng(rows + dim)
+            b = cases.Batch(g, [rows, 1], [700, 60], 16, n_kv, dim, prefix=prefix)
+            k, v, _ = b.fill(g, 0.0)
+            d, q = Device(c, b, "f16", n_q, k, v), cases.rounded(g.standard_normal((b.total, n_q, dim)), "f16")
+            want = d.attend(q, 0.1)
+            dq, out, (work, size) = c.to_device(np.float16(q)), c.to_device(np.full(q.shape, 7, np.float16)), d.workspace()
+            sides.append((c, (C.byref(d.cache), C.byref(d.batch), dq.ptr, n_q * dim, out.ptr, n_q * dim, 0.1, 0, work.ptr, size), out, want, (d, dq, work)))
+        for _ in range(30):
+            for c, args, _, _, _ in sides:
+                c.call("paged_attention", *args)
+        for _, _, out, want, _ in sides:
+            assert np.array_equal(out.download(np.float16, want.shape).astype(np.float64), want)
+        assert other.device_error_flags() == 0
+        del sides
+    finally:
+        other.close()
