@@ -66,10 +66,10 @@ size_t attention_plan(const smelt_cuda_ctx* ctx, const smelt_paged_cache* k, con
         return p;
     };
     // Columns of a source: up to 16 on the streaming kernel (8 with heads of 256), more on the tensor core.  us with 16 | 32 columns, 16 sequences of
-    // 2000 tokens and 8 key heads of 128: streaming 45 | 69, tensor core 60 | 59; heads of 64: 35 | 53 and 43 | 43; heads of 256 and 8 | 16
-    // columns: 72 | 123 and 84 | 84.  A launch takes sequences and prefix together where they go to the same kernel, and a prefix that is no
+    // 2000 tokens and 8 key heads of 128: streaming 42 | 67, tensor core 46 | 46; heads of 64: 34 | 51 and 35 | 35; heads of 256 and 8 | 16
+    // columns: 70 | 122 and 70 | 71.  A launch takes sequences and prefix together where they go to the same kernel, and a prefix that is no
     // more than four tiles a warp goes with the sequences on the streaming kernel (64 sequences of 300 tokens behind a prefix of 1000 | 2000 | 4000,
-    // heads of 128: together 43 | 51 | 72 us, a launch each 47 | 41 | 43).
+    // 32 query and 8 key heads of 128: together 53 | 60 | 83 us, a launch each 55 | 60 | 62).
     const int64_t own = (int64_t)(b->max_rows > 0 ? b->max_rows : 1) * a->c.ratio, prefix = b->prefix_length > 0 ? (int64_t)b->rows * a->c.ratio : 0;
     const bool can = paged_wide_takes(D, b->n_seqs);
     const int64_t most = D == 256 ? 8 : 16, prefix_tiles = (prefix + most - 1) / most * k->n_kv * ((b->prefix_length >> paged_narrow_keys()) + 2);
@@ -88,7 +88,7 @@ size_t attention_plan(const smelt_cuda_ctx* ctx, const smelt_paged_cache* k, con
         line.column_div = Divisor::of((uint32_t)line.columns);
         line.keys = wide ? paged_wide_keys(D) : paged_narrow_keys();
         // What an item costs beside its steps: 11 us of 2.2 us a step on the tensor core (the first scores, a masked step, the end; three | five | eight
-        // places: two ragged prompts of up to 1500 rows behind 4100 tokens 180 | 172 | 173 us, 64 sequences of 16 rows 59 | 60 | 67), 1 us of 1 us a tile on the streaming kernel.
+        // places: two ragged prompts of up to 1500 rows behind 4100 tokens 177 | 167 | 170 us, 16 sequences of up to six rows 28.6 | 29.2 | 32.9), 1 us of 1 us a tile on the streaming kernel.
         line.extra = wide ? 5 : 1;
         line.ctas = ctx->sm_count < kPagedCtas ? ctx->sm_count : kPagedCtas;
         line.workers = wide ? 1 : paged_narrow_workers(D);

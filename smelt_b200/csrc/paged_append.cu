@@ -8,9 +8,10 @@
 // 16-bit type.
 //
 // A CTA takes one row, or two from 900 rows on (the chain row -> sequence -> length -> page and the sines are then paid for
-// twice the bytes; us with one | two, 40 query and 8 key heads of 128: 600 rows 6.2 | 6.9, 900 8.4 | 8.3, 1200 10.3 | 8.4, 32768 103 | 96): a warp a row
-// finds its sequence, all threads share the sines and cosines through shared memory, then a thread takes 16 bytes of a head and
-// the 16 bytes they turn with.  Memory bounds it: 515 MB of 32768 rows go through in 96 us, 5.3 TB/s.
+// twice the bytes; us with one | two: 16 query and 4 key heads of 128, 600 rows 3.8 | 4.4, 900 5.3 | 5.3, 2400 8.9 | 7.8, 32768 114 | 91; 40 and 8 heads,
+// 900 rows 6.9 | 7.7, 2400 18.2 | 18.5, 6000 37.8 | 36.7, 32768 182 | 170): a warp a row finds its sequence, all threads share the sines and cosines
+// through shared memory, then a thread takes 16 bytes of a head and the 16 bytes they turn with.  Memory bounds it: 940 MB of 32768 rows go
+// through in 170 us, 5.5 TB/s.
 #include <cuda_bf16.h>
 
 #include "paged.h"

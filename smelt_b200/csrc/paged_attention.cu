@@ -801,7 +801,7 @@ cudaError_t launch_paged_narrow(const Launch& l, PagedType type, int head_dim, c
 cudaError_t launch_paged_merge(const Launch& l, PagedType type, int head_dim, const PagedAttentionArgs& a) {
     const int64_t all = (int64_t)a.c.rows * a.c.n_q;
     // A head a warp while 64 warps an SM hold them all, else a group (us of the call with a head | a group, 40 query and 8 key heads behind a prefix of
-    // 2000: 100 rows 29 | 37, 200 39 | 43, 300 51 | 49, 1500 207 | 196).
+    // 2000: 100 rows 27 | 36, 200 37 | 41, 300 51 | 48, 1500 205 | 193).
     const int heads = all > (int64_t)a.line[0].ctas * 64 ? a.c.ratio : 1;
     const int grid = (int)((all / heads + kMergeWarps - 1) / kMergeWarps);
     auto go = [&](auto f16, auto bf16) { return type == kPagedF16 ? launch(l, f16, grid, kMergeWarps * 32, 0, a, heads) : launch(l, bf16, grid, kMergeWarps * 32, 0, a, heads); };

@@ -8,7 +8,7 @@
 // set is at its exponentials (128 x 128 of them take the SM's 16 a clock 1024 clocks) the tensor core works for the other (1024 clocks a
 // tile and step).  A block of 128 columns or fewer gives both sets the same tile and every other step, and their sums are joined at the
 // end.  The maximum that P is relative to is the first step's, and moves only when a step's weights add up to more than 2^10 times the first step's largest: O is rescaled
-// a few times an item at most, and behind the first step nobody looks for a maximum (1500 rows over 20000 tokens: 594 us with it, 542 without).
+// a few times an item at most, and behind the first step nobody looks for a maximum (1500 rows over 20000 tokens, as both were built: 594 us with it, 542 without).
 // P is rounded once to the 16-bit type, the type of the values it is multiplied with; sums are fp32.  The streaming kernel, which waits for memory,
 // multiplies with P in two parts and is as near to 64 bits as the rounded outputs are; here outputs are 1.2 to 1.35 times as far off (bf16, 4100
 // tokens: 2.1e-3 of the norm against 1.6e-3), because a second part, rounded from what the first leaves, costs its products and as much again of the
@@ -17,8 +17,9 @@
 //
 // What bounds it: the way from a set's scores through its exponentials to its product and the next scores, 4000 clocks for two tiles and 128 keys, of
 // which the tensor core works 2048 and the exponentials take as many beside it; the loads are hidden.  bf16, 40 query and 8 key heads of
-// 128, pages of 32: 1500 rows over 20000 tokens in 525 us (1.13 PFLOP/s, 67 % of a library product's rate), 4 x 1500 rows over their own 1500
-// tokens in 122, where an item of six steps costs as much again for its beginning and end (lookups and first loads, the masked step, the sums).
+// 128, pages of 32: 1500 rows over 20000 tokens in 527 us (1.12 PFLOP/s, 67 % of a library product's rate; 587 when a second of such calls has brought
+// the clock down to what the power allows), 4 x 1500 rows over their own 1500 tokens in 191 (167 there; 136 with 32 query heads), where an item of six
+// steps costs as much again for its beginning and end (lookups and first loads, the masked step, the sums).
 //
 // Value rows that are not finite and that not every column of the step sees are taken out of the product (as zeros) and added
 // for the columns that see them alone, so that nothing reaches a row that it does not see.  An fp16 weight may round to 0, and 0 times infinity is

@@ -13,9 +13,9 @@
 // drawn by, and its last CTA of a sequence finds the index.  (A cluster of eight CTAs a sequence, which did all of that in one
 // launch, took 45 us for one sequence and 70 for 48 of them, its fp64 pipe busy for an eighth of the time.)
 //
-// us with 152k tokens and a draft's probabilities: 1 sequence of up to six rows 23, 16 45, 48 76, 192 of three 177.  Memory bounds none of it: the statistics of 48
-// sequences (94 MB) take 34 of the 76 (10 operations an element, and four microseconds of a CTA's beginning and end), the fp64 weights, two to an
-// element and twice over, the rest.
+// us with 152k tokens and a draft's probabilities, logits from memory: 1 sequence of up to six rows 28, 16 46, 48 87, 192 of three 175 (the same logits again, 94 MB
+// of 48 sequences in L2: 82).  Memory bounds none of it: the statistics of 48 sequences take 35 of the 87 (11 operations an element, and four
+// microseconds of a CTA's beginning and end), the fp64 weights, two to an element and twice over, the rest.
 #include <cuda_bf16.h>
 
 #include "paged.h"
@@ -24,8 +24,8 @@ namespace smelt {
 namespace {
 
 constexpr int kStatThreads = 256, kStatWords = 4;  // words of 16 bytes a thread has on their way at a time
-// CTAs of a launch of the draw, and their threads: 80 registers let eight fp64 chains of a thread run side by side (us of the whole, 48 | 192 sequences:
-// 256 threads and three CTAs an SM 76 | 177, 512 and two, of 64 registers, 78 | 186, 512 and one, of 108, 83 | 182).
+// CTAs of a launch of the draw, and their threads: 80 registers let eight fp64 chains of a thread run side by side (us of the whole, 16 | 48 | 192
+// sequences: 256 threads and three CTAs an SM 46 | 87 | 174, 512 and two, of 64 registers, 53 | 91 | 170, 512 and one, of 108, 64 | 108 | 191).
 constexpr int kDrawCtas = 1184, kDrawThreads = 256, kDrawWarps = kDrawThreads / 32;
 constexpr float kNone = -INFINITY;
 
@@ -96,8 +96,8 @@ struct Row {
     }
 };
 
-// Stretches of a row: as many as give every SM four CTAs (us of the whole with four | eight, 152k tokens: 8 sequences 37 | 39, 16 46 | 50,
-// 48 81 | 81), of 1024 words at least and 16384 at most.
+// Stretches of a row: as many as give every SM four CTAs (us of the whole with four | eight, 152k tokens: 8 sequences 36 | 37.5, 16 43 | 47,
+// 48 87 | 89), of 1024 words at least and 16384 at most.
 struct Stretches { int count, words; };
 Stretches stretches_of(int rows, int vocab, int per_word) {
     const int words = (vocab + 2 * per_word - 2) / per_word, least = (words + 16383) / 16384, most = (words + 1023) / 1024;
