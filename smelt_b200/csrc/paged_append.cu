@@ -12,27 +12,15 @@
 // 900 rows 6.9 | 7.7, 2400 18.2 | 18.5, 6000 37.8 | 36.7, 32768 182 | 170): a warp a row finds its sequence, all threads share the sines and cosines
 // through shared memory, then a thread takes 16 bytes of a head and the 16 bytes they turn with.  Memory bounds it: 940 MB of 32768 rows go
 // through in 170 us, 5.5 TB/s.
-#include <cuda_bf16.h>
-
+#include "attention.cuh"
 #include "paged.h"
 
 namespace smelt {
 namespace {
 
-constexpr int kThreads = 256, kMostRows = 2, kMostPairs = 128;
+using attn::TileElem;
 
-template <class E> struct Pair16;
-template <> struct Pair16<__half> {
-    static __device__ __forceinline__ float2 unpack(uint32_t v) { return __half22float2(u32_as_h2(v)); }
-    static __device__ __forceinline__ uint32_t pack(float x, float y) { return h2_as_u32(__floats2half2_rn(x, y)); }
-};
-template <> struct Pair16<__nv_bfloat16> {
-    static __device__ __forceinline__ float2 unpack(uint32_t v) { return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xFFFF0000u)); }
-    static __device__ __forceinline__ uint32_t pack(float x, float y) {
-        const __nv_bfloat162 v = __floats2bfloat162_rn(x, y);
-        return *reinterpret_cast<const uint32_t*>(&v);
-    }
-};
+constexpr int kThreads = 256, kMostRows = 2, kMostPairs = 128;
 
 // Every eight pairs a gap of 16 bytes: the lanes of a load, 64 bytes apart, would meet in four banks.
 __host__ __device__ constexpr int slot(int pair) { return pair + (pair >> 3) * 2; }
@@ -118,9 +106,9 @@ __global__ void __launch_bounds__(kThreads) paged_append_kernel(const PagedAppen
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         const float4 two = *reinterpret_cast<const float4*>(t + slot(d) + 2 * e);
-                        const float2 p = Pair16<E>::unpack(xs[e]), q = Pair16<E>::unpack(ys[e]), t0 = make_float2(two.x, two.y), t1 = make_float2(two.z, two.w);
-                        u[e] = Pair16<E>::pack(first_of(p.x, q.x, t0), first_of(p.y, q.y, t1));
-                        w[e] = Pair16<E>::pack(second_of(p.x, q.x, t0), second_of(p.y, q.y, t1));
+                        const float2 p = TileElem<E>::unpack(xs[e]), q = TileElem<E>::unpack(ys[e]), t0 = make_float2(two.x, two.y), t1 = make_float2(two.z, two.w);
+                        u[e] = TileElem<E>::pack(first_of(p.x, q.x, t0), first_of(p.y, q.y, t1));
+                        w[e] = TileElem<E>::pack(second_of(p.x, q.x, t0), second_of(p.y, q.y, t1));
                     }
                     *reinterpret_cast<uint4*>(dst + d) = make_uint4(u[0], u[1], u[2], u[3]);
                     *reinterpret_cast<uint4*>(dst + d + pairs) = make_uint4(w[0], w[1], w[2], w[3]);
@@ -132,9 +120,9 @@ __global__ void __launch_bounds__(kThreads) paged_append_kernel(const PagedAppen
 #pragma unroll
                     for (int e = 0; e < 4; e += 2) {
                         const float4 two = *reinterpret_cast<const float4*>(t + slot(4 * j) + e);
-                        const float2 p = Pair16<E>::unpack(xs[e]), q = Pair16<E>::unpack(xs[e + 1]), t0 = make_float2(two.x, two.y), t1 = make_float2(two.z, two.w);
-                        u[e] = Pair16<E>::pack(first_of(p.x, p.y, t0), second_of(p.x, p.y, t0));
-                        u[e + 1] = Pair16<E>::pack(first_of(q.x, q.y, t1), second_of(q.x, q.y, t1));
+                        const float2 p = TileElem<E>::unpack(xs[e]), q = TileElem<E>::unpack(xs[e + 1]), t0 = make_float2(two.x, two.y), t1 = make_float2(two.z, two.w);
+                        u[e] = TileElem<E>::pack(first_of(p.x, p.y, t0), second_of(p.x, p.y, t0));
+                        u[e + 1] = TileElem<E>::pack(first_of(q.x, q.y, t1), second_of(q.x, q.y, t1));
                     }
                     *reinterpret_cast<uint4*>(dst + d) = make_uint4(u[0], u[1], u[2], u[3]);
                 }
@@ -147,7 +135,7 @@ __global__ void __launch_bounds__(kThreads) paged_append_kernel(const PagedAppen
                     dst[d1] = y;
                 } else {
                     const float fx = (float)x, fy = (float)y;
-                    const uint32_t v = Pair16<E>::pack(first_of(fx, fy, t[slot(j)]), second_of(fx, fy, t[slot(j)]));
+                    const uint32_t v = TileElem<E>::pack(first_of(fx, fy, t[slot(j)]), second_of(fx, fy, t[slot(j)]));
                     reinterpret_cast<uint16_t*>(dst)[d0] = (uint16_t)v;
                     reinterpret_cast<uint16_t*>(dst)[d1] = (uint16_t)(v >> 16);
                 }

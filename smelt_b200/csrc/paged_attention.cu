@@ -55,9 +55,6 @@ constexpr uint32_t kHidden = 0x7FFFF00Du;  // a NaN of our own
 template <class E> constexpr float kAbove = std::is_same<E, __half>::value ? 14.f : 0.f;
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory"); }
-__device__ __forceinline__ void cp_async16_or_zero(uint32_t dst, const void* src, bool take) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(take ? 16 : 0) : "memory");
-}
 
 template <class E> __device__ __forceinline__ E round_to(float v);
 template <> __device__ __forceinline__ __half round_to<__half>(float v) { return __float2half_rn(v); }
@@ -581,8 +578,10 @@ __global__ void __launch_bounds__(kWarps<D> * 32, 1) paged_narrow_kernel(const _
         }
         if (infinite) {  // (worked out again, so that nothing more is kept over the item's steps)
             const Range of = item.source == 0 ? Range{batch.prefix_lo, c.prefix_length} : block_keys(c, line, seq_of(item.source), item.block, a.window);
+            const int first = of.lo / kTile;
             put_infinities<D, NH, E>(a, before ? fronts + warp * C * (D + 1) : behind ? reinterpret_cast<float*>(ring) : nullptr, item.source, item.head, seq.row, f0, width,
-                                     max((of.lo / kTile + max(begin - item_at, 0)) * kTile, of.lo), min(k0 + kTile, of.hi), keys[0][0], keys[0][1], keys[NH - 1][0], keys[NH - 1][1]);
+                                     max((first + max(begin - item_at, 0)) * kTile, of.lo), min((first + min(end - item_at, item.steps)) * kTile, of.hi), keys[0][0], keys[0][1],
+                                     keys[NH - 1][0], keys[NH - 1][1]);
         }
     }
     cp_async_wait<0>();

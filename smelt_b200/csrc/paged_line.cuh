@@ -10,6 +10,10 @@ namespace paged {
 constexpr float kLowest = -3.402823466e38f;
 constexpr int kDisordered = -1;  // in the place of the first prefix key that any row sees: row starts that go down, nothing is computed
 
+__device__ __forceinline__ void cp_async16_or_zero(uint32_t dst, const void* src, bool take) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(take ? 16 : 0) : "memory");
+}
+
 struct Range { int lo, hi; };  // keys [lo, hi)
 
 // A sequence's rows of the batch and its tokens, cut to what the arrays hold.
@@ -62,27 +66,17 @@ __device__ __forceinline__ void scan_line(const PagedArgs& c, const PagedLine& l
     b.row = b.cum + n + 2;
     b.length = b.row + n + 1;
     if (tid == 0) lowest = c.prefix_length;
-    bool down = false;
     for (int s = tid; s <= n; s += THREADS) {
         b.row[s] = first_row(c, s);
-        if (s < n) {
-            b.length[s] = tokens_of(c, s);
-            down |= first_row(c, s + 1) < b.row[s];
-        }
+        if (s < n) b.length[s] = tokens_of(c, s);
     }
-    // Starts that go down would give rows to several sequences, and their places could be more than are counted in 32 bits: nobody has rows then.
-    if (__syncthreads_or(down)) {
-        for (int s = tid; s <= n; s += THREADS) b.row[s] = 0;
-        if (tid == 0) {
-            lowest = kDisordered;
-            if (blockIdx.x == 0 && c.err) atomicOr(c.err, KERR_BAD_PAGE);
-        }
-        __syncthreads();
-    }
+    __syncthreads();
     const int per = (n + THREADS - 1) / THREADS, s0 = min(n, tid * per), s1 = min(n, s0 + per);
     int mine = 0;
+    bool down = false;
     for (int s = s0; s < s1; ++s) {
         const Seq q = b.seq(s);
+        down |= b.row[s + 1] < b.row[s];
         if (line.with_own) mine += c.n_kv * places_of_seq(c, line, q, blocks_of(c, line, q.n), window);
         if (line.with_prefix && window && q.n) atomicMin(&lowest, prefix_keys(q, 0, c.prefix_length, window).lo);
     }
@@ -95,8 +89,8 @@ __device__ __forceinline__ void scan_line(const PagedArgs& c, const PagedLine& l
         }
     }
     if (lane == 31) warp_sums[warp] = run;
-    __syncthreads();
-    b.prefix_lo = window || lowest < 0 ? lowest : 0;
+    const int disordered = __syncthreads_or(down);
+    b.prefix_lo = window ? lowest : 0;
     int before = run - mine;
     if (n > 32 * per)
         for (int w = 0; w < warp; ++w) before += warp_sums[w];
@@ -112,9 +106,15 @@ __device__ __forceinline__ void scan_line(const PagedArgs& c, const PagedLine& l
         }
     }
     __syncthreads();
+    if (disordered) {  // Starts that go down give rows to several sequences, and their places may be more than are counted in 32 bits: nobody has rows.
+        for (int s = tid; s < n + 2; s += THREADS) b.cum[s] = 0;
+        for (int s = tid; s <= n; s += THREADS) b.row[s] = 0;
+        if (tid == 0 && blockIdx.x == 0 && c.err) atomicOr(c.err, KERR_BAD_PAGE);
+        __syncthreads();
+    }
     if (blockIdx.x == 0) {
         for (int s = tid; s < n + 2; s += THREADS) line.cum[s] = b.cum[s];
-        if (tid == 0) line.cum[n + 2] = b.prefix_lo;
+        if (tid == 0) line.cum[n + 2] = disordered ? kDisordered : b.prefix_lo;
     }
 }
 

@@ -24,10 +24,9 @@
 // Value rows that are not finite and that not every column of the step sees are taken out of the product (as zeros) and added
 // for the columns that see them alone, so that nothing reaches a row that it does not see.  An fp16 weight may round to 0, and 0 times infinity is
 // NaN: where fp16 sums come out not finite, what infinite values make of them is put in afterwards.
-#include <cuda_bf16.h>
-
 #include <type_traits>
 
+#include "attention.cuh"
 #include "paged_line.cuh"
 #include "tcgen05.cuh"
 
@@ -35,6 +34,7 @@ namespace smelt {
 namespace {
 
 using namespace paged;
+using attn::TileElem;
 
 template <int D>
 struct Cfg {
@@ -63,18 +63,13 @@ constexpr size_t wide_shared(int n_seqs) {
     return (size_t)Cfg<D>::kSets * Cfg<D>::kQTile + 2 * Cfg<D>::kStages * Cfg<D>::kTile + Cfg<D>::kJoint + ((sizeof(Shared) + 15) & ~(size_t)15) + batch_bytes(n_seqs);
 }
 
-template <class E> struct Pack;
-template <> struct Pack<__half> {
+template <class E> struct Half16;  // of the products' 16-bit type: its code in a descriptor, its infinity, a value of it
+template <> struct Half16<__half> {
     static constexpr uint32_t kType = 0u, kInf = 0x7C00u;
-    static __device__ __forceinline__ uint32_t two(float x, float y) { return h2_as_u32(__floats2half2_rn(x, y)); }
     static __device__ __forceinline__ float one(uint16_t v) { return __half2float(__ushort_as_half(v)); }
 };
-template <> struct Pack<__nv_bfloat16> {
+template <> struct Half16<__nv_bfloat16> {
     static constexpr uint32_t kType = (1u << 7) | (1u << 10), kInf = 0x7F80u;
-    static __device__ __forceinline__ uint32_t two(float x, float y) {
-        const __nv_bfloat162 v = __floats2bfloat162_rn(x, y);
-        return *reinterpret_cast<const uint32_t*>(&v);
-    }
     static __device__ __forceinline__ float one(uint16_t v) { return __uint_as_float((uint32_t)v << 16); }
 };
 
@@ -130,12 +125,9 @@ __device__ __forceinline__ void tmem_st16(uint32_t t, const uint32_t (&v)[16]) {
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void barrier(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
-__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool take) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(take ? 16 : 0) : "memory");
-}
 // Not 0 where one of the eight values is not finite: an exponent of all ones, and one more, carries into the sign's place.
 template <class E> __device__ __forceinline__ uint32_t not_finite(const uint4& w) {
-    constexpr uint32_t m = Pack<E>::kInf * 0x10001u, one = (0x8000u - Pack<E>::kInf) * 0x10001u;
+    constexpr uint32_t m = Half16<E>::kInf * 0x10001u, one = (0x8000u - Half16<E>::kInf) * 0x10001u;
     return (((w.x & m) + one) | ((w.y & m) + one) | ((w.z & m) + one) | ((w.w & m) + one)) & 0x80008000u;
 }
 
@@ -322,7 +314,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_wide_kernel(const _
                     const bool live = f < it.width;
                     const E* from = static_cast<const E*>(a.q) + (live ? (size_t)(it.seq.row + i) * a.q_stride + (size_t)(cur.head * c.ratio + ff - i * c.ratio) * D : 0);
                     const uint32_t to = smem_u32(q_tiles + (f >> 7) * C::kQTile);
-                    for (int k = ch; k < CHUNKS; k += LANES) copy16(to + place(128, f & 127, k), from + 8 * k, live);
+                    for (int k = ch; k < CHUNKS; k += LANES) cp_async16_or_zero(to + place(128, f & 127, k), from + 8 * k, live);
                 }
             }
             cp_async_commit();
@@ -412,7 +404,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_wide_kernel(const _
 #pragma unroll 4
                         for (int r = r_first; r < KEYS; r += ROWS) {
                             const long long at = rows[r];
-                            for (int k = ch; k < CHUNKS; k += LANES) copy16(dst + place(KEYS, r, k), static_cast<const E*>(pool) + max(at, 0ll) + 8 * k, at >= 0);
+                            for (int k = ch; k < CHUNKS; k += LANES) cp_async16_or_zero(dst + place(KEYS, r, k), static_cast<const E*>(pool) + max(at, 0ll) + 8 * k, at >= 0);
                         }
                     }
                     cp_async_commit();
@@ -470,8 +462,8 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_wide_kernel(const _
         }
     } else if (warp == C::kMmaWarp) {
         // ── products ──
-        constexpr uint32_t kScores = (1u << 4) | Pack<E>::kType | ((uint32_t)(KEYS >> 3) << 17) | ((128u >> 4) << 24);
-        constexpr uint32_t kValues = (1u << 4) | Pack<E>::kType | (1u << 16) | ((uint32_t)(D >> 3) << 17) | ((128u >> 4) << 24);
+        constexpr uint32_t kScores = (1u << 4) | Half16<E>::kType | ((uint32_t)(KEYS >> 3) << 17) | ((128u >> 4) << 24);
+        constexpr uint32_t kValues = (1u << 4) | Half16<E>::kType | (1u << 16) | ((uint32_t)(D >> 3) << 17) | ((128u >> 4) << 24);
         const uint64_t q_desc = smem_desc_sw128(smem_u32(q_tiles)), k_desc = smem_desc_sw128(smem_u32(k_tiles)), v_desc = value_desc(smem_u32(v_tiles), KEYS * 128);
         auto wait = [&](uint64_t* bar, uint32_t parity) {
             alive = __all_sync(0xffffffffu, alive && wait_alive_short(smem_u32(bar), parity, smem_u32(&sh.dead))) != 0;
@@ -578,7 +570,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_wide_kernel(const _
                         split(fma2(pair_of(__uint_as_float(v[x + e]), __uint_as_float(v[x + e + 1])), scales, minus), y0, y1);
                         const float p0 = exp2_approx(y0), p1 = exp2_approx(y1);
                         sums[e >> 1 & 1] = add2(sums[e >> 1 & 1], pair_of(p0, p1));
-                        p[e / 2] = Pack<E>::two(p0, p1);
+                        p[e / 2] = TileElem<E>::pack(p0, p1);
                     }
                     tmem_st16(s_at + x / 2, p);
                 }
@@ -663,7 +655,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_wide_kernel(const _
                                 tmem_wait_ld();
                                 float p = 0.f;
                                 for (int e = 0; e < 8; ++e)
-                                    if (e == ((k >> 1) & 7)) p = Pack<E>::one((uint16_t)(k & 1 ? pk[e] >> 16 : pk[e] & 0xffffu));
+                                    if (e == ((k >> 1) & 7)) p = Half16<E>::one((uint16_t)(k & 1 ? pk[e] >> 16 : pk[e] & 0xffffu));
                                 const bool sees = key >= keys.lo && key < keys.hi;
                                 for (int x = 0; x < D; x += 16) {
                                     uint32_t v[16];
@@ -762,7 +754,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_wide_kernel(const _
                 } else {
                     uint32_t w[16];
 #pragma unroll
-                    for (int e = 0; e < 32; e += 2) w[e / 2] = l == 0.f ? 0u : Pack<E>::two(__uint_as_float(v[e]) * rate, __uint_as_float(v[e + 1]) * rate);
+                    for (int e = 0; e < 32; e += 2) w[e / 2] = l == 0.f ? 0u : TileElem<E>::pack(__uint_as_float(v[e]) * rate, __uint_as_float(v[e + 1]) * rate);
 #pragma unroll
                     for (int e = 0; e < 16; e += 8) store32(to + x + 2 * e, *reinterpret_cast<const uint32_t(*)[8]>(w + e), sectors);
                 }
