@@ -94,15 +94,17 @@ __device__ __noinline__ void weighted_sum_masked(uint32_t values, MaskedTile<D, 
 }
 
 // Writes what an item's sums are where a value that a column sees is not finite, over what the warp has just written of the item: parts (part: [columns][D + 1]),
-// sums beside a prefix or outputs.  In a function of its own and through memory, so that the sums' registers are not kept for it.
+// sums beside a prefix or outputs (which stay NaN where the sum of weights l is).  In a function of its own and through memory, so that the sums' registers are not kept for it.
 template <int D, int NH, class E>
-__device__ __noinline__ void put_infinities(const PagedAttentionArgs& a, float* part, int source, int head, int row, int f0, int width, int from, int to, Range k0, Range k1, Range k2, Range k3) {
+__device__ __noinline__ void put_infinities(const PagedAttentionArgs& a, float* part, int source, int head, int row, int f0, int width, int from, int to, Range k0, Range k1, Range k2, Range k3,
+                                           float l0, float l1, float l2, float l3) {
     const PagedArgs& c = a.c;
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int32_t* table = source == 0 ? c.prefix_table : c.table + (size_t)(source - 1) * c.table_stride;
     Infinite<2 * NH> found;
     found.seen[0] = k0;
     found.seen[1] = k1;
+    const float l[4] = {l0, l1, l2, l3};
     if constexpr (NH == 2) { found.seen[2] = k2; found.seen[3] = k3; }
     __syncwarp();
     for (int x = 0; x < D; x += 32) {
@@ -116,7 +118,7 @@ __device__ __noinline__ void put_infinities(const PagedAttentionArgs& a, float* 
                 const float v = found.sum(col, e, 0.f);
                 if (part) part[f * (D + 1) + x + e] = v;
                 else if (a.whole_o) a.whole_o[(((source == 0 ? (size_t)c.rows : 0) + row + i) * c.n_q + out_head) * D + x + e] = v;
-                else static_cast<E*>(a.out)[(size_t)(row + i) * a.out_stride + out_head * D + x + e] = round_to<E>(v);
+                else if (l[col] == l[col]) static_cast<E*>(a.out)[(size_t)(row + i) * a.out_stride + out_head * D + x + e] = round_to<E>(v);
             }
         }
     }
@@ -581,7 +583,7 @@ __global__ void __launch_bounds__(kWarps<D> * 32, 1) paged_narrow_kernel(const _
             const int first = of.lo / kTile;
             put_infinities<D, NH, E>(a, before ? fronts + warp * C * (D + 1) : behind ? reinterpret_cast<float*>(ring) : nullptr, item.source, item.head, seq.row, f0, width,
                                      max((first + max(begin - item_at, 0)) * kTile, of.lo), min((first + min(end - item_at, item.steps)) * kTile, of.hi), keys[0][0], keys[0][1],
-                                     keys[NH - 1][0], keys[NH - 1][1]);
+                                     keys[NH - 1][0], keys[NH - 1][1], l_run[0][0], l_run[0][1], l_run[NH - 1][0], l_run[NH - 1][1]);
         }
     }
     cp_async_wait<0>();

@@ -432,3 +432,31 @@ def test_two_contexts_side_by_side(ctx):
         del sides
     finally:
         other.close()
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("n_q,n_kv,dim,rows", [(2, 2, 64, 1), (8, 2, 128, 2), (4, 1, 256, 2), (8, 2, 64, 40), (16, 1, 256, 9)])
+@pytest.mark.parametrize("prefix", [0, 50])
+@pytest.mark.parametrize("length", [20, 900])
+def test_scores_that_are_not_numbers_beside_infinite_values(ctx, kind, n_q, n_kv, dim, rows, prefix, length):
+    """A key that is not a number makes NaN of every output of the rows that see it, infinite values or not; the other rows do not notice."""
+    g = np.random.default_rng(dim + rows)
+    b = cases.Batch(g, [rows, 1], [rows + length, 30], 16, n_kv, dim, prefix=prefix)
+    k, v, tokens = b.fill(g, 0.0)
+    q = cases.rounded(g.standard_normal((b.total, n_q, dim)), kind)
+    clean = Device(ctx, b, kind, n_q, k, v).attend(q, 0.1)
+    for t in (length // 2, length // 2 + 7):
+        p, i = b.place(0, t)
+        v[p, :, i, 3], v[p, :, i, dim - 1] = np.inf, -np.inf
+    p, i = b.place(0, 2)
+    k[p, 0, i, 5] = np.nan
+    got = Device(ctx, b, kind, n_q, k, v).attend(q, 0.1)
+    ratio = n_q // n_kv
+    assert np.isnan(got[:rows, :ratio]).all() and np.array_equal(got[rows:], clean[rows:])
+    other = got[:rows, ratio:]
+    assert (other[..., 3] == np.inf).all() and (other[..., dim - 1] == -np.inf).all()
+    rest = [d for d in range(dim) if d not in (3, dim - 1)]
+    # a key whose values are not finite is added apart where not every column sees it, so these are not the clean call's bits: two sums of the same
+    # terms in another order, each within the bound of the one in 64 bits
+    want, size, reach = cases.attend(b, [cases.rounded(t, kind) for t in tokens], q, np.float32(0.1))
+    assert (np.abs(other - want[:rows, ratio:]) <= cases.attend_bound(want, size, reach, kind, dim)[:rows, ratio:])[..., rest].all()
