@@ -897,7 +897,8 @@ SMELT_CUDA_API smelt_status smelt_cuda_paged_attention(smelt_cuda_ctx* ctx, cons
  * T = temperature[s] (null: 1); 0 or less takes the lowest index of the largest logit and accepts drafts that are it.
  * Logits of -inf or NaN have no chance; a drafted id outside the vocabulary falls.
  * Whether a draft stands is judged with fp32 sums: u q(x) within about 1e-6 of p(x), relative, may fall either way.  What is drawn goes by
- * fp64 weights and sums; a whole of max(p - q, 0) below 1e-12 is what equal chances differ by, and counts as nothing.
+ * fp64 weights and sums; a whole of max(p - q, 0) below 1e-12 is what equal chances differ by, and counts as nothing, and so does a
+ * chance below 1e-299 of the largest.
  * row_start is read on the device: where it may give a sequence more drafts than `draft` has steps, draft_steps says how many there
  * are, and the drafts behind them are not judged: the token behind the last judged one that stands is drawn from p of its row.
  * Leaves out_tokens[row_start[s] + i] = the accepted drafts, the drawn token (-1 where no token has a chance), then -1, and accepted[s]. */
